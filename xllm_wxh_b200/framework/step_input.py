@@ -77,5 +77,21 @@ class StepInput:
         return self.fwd_type == FWD_DECODE
 
 
+class TreeStep:
+    """Step input whose sequences bring trees of drafted tokens, built on the device: `rows` from `ops.step_rows` with parents, the
+    rows' tokens, and bounds of the rows and of the cached tokens of a sequence.  Models whose layers attend through
+    `ops.paged_attention` run on it (eagerly or captured: every launch is sized by these bounds); their logits are of all rows."""
+
+    def __init__(self, tokens: torch.Tensor, rows, block_size: int, max_q: int, max_kv: int):
+        self.tokens = tokens
+        self.positions, self.slots, self.token_seq, self.q_cu, self.kv_lens, self.block_tables, self.tree = rows
+        if self.tree is None:
+            raise ValueError("rows of a tree step come from step_rows with parents")
+        self.n_tokens = self.T = tokens.shape[0]
+        self.n_seqs = self.B = self.kv_lens.shape[0]
+        self.block_size, self.max_q, self.max_kv = block_size, max_q, max_kv
+        self.sample_idx = None
+
+
 def make_layout(T_cap: int, B_cap: int, MB_cap: int, S_cap: int, P_cap: int = 0) -> "_core.BatchLayout":
     return _core.BatchLayout(max(T_cap, 1), max(B_cap, 1), max(MB_cap, 1), max(S_cap, 1), max(P_cap, 32))

@@ -12,6 +12,11 @@ def _cuda():
     return cuda_ops
 
 
+def _no_tree(inp):
+    if getattr(inp, "tree", None) is not None:
+        raise NotImplementedError("trees of drafted tokens run on `paged_attention` layers only")
+
+
 def rms_norm(x, w, eps):
     return _cuda().rms_norm(x, w, eps) if x.is_cuda else ref.rms_norm(x, w, eps)
 
@@ -38,7 +43,10 @@ def rope_qknorm_kvwrite(qkv, positions, slots, cos_sin, q_w, k_w, eps, k_cache, 
 
 
 def paged_attention(q, k_cache, v_cache, inp, scale, sliding_window=-1):
-    """q [T, Hq, D]; `inp` is a StepInput (q_cu, kv_lens, block_tables, n_seqs, n_decode ...)."""
+    """q [T, Hq, D]; `inp` is a StepInput (q_cu, kv_lens, block_tables, n_seqs, n_decode ...).  The rows of a TreeStep see their
+    ancestors only (`tree_attention`)."""
+    if getattr(inp, "tree", None) is not None:
+        return tree_attention(q, k_cache, v_cache, inp, inp.tree, scale, sliding_window)
     if q.is_cuda:
         return _cuda().paged_attention(q, k_cache, v_cache, inp, scale, sliding_window)
     return ref.paged_attention(q, k_cache, v_cache, inp.q_cu, inp.kv_lens, inp.block_tables, inp.n_seqs, scale,
@@ -55,6 +63,7 @@ def paged_attention_ext(q, k_cache, v_cache, inp, scale, window=-1, chunk=0, slo
     heads has one value head's values, and its output is rms(first - factor * second) * mult: [T, Hq / 2 * dv].
     `bound` > 0 promises |q . k| <= bound (normed queries and keys), which saves the kernels a check of bounded scores.
     k_cache may have one key head beside several value heads: all query heads then share it (queries of `mix_query_heads`)."""
+    _no_tree(inp)
     if q.is_cuda:
         return _cuda().paged_attention_ext(q, k_cache, v_cache, inp, scale, window, chunk, slopes, sinks, keep_first, softcap, mix, bound)
     return ref.paged_attention(q, k_cache, v_cache, inp.q_cu, inp.kv_lens, inp.block_tables, inp.n_seqs, scale, window, chunk,
@@ -314,6 +323,155 @@ def rotate_into(x, rot, out):
     (_cuda() if x.is_cuda else ref).rotate_into(x, rot, out)
 
 
+# ----------------------------------------------------------------------------- steps with trees of drafted tokens
+TREE_MAX_ROWS = ref.TREE_MAX_ROWS
+StepRows = ref.StepRows
+
+
+def _tree():
+    from . import tree_cuda
+    return tree_cuda
+
+
+def _like(t, dtype, shape, device, name):
+    """Checks one argument: element type, sizes (None: any), dense, on the same device."""
+    import torch
+    assert isinstance(t, torch.Tensor) and t.dtype == dtype, f"{name}: a tensor of {dtype}"
+    assert t.dim() == len(shape) and all(n is None or n == m for n, m in zip(shape, t.shape)), f"{name}: shape {tuple(t.shape)}, not {shape}"
+    assert t.is_contiguous() and t.device == device, f"{name}: contiguous, on {device}"
+
+
+def step_rows(tables, lens, seqs, counts, n_rows, block_size, parents=None, max_q=None, max_blocks=None):
+    """The maps of a step whose lengths are on the device: sequence b adds counts[b] rows behind the lens[seqs[b]] tokens that row
+    seqs[b] of the pool holds.  tables [pool, blocks], lens [pool], seqs, counts [B], int32.
+    Row i of a sequence goes to cache position len + i.  Without `parents` the rows follow one another; with `parents` (int32
+    [n_rows]: each row's predecessor as a number among its sequence's rows, below its own; anything else: it follows the cached
+    tokens) they form trees, a row's position counts its ancestors, and `tree` holds these and the row itself, 64 to a word.
+    n_rows: rows of the outputs, at least the sum of counts; rows behind the last sequence have position 0, sequence -1 and a slot in
+    the reserved block 0.  max_q bounds counts (trees: at most 256); max_blocks: columns of the new tables (all), unused ones 0.
+    Sequences outside the pool (padding: -1) add nothing.  Returns StepRows (positions, slots, token_seq, q_cu, kv_lens,
+    block_tables, tree)."""
+    import torch
+    dev, i32 = tables.device, torch.int32
+    assert tables.dim() == 2 and tables.dtype == i32 and (tables.stride(1) == 1 or tables.shape[1] <= 1), "tables: int32 [pool, blocks]"
+    pool, B = tables.shape[0], seqs.numel()
+    _like(lens, i32, (pool,), dev, "lens")
+    _like(seqs, i32, (B,), dev, "seqs")
+    _like(counts, i32, (B,), dev, "counts")
+    max_q = max(1, n_rows) if max_q is None else max_q
+    max_blocks = tables.shape[1] if max_blocks is None else max_blocks
+    assert n_rows >= 0 and block_size >= 1 and max_q >= 1 and 0 <= max_blocks <= tables.shape[1] and B < 65535
+    if parents is not None:
+        _like(parents, i32, (n_rows,), dev, "parents")
+        assert max_q <= TREE_MAX_ROWS, f"trees have at most {TREE_MAX_ROWS} rows a sequence: give max_q"
+    f = _tree().step_rows if tables.is_cuda else ref.step_rows
+    return f(tables, lens, seqs, counts, n_rows, block_size, parents, max_q, max_blocks)
+
+
+def tree_attention(q, k_cache, v_cache, inp, tree, scale, sliding_window=-1):
+    """Attention of rows that see their sequence's cached tokens ahead of the step and those of its own rows whose bit is set in `tree`
+    (int64 [T, words], as `step_rows` makes it; any set of a sequence's first 64 x words rows will do).  q [T, Hq, D], caches [blocks,
+    block, Hkv, D] that hold the step's rows already; `inp` has q_cu, kv_lens, block_tables, token_seq, positions, n_seqs, and max_q and
+    max_kv as bounds.  `sliding_window`: only keys at positions above the row's own - window.  Rows that see nothing and rows of no
+    sequence are zero.  Returns [T, Hq * D].  bf16 or fp32, up to 512 columns a head."""
+    import torch
+    T, Hq, D = q.shape
+    assert q.dtype in (torch.bfloat16, torch.float32) and k_cache.dtype == v_cache.dtype == q.dtype, "q and caches: one type, bf16 or fp32"
+    assert k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.shape[3] == D and D <= 512, "caches: [blocks, block, Hkv, D]"
+    assert Hq % k_cache.shape[2] == 0 and k_cache.is_contiguous() and v_cache.is_contiguous()
+    dev, i32, B = q.device, torch.int32, inp.n_seqs
+    assert k_cache.device == v_cache.device == dev
+    assert tree.dim() == 2 and 1 <= tree.shape[1] <= TREE_MAX_ROWS // 64, "tree: one to four words a row"
+    _like(tree, torch.int64, (T, None), dev, "tree")
+    _like(inp.q_cu, i32, (B + 1,), dev, "q_cu")
+    _like(inp.kv_lens, i32, (B,), dev, "kv_lens")
+    _like(inp.block_tables, i32, (B, None), dev, "block_tables")
+    _like(inp.token_seq, i32, (T,), dev, "token_seq")
+    _like(inp.positions, i32, (T,), dev, "positions")
+    f = _tree().tree_attention if q.is_cuda else ref.tree_attention
+    return f(q, k_cache, v_cache, inp, tree, float(scale), int(sliding_window))
+
+
+def adjust_logits(logits, q_cu, seqs=None, history=None, penalties=None, tokens=None, parents=None, bias=None, mask=None, max_q=None):
+    """Penalties, biases and grammar masks on logits [S, V] (fp32 or bf16), in place.  Sequence b owns rows q_cu[b] .. q_cu[b + 1] - 1
+    and reads row seqs[b] of the per-request tensors (None: row b; outside the pool: nothing is changed but by masks).
+    history = (ids int32 [pool, cap], lens [pool], prompt_lens [pool]) with penalties = (repetition, frequency, presence), fp32 [pool]:
+    for every id among the lens[p] first ones, made of them behind the prompt: x -= made * frequency + (made > 0) * presence, then
+    x * repetition below 0, else x / repetition.  With `tokens` (int32 [S]) a row's own token and those of the rows ahead of it follow the
+    lens[p] first ones: with `parents` (as in `step_rows`) its ancestors', without all earlier rows' of the sequence.  At most 256 rows a
+    sequence then; rows past max_q of a sequence are left as they are.
+    bias = (cu int32 [pool + 1], ids int32, values fp32): added; the last entry of an id holds.
+    mask = (words int32 [masks, >= V / 32], rows int32 [S]): ids whose bit is 0 in the row's mask become -inf (rows: -1 for none).
+    Ids outside the vocabulary are passed over.  Returns logits."""
+    import torch
+    S, V = logits.shape
+    dev, i32, f32 = logits.device, torch.int32, torch.float32
+    assert logits.dtype in (f32, torch.bfloat16) and (logits.stride(1) == 1 or V == 1) and (logits.stride(0) >= V or S <= 1), "logits: fp32 or bf16 rows"
+    assert q_cu.numel() >= 1
+    _like(q_cu, i32, (None,), dev, "q_cu")
+    B = q_cu.numel() - 1
+    pool = None
+    if history is not None:
+        ids, lens, prompts = history
+        pool = lens.numel()
+        assert ids.dtype == i32 and ids.dim() == 2 and ids.shape[0] == pool and (ids.stride(1) == 1 or ids.shape[1] <= 1) and ids.device == dev, \
+            "history: int32 [pool, cap]"
+        _like(lens, i32, (pool,), dev, "lens")
+        _like(prompts, i32, (pool,), dev, "prompt_lens")
+        assert penalties is not None and len(penalties) == 3, "history needs (repetition, frequency, presence)"
+        for t, name in zip(penalties, ("repetition", "frequency", "presence")):
+            _like(t, f32, (pool,), dev, name)
+    else:
+        assert penalties is None and tokens is None, "penalties and tokens need a history"
+    if tokens is not None:
+        _like(tokens, i32, (S,), dev, "tokens")
+    if parents is not None:
+        assert tokens is not None, "parents need tokens"
+        _like(parents, i32, (S,), dev, "parents")
+    if bias is not None:
+        cu, ids, values = bias
+        _like(cu, i32, (None,) if pool is None else (pool + 1,), dev, "bias cu")
+        pool = cu.numel() - 1
+        _like(ids, i32, (None,), dev, "bias ids")
+        _like(values, f32, (ids.numel(),), dev, "bias values")
+    if seqs is not None:
+        _like(seqs, i32, (B,), dev, "seqs")
+    if mask is not None:
+        words, rows = mask
+        assert words.dim() == 2 and words.dtype == i32 and words.stride(1) == 1 and words.shape[1] * 32 >= V and words.device == dev, \
+            "mask: int32 [masks, V / 32]"
+        _like(rows, i32, (S,), dev, "mask rows")
+    max_q = max(1, S) if max_q is None else max_q
+    assert max_q >= 1 and (tokens is None or max_q <= TREE_MAX_ROWS), f"at most {TREE_MAX_ROWS} rows a sequence with tokens: give max_q"
+    f = _tree().adjust_logits if logits.is_cuda else ref.adjust_logits
+    return f(logits, q_cu, seqs, history, penalties, tokens, parents, bias, mask, max_q)
+
+
+def accept_tree(target, inp, parents, caches=(), max_depth=None):
+    """The drafted tokens that the target model agrees with.  target [T] is the target's own token behind every row, inp.tokens the rows'
+    tokens, parents as in `step_rows`; row 0 of a sequence is its last token, which counts as agreed.  From there the path goes to the
+    first row that follows with the target's token, up to max_depth rows (default: inp.max_q - 1).  Returns (out [B, max_depth + 1]: the
+    target's tokens along the path, then -1; accepted [B]: drafted rows on the path; path [B, max_depth + 1]: their numbers, then -1).
+    In every tensor of `caches` ([blocks, block, ...], contiguous, no tensor twice) the path's rows move to the positions behind the
+    sequence's earlier tokens, which then has 1 + accepted more; the other drafted rows' places hold what they held."""
+    import torch
+    T, dev, i32, B = target.numel(), target.device, torch.int32, inp.n_seqs
+    _like(target, i32, (T,), dev, "target")
+    _like(inp.tokens, i32, (T,), dev, "tokens")
+    _like(parents, i32, (T,), dev, "parents")
+    _like(inp.q_cu, i32, (B + 1,), dev, "q_cu")
+    _like(inp.kv_lens, i32, (B,), dev, "kv_lens")
+    _like(inp.block_tables, i32, (B, None), dev, "block_tables")
+    assert inp.max_q <= TREE_MAX_ROWS, f"trees have at most {TREE_MAX_ROWS} rows a sequence"
+    depth = max(0, inp.max_q - 1) if max_depth is None else max_depth
+    assert 0 <= depth < TREE_MAX_ROWS and B < 65536
+    for c in caches:
+        assert c.dim() >= 2 and c.shape[1] == inp.block_size and c.is_contiguous() and c.device == dev, "caches: [blocks, block, ...], contiguous"
+    assert len({c.data_ptr() for c in caches if c.numel()}) == sum(c.numel() > 0 for c in caches), "a cache may be named once"
+    f = _tree().accept_tree if target.is_cuda else ref.accept_tree
+    return f(target, inp, parents, caches, depth)
+
+
 # ----------------------------------------------------------------------------- MLA (DeepSeek)
 def mla_prepare(q, kv_a, positions, slots, cos_sin, kv_norm_w, eps, cache, w_kc, nope, rope, kv_lora):
     """Latent RMSNorm + interleaved RoPE of k_pe -> one [kv_lora + rope] cache row per token; RoPE of q_pe; q_nope absorbed
@@ -333,6 +491,7 @@ def mla_prepare(q, kv_a, positions, slots, cos_sin, kv_norm_w, eps, cache, w_kc,
 
 
 def mla_attention(q_lat, q_pe, cache, inp, scale, kv_lora):
+    _no_tree(inp)
     if q_lat.is_cuda:
         return _cuda().mla_attention(q_lat, q_pe, cache, inp, scale, kv_lora)
     return ref.mla_attention(q_lat, q_pe, cache, inp.q_cu, inp.kv_lens, inp.block_tables, inp.n_seqs, scale, kv_lora)

@@ -10,7 +10,7 @@ RoPE (fused_qknorm_rope.cu:75-280), paged cache write (reshape_paged_cache.cu:23
 from __future__ import annotations
 
 import math
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -765,3 +765,175 @@ def linear_fp8_scaled(xq, xs, wq, col_scale=None, tensor_scale: float = 1.0, bia
     if bias is not None:
         y = y + bias.float()
     return y.to(out_dtype)
+
+
+# ----------------------------------------------------------------------------- steps with trees of drafted tokens
+TREE_MAX_ROWS = 256          # rows of one sequence that can form a tree
+
+
+class StepRows(NamedTuple):
+    """What a step's rows need to run: see `ops.step_rows`."""
+    positions: torch.Tensor
+    slots: torch.Tensor
+    token_seq: torch.Tensor
+    q_cu: torch.Tensor
+    kv_lens: torch.Tensor
+    block_tables: torch.Tensor
+    tree: Optional[torch.Tensor]
+
+
+def _tree_lines(parents):
+    """For each row of one sequence the rows from itself up to the root; only an earlier row can be followed."""
+    lines = []
+    for i, up in enumerate(parents):
+        lines.append([i] + (lines[up] if 0 <= up < i else []))
+    return lines
+
+
+def _signed(words: int) -> int:
+    return words - (1 << 64) if words >> 63 else words
+
+
+def step_rows(tables, lens, seqs, counts, n_rows: int, block_size: int, parents, max_q: int, max_blocks: int) -> StepRows:
+    B, pool = seqs.numel(), tables.shape[0]
+    words = 0 if parents is None else -(-max_q // 64)
+    positions = torch.zeros(n_rows, dtype=torch.int32)
+    slots = (torch.arange(n_rows) % block_size).int()
+    token_seq = torch.full((n_rows,), -1, dtype=torch.int32)
+    q_cu = torch.zeros(B + 1, dtype=torch.int32)
+    kv_lens = torch.zeros(B, dtype=torch.int32)
+    out = torch.zeros(B, max_blocks, dtype=torch.int32)
+    tree = None if parents is None else torch.zeros(n_rows, words, dtype=torch.int64)
+    up = None if parents is None else parents.tolist()
+    at = 0
+    for b, (src, n) in enumerate(zip(seqs.tolist(), counts.tolist())):
+        held = 0 <= src < pool
+        want = min(max(n, 0), max_q) if held else 0
+        n = min(want, n_rows - at)
+        before = max(int(lens[src]), 0) if held else 0
+        used = min(max_blocks, -(-(before + want) // block_size))
+        if held:
+            out[b, :used] = tables[src, :used]
+        lines = _tree_lines(up[at:at + n]) if up is not None else None
+        for i in range(n):
+            p = before + i
+            positions[at + i] = before + (len(lines[i]) - 1 if lines else i)
+            if p // block_size < tables.shape[1]:
+                slots[at + i] = int(tables[src, p // block_size]) * block_size + p % block_size
+            token_seq[at + i] = b
+            if lines:
+                bits = sum(1 << j for j in lines[i])
+                for w in range(words):
+                    tree[at + i, w] = _signed(bits >> 64 * w & (1 << 64) - 1)
+        at += n
+        q_cu[b + 1] = at
+        kv_lens[b] = before + n
+    return StepRows(positions, slots, token_seq, q_cu, kv_lens, out, tree)
+
+
+def tree_attention(q, k_cache, v_cache, inp, tree, scale: float, window: int) -> torch.Tensor:
+    T, Hq, D = q.shape
+    block, Hkv = k_cache.shape[1], k_cache.shape[2]
+    out = torch.zeros(T, Hq, D, dtype=q.dtype)
+    cu = inp.q_cu.tolist()
+    for i in range(inp.n_seqs):
+        a, n, L = cu[i], cu[i + 1] - cu[i], int(inp.kv_lens[i])
+        if n <= 0 or L <= 0:
+            continue
+        blocks = inp.block_tables[i, :-(-L // block)].long()
+        k = k_cache.index_select(0, blocks).reshape(-1, Hkv, D)[:L].float()
+        v = v_cache.index_select(0, blocks).reshape(-1, Hkv, D)[:L].float()
+        pos = inp.positions[a:a + n].long()
+        base = L - n
+        see = torch.zeros(n, L, dtype=torch.bool)
+        see[:, :base] = True
+        for j in range(min(n, 64 * tree.shape[1])):
+            see[:, base + j] = (tree[a:a + n, j // 64] >> (j % 64) & 1).bool()
+        if window > 0:
+            see &= torch.cat([torch.arange(base), pos])[None] > pos[:, None] - window
+        s = torch.einsum("nhd,lhd->hnl", q[a:a + n].float(), k.repeat_interleave(Hq // Hkv, 1)) * scale
+        s = s.masked_fill(~see[None], float("-inf"))
+        top = s.amax(-1, keepdim=True)
+        e = (s - torch.where(top == float("-inf"), torch.zeros_like(top), top)).exp()
+        total = e.sum(-1, keepdim=True)
+        e = torch.where(total == 0, torch.zeros_like(e), e / total)
+        # values behind a mask do not enter, whatever they are
+        v = v.repeat_interleave(Hq // Hkv, 1)
+        o = torch.einsum("hnl,lhd->nhd", e, torch.nan_to_num(v, 0.0, 0.0, 0.0))
+        for j in (~v.isfinite()).flatten(1).any(1).nonzero().flatten().tolist():
+            o = torch.where(see[:, j, None, None] & ~v[j][None].isfinite(), o + v[j][None], o)
+        out[a:a + n] = o.to(q.dtype)
+    return out.flatten(1)
+
+
+def adjust_logits(logits, q_cu, seqs, history, penalties, tokens, parents, bias, mask, max_q: int) -> torch.Tensor:
+    S, V = logits.shape
+    cu = q_cu.tolist()
+    words, mask_of = mask if mask is not None else (None, None)
+    pool = history[1].numel() if history is not None else bias[0].numel() - 1 if bias is not None else len(cu) - 1
+    forbidden = {}
+    if mask is not None:
+        for r, m in enumerate(mask_of.tolist()):
+            if 0 <= m < words.shape[0]:
+                bits = words[m].long()[:, None] >> torch.arange(32)[None] & 1
+                forbidden[r] = (bits.reshape(-1)[:V] == 0).nonzero().flatten()
+    for b in range(len(cu) - 1):
+        src = b if seqs is None else int(seqs[b])
+        a, n = cu[b], min(cu[b + 1], S) - cu[b]
+        if not 0 <= src < pool or n <= 0:
+            continue
+        n = min(n, max_q)
+        if history is not None:
+            text, lens, prompts = history
+            rep, freq, pres = (float(t[src]) for t in penalties)
+            ids = text[src, :min(max(int(lens[src]), 0), text.shape[1])].tolist()
+            path = tokens[a:a + n].tolist() if tokens is not None else None
+            lines = _tree_lines(parents[a:a + n].tolist() if parents is not None else list(range(-1, n - 1)))
+        add = {}
+        if bias is not None:
+            for e in range(int(bias[0][src]), int(bias[0][src + 1])):
+                add[int(bias[1][e])] = float(bias[2][e])           # the last entry of an id holds
+        for r in range(n):
+            x = logits[a + r].float()
+            if history is not None:
+                mine = [path[j] for j in reversed(lines[r])] if path is not None else []
+                seen = ids + mine
+                made = ids[max(int(prompts[src]), 0):] + mine[max(int(prompts[src]) - max(int(lens[src]), 0), 0):]
+                for i in {i for i in seen if 0 <= i < V}:
+                    c = made.count(i)
+                    y = x[i] - c * freq - (pres if c > 0 else 0.0)
+                    x[i] = y * rep if y < 0 else y / rep
+            for i, v in add.items():
+                if 0 <= i < V:
+                    x[i] += v
+            logits[a + r] = x.to(logits.dtype)
+    for r, ids in forbidden.items():
+        logits[r, ids] = float("-inf")
+    return logits
+
+
+def accept_tree(target, inp, parents, caches, depth: int):
+    B, block = inp.n_seqs, inp.block_size
+    out = torch.full((B, depth + 1), -1, dtype=torch.int32)
+    path = torch.full((B, depth + 1), -1, dtype=torch.int32)
+    accepted = torch.zeros(B, dtype=torch.int32)
+    cu, up, tok, want = inp.q_cu.tolist(), parents.tolist(), inp.tokens.tolist(), target.tolist()
+    for b in range(B):
+        a, n = cu[b], cu[b + 1] - cu[b]
+        rows = [0] if n > 0 else []
+        while rows and len(rows) <= depth:
+            at = rows[-1]
+            nxt = [j for j in range(at + 1, n) if up[a + j] == at and tok[a + j] == want[a + at]]
+            if not nxt:
+                break
+            rows.append(nxt[0])
+        for i, j in enumerate(rows):
+            out[b, i], path[b, i] = want[a + j], j
+        accepted[b] = max(len(rows) - 1, 0)
+        base = int(inp.kv_lens[b]) - n
+        place = lambda p: (int(inp.block_tables[b, p // block]), p % block)
+        for i, j in enumerate(rows):
+            (b1, o1), (b0, o0) = place(base + i), place(base + j)
+            for c in caches:
+                c[b1, o1] = c[b0, o0]
+    return out, accepted, path

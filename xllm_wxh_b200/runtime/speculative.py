@@ -279,19 +279,20 @@ class SpeculativeEngine(LLMEngine):
         if k == 1:
             return first
         B = first.shape[0]
-        seq = inp.token_seq.index_select(0, seq_rows).long()                 # index of each sequence in the step's tables
-        bt = inp.block_tables.index_select(0, seq)
+        seq = inp.token_seq.index_select(0, seq_rows)                        # index of each sequence in the step's tables
         bs = inp.block_size
+        lens = torch.zeros(inp.block_tables.shape[0], dtype=torch.int32, device=first.device)
+        lens.index_copy_(0, seq.long(), pos.int())
+        one = torch.ones_like(seq)
         out = [first]
         tok, h = first, hidden
-        arange = torch.arange(B + 1, dtype=torch.int32, device=first.device)
         for j in range(1, k):
-            p = (pos + (j - 1)).long()
-            slot = bt.gather(1, (p // bs).view(B, 1)).view(B).long() * bs + p % bs
-            mini = _DraftRows(tok, p.int(), slot.int(), arange, (p + 1).int(), bt, bs, inp.layout.MB_cap, max_kv=inp.max_kv + j)
+            r = ops.step_rows(inp.block_tables, lens, seq, one, B, bs, max_q=1)
+            mini = _DraftRows(tok, r.positions, r.slots, r.q_cu, r.kv_lens, r.block_tables, bs, inp.layout.MB_cap, max_kv=inp.max_kv + j)
             h = self.draft.forward_mtp(mini, self.draft_kv, h)
             tok = self._propose(h, None)
             out.append(tok)
+            lens += 1
         return torch.stack(out, 1).reshape(-1)
 
     # ------------------------------------------------------------------ rank 0
