@@ -3,6 +3,7 @@
 //
 // The fp32-pipe kernel serves every type and size: one warp per (row, query head), 32 keys at a time, one key per lane for the scores, then
 // one slice of the value columns per lane for the weighted sum, with a running maximum and sum.
+#include "attention_tc.cuh"
 #include "vec8.cuh"
 
 namespace xl_at {
@@ -95,12 +96,691 @@ __global__ void __launch_bounds__(128) attention_tree_simt_kernel(const Params p
     if (c * 32 + lane < p.D) from_f32(out + c * 32 + lane, acc[c] * inv);
 }
 
+// ---------------------------------------------------------------- tensor-core kernel
+// bf16, up to 128 columns a head.  A key head's query heads times a tree's nodes are the rows of one product: 128 rows (TMEM lanes) take in
+// 128 / G nodes of G heads each, so that a key is read once for all of them (PAIR: for 256 rows).  Reading K and V bounds the kernel up to
+// about 256 rows; above, exponentials and products do.
+//
+//   work      : the key tiles (64 keys) of every (sequence, key head, rows) one behind the other, cut into equal stretches, one per CTA
+//               (one CTA per SM): ragged lengths leave no SM idle.  A stretch begins and ends anywhere; the at most two pieces of it
+//               that are not whole leave fp32 partials (sums, maximum, denominator) that the merge kernel joins.
+//   warp 0    : TMA producer - query rows of a piece (box: 64 columns x G heads x nodes), then a ring of units in the order of use, each
+//               64 tokens of K or of V through the block table;
+//   warp 1    : MMA issuer   - S = Q K^T (128 x 64 x D, fp32 in TMEM, two buffers a group), O += P V;
+//   warps 2-5 and 6-9: two softmax groups, one row per thread: running maximum and sum in the log2 domain, P as bf16 through shared
+//               memory, O rescaled only when the maximum grew by more than 2^8.
+//               PAIR: each group has 128 rows of its own, both read the same keys.  Otherwise the groups take the key tiles in turn
+//               for the same rows, each with its own O, and join at the end of a piece: a single group could not keep up with memory.
+//
+// Masks: keys ahead of the tree are seen by all rows (within the window), the tree's by the row's words; only tiles that hold either
+// border look at them.  There, values behind the last row are cleared, and values that are not finite are taken out of the tile and
+// added to the rows that do see them, so that whatever stands in a masked place reaches no other row.
+// Every wait is bounded; on expiry the kernel records a status code and leaves.
+constexpr int BQ = 128, BKV = 64;
+constexpr int kTcThreads = 320;
+constexpr int Q_SLAB = BQ * 128, KV_SLAB = BKV * 128, P_BYTES = BQ * BKV * 2;
+constexpr int kMaxUnits = 16;
+struct TcBarriers {
+  uint64_t full[kMaxUnits], empty[kMaxUnits];
+  uint64_t q_full, q_empty;
+  uint64_t s_full[2][2], s_free[2][2];                       // [group][buffer]
+  uint64_t p_full[2], pv_done[2];
+  uint32_t tmem_base;
+  int seq, any_bad[4];
+  long seq_tiles;                                            // tiles ahead of `seq`
+  long part[kTcThreads / 32];
+  uint32_t bad[4][2][16][2];                                 // [piece & 3][group][tile][key]: keys whose values are not all finite
+  float2 ml[2][BQ];
+};
+
+template <int QS, bool PAIR> struct Cfg {
+  static constexpr int DV = 64 * QS;                         // padded columns
+  static constexpr int Q_BYTES = QS * Q_SLAB, UNIT = QS * KV_SLAB, NQ = PAIR ? 2 : 1;
+  static constexpr int kFit = (227 * 1024 - int(sizeof(TcBarriers)) - NQ * Q_BYTES - 2 * P_BYTES) / UNIT;
+  static constexpr int U = kFit < kMaxUnits ? kFit : kMaxUnits;
+  static constexpr int LAG = PAIR ? 1 : 2;                   // S of a tile is issued ahead of P V of the tile LAG before it
+  static constexpr int kSmem = NQ * Q_BYTES + U * UNIT + 2 * P_BYTES + int(sizeof(TcBarriers));
+  static_assert(U >= 6 && kSmem <= 227 * 1024, "a piece's next units fit the ring");
+  static constexpr int kRows = PAIR ? 256 : 128;
+};
+
+struct TcParams {
+  Params a;
+  int group, nodes;             // query heads per key head, nodes of one row tile
+  int box_tokens, min_tiles;
+  float scale_log2;
+  float4* ws_o;                 // [2 * CTA + which][D / 4][rows]
+  float2* ws_ml;                // [2 * CTA + which][rows]: (maximum in the log2 domain, sum)
+  int* ws_desc;                 // [CTA][8]
+  int* status;
+};
+enum { DESC_MERGE, DESC_FIRST, DESC_SLOT, DESC_START, DESC_NODES, DESC_HEAD };   // of the item that ends in a CTA's first piece
+
+struct Seq {
+  int q_start, n, kv_len, base, kv_begin, row_tiles, key_tiles;
+  __device__ __forceinline__ long tiles(int n_kv) const { return long(row_tiles) * key_tiles * n_kv; }
+};
+__device__ __forceinline__ Seq load_seq(const Params& p, int s, int per_item) {
+  Seq q;
+  q.q_start = p.q_cu[s];
+  q.n = min(p.q_cu[s + 1], p.T) - q.q_start;
+  q.kv_len = min(long(p.kv_lens[s]), long(p.max_blocks) * p.block_size);
+  q.base = max(q.kv_len - q.n, 0);
+  q.kv_begin = p.window > 0 ? max(0, q.base - p.window + 1) / BKV * BKV : 0;
+  q.row_tiles = q.n > 0 && q.kv_len > 0 ? (q.n + per_item - 1) / per_item : 0;
+  q.key_tiles = (q.kv_len - q.kv_begin + BKV - 1) / BKV;
+  return q;
+}
+
+// The pieces of a CTA's stretch [w, w1) of the tiles; every role walks them by itself.
+struct Walk {
+  Seq q;
+  int seq, head, node0, j0, nt;            // node0: first node of the piece's rows; its key tiles j0 .. j0 + nt - 1
+  long w, w1, ahead;                       // ahead: tiles in front of `seq`
+  __device__ __forceinline__ void start(const TcParams& p, const TcBarriers* b, long w0, long w_end, int per_item) {
+    w = w0;
+    w1 = w_end;
+    seq = b->seq;
+    ahead = b->seq_tiles;
+    q = load_seq(p.a, seq, per_item);
+    nt = 0;
+  }
+  __device__ __forceinline__ bool next(const TcParams& p, int per_item) {
+    w += nt;
+    if (w >= w1) return false;
+    while (w >= ahead + q.tiles(p.a.n_kv)) {
+      ahead += q.tiles(p.a.n_kv);
+      q = load_seq(p.a, ++seq, per_item);
+    }
+    const long at = w - ahead;
+    const int item = int(at / q.key_tiles);
+    j0 = int(at - long(item) * q.key_tiles);
+    nt = int(min(long(q.key_tiles - j0), w1 - w));
+    head = item / q.row_tiles;
+    node0 = item % q.row_tiles * per_item;
+    return true;
+  }
+  __device__ __forceinline__ bool whole() const { return nt == q.key_tiles; }
+  __device__ __forceinline__ int key0(int j) const { return q.kv_begin + (j0 + j) * BKV; }
+  // tiles in which some row may see only a part: the window's border, the tree, the end
+  __device__ __forceinline__ bool partly(const Params& p, int kv0) const {
+    return kv0 + BKV > q.base || (p.window > 0 && kv0 < q.base + q.n - p.window);
+  }
+  __device__ __forceinline__ int tile_number(int kv0) const {        // of such a tile among its piece's (at most 16)
+    return kv0 + BKV > q.base ? min(8 + (kv0 - q.base / BKV * BKV) / BKV, 15) : min((kv0 - q.kv_begin) / BKV, 7);
+  }
+};
+
+// unit (within its piece) of the keys and values of tile j
+template <int LAG> __device__ __forceinline__ int k_unit(int j) { return j < LAG ? j : 2 * j - LAG; }
+template <int LAG> __device__ __forceinline__ int v_unit(int j, int nt) { return j + LAG < nt ? 2 * j + LAG + 1 : nt + j; }
+
+// keys of the tile at kv0 that row t (node of its sequence, at position pos) sees
+__device__ __forceinline__ uint64_t seen_keys(const Params& p, const Seq& q, int t, int pos, int kv0) {
+  const int c = q.base - kv0;
+  uint64_t see = c >= 64 ? ~0ull : c > 0 ? (1ull << c) - 1 : 0;
+  if (p.window > 0) {
+    const int lo = pos - p.window + 1 - kv0;
+    see = lo >= 64 ? 0 : lo > 0 ? see >> lo << lo : see;
+  }
+  if (c < 64) {
+    const unsigned long long* words = p.tree + size_t(t) * p.words;
+    uint64_t bits;
+    if (c >= 0) {
+      bits = words[0] << c;
+    } else {
+      const int i = (-c) >> 6, sh = (-c) & 63;
+      bits = i < p.words ? words[i] >> sh : 0;
+      if (sh && i + 1 < p.words) bits |= words[i + 1] << (64 - sh);
+    }
+    const int end = q.base + q.n - kv0;
+    if (end < 64) bits = end > 0 ? bits & ((1ull << end) - 1) : 0;
+    if (p.window > 0 && pos - p.window >= q.base)
+      for (uint64_t todo = bits; todo; todo &= todo - 1) {
+        const int k = __ffsll(todo) - 1;
+        if (p.positions[q.q_start + kv0 + k - q.base] <= pos - p.window) bits &= ~(1ull << k);
+      }
+    see |= bits;
+  }
+  return see;
+}
+
+__device__ __forceinline__ bool not_finite(uint32_t pair) {
+  return (pair & 0x7F800000u) == 0x7F800000u || (pair & 0x7F80u) == 0x7F80u;
+}
+
+template <int QS, bool PAIR>
+__global__ void __launch_bounds__(kTcThreads, 1)
+attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                         const TcParams p) {
+  using C = Cfg<QS, PAIR>;
+  constexpr int U = C::U, UNIT = C::UNIT, DV = C::DV, LAG = C::LAG;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* sQ = smem;
+  uint8_t* ring = sQ + C::NQ * C::Q_BYTES;
+  uint8_t* sP = ring + U * UNIT;
+  TcBarriers* bars = reinterpret_cast<TcBarriers*>(sP + 2 * P_BYTES);
+  const Params& a = p.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  grid_dep_launch();                                         // the merge kernel may take its place; it waits for this one's end
+  if (smem_u32(smem) & 1023u) {
+    if (tid == 0) atomicExch(p.status, XL_ERR_BOUNDS);
+    return;
+  }
+  // rows of no sequence
+  {
+    const int behind = max(a.q_cu[a.B], 0), width = a.n_q * a.D;
+    for (long t = long(behind) + blockIdx.x; t < a.T; t += gridDim.x)
+      for (int c = tid; c < width / 8; c += kTcThreads) reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + t * width)[c] = make_uint4(0, 0, 0, 0);
+  }
+  // ------------------------------------------------------------ this CTA's stretch of the tiles
+  const int per_item = (PAIR ? 2 : 1) * p.nodes;
+  const int share = (a.B + kTcThreads - 1) / kTcThreads;
+  const int s0 = min(tid * share, a.B), s1 = min(s0 + share, a.B);
+  long mine = 0;
+  for (int s = s0; s < s1; ++s) mine += load_seq(a, s, per_item).tiles(a.n_kv);
+  long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) bars->part[warp] = incl;
+  __syncthreads();
+  long total = 0;
+#pragma unroll
+  for (int i = 0; i < kTcThreads / 32; ++i) {
+    if (i < warp) incl += bars->part[i];
+    total += bars->part[i];
+  }
+  const long ctas = max(1l, min(long(gridDim.x), total / p.min_tiles));
+  const long w0 = blockIdx.x * total / ctas, w1 = (blockIdx.x + 1) * total / ctas;
+  if (long(blockIdx.x) >= ctas || w0 >= w1) {
+    if (tid == 0) p.ws_desc[blockIdx.x * 8 + DESC_MERGE] = 0;
+    return;
+  }
+  if (incl - mine <= w0 && w0 < incl) {
+    long at = incl - mine;
+    for (int s = s0; s < s1; ++s) {
+      const long n = load_seq(a, s, per_item).tiles(a.n_kv);
+      if (w0 < at + n) {
+        bars->seq = s;
+        bars->seq_tiles = at;
+        break;
+      }
+      at += n;
+    }
+  }
+  if (tid == 0) {
+    for (int u = 0; u < U; ++u) {
+      mbar_init(&bars->full[u], 1);
+      mbar_init(&bars->empty[u], 1);
+    }
+    mbar_init(&bars->q_full, 1);
+    mbar_init(&bars->q_empty, 1);
+    for (int g = 0; g < 2; ++g) {
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&bars->s_full[g][b], 1);
+        mbar_init(&bars->s_free[g][b], 4);
+      }
+      mbar_init(&bars->p_full[g], 4);
+      mbar_init(&bars->pv_done[g], 1);
+    }
+    mbar_fence_init();
+  }
+  for (int i = tid; i < 4 * 2 * 16 * 2; i += kTcThreads) (&bars->bad[0][0][0][0])[i] = 0;
+  if (tid < 4) bars->any_bad[tid] = 0;
+  if (warp == 1) {
+    tmem_alloc(&bars->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;                     // group g: S buffers at g * 256 + {0, 64}, O at g * 256 + 128
+  Walk x;
+  x.start(p, bars, w0, w1, per_item);
+
+  if (warp == 0) {
+    // ---------------------------------------------------------- TMA producer (whole warp: lanes share the boxes)
+    if (lane == 0) {
+      prefetch_tmap(&tmQ);
+      prefetch_tmap(&tmK);
+      prefetch_tmap(&tmV);
+    }
+    const int boxes = BKV / p.box_tokens, per_unit = boxes * QS;       // boxes of a 64-column slab; at most 8 x 2
+    const int slab = lane / boxes, bx = lane % boxes;
+    const long num_slots = a.num_slots;
+    bool ok = true;
+    int u = 0;
+    for (int piece = 0; ok && x.next(p, per_item); ++piece) {
+      if (lane == 0) {
+        ok = mbar_wait(&bars->q_empty, (piece & 1) ^ 1);
+        if (ok) {
+          const int tiles = PAIR && x.q.n - x.node0 > p.nodes ? 2 : 1;
+          mbar_arrive_expect_tx(&bars->q_full, uint32_t(tiles * QS * 128 * p.group * p.nodes));
+          for (int h = 0; h < tiles; ++h)
+#pragma unroll
+            for (int sl = 0; sl < QS; ++sl)
+              tma_load_3d(sQ + h * C::Q_BYTES + sl * Q_SLAB, &tmQ, &bars->q_full, sl * 64, x.head * p.group, x.q.q_start + x.node0 + h * p.nodes);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      const int* bt = a.block_tables + size_t(x.seq) * a.max_blocks;
+      auto unit = [&](const CUtensorMap* map, int j) {
+        long slot = 0;
+        if (lane < per_unit) {
+          const int tok = x.key0(j) + bx * p.box_tokens, bi = min(tok / a.block_size, a.max_blocks - 1);
+          slot = long(bt[bi]) * a.block_size + tok % a.block_size;
+          if (slot < 0 || slot + p.box_tokens > num_slots) slot = 0;   // places behind the last row
+        }
+        const int st = u % U;
+        if (lane == 0) {
+          ok = mbar_wait(&bars->empty[st], ((u / U) & 1) ^ 1);
+          if (ok) mbar_arrive_expect_tx(&bars->full[st], UNIT);
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (ok && lane < per_unit)
+          tma_load_3d(ring + st * UNIT + slab * KV_SLAB + bx * p.box_tokens * 128, map, &bars->full[st], slab * 64, x.head, int(slot));
+        __syncwarp();
+        ++u;
+      };
+      for (int j = 0; ok && j < x.nt + LAG; ++j) {
+        if (j < x.nt) unit(&tmK, j);
+        if (ok && j >= LAG) unit(&tmV, j - LAG);
+      }
+    }
+    if (!ok && lane == 0) atomicExch(p.status, XL_ERR_WAIT_EMPTY);
+  } else if (warp == 1) {
+    // ---------------------------------------------------------- MMA issuer
+    if (elect_one_sync()) {
+      const uint32_t idesc_s = umma_idesc_f16(BQ, BKV, 1), idesc_o = umma_idesc_f16(BQ, DV, 1) | (1u << 16);   // V is MN-major
+      const uint32_t q_addr = smem_u32(sQ), ring_addr = smem_u32(ring), p_addr = smem_u32(sP);
+      bool ok = true;
+      int u0 = 0, s_count[2] = {0, 0}, p_count[2] = {0, 0};
+      for (int piece = 0; ok && x.next(p, per_item); ++piece) {
+        const int nt = x.nt, groups = PAIR && x.q.n - x.node0 > p.nodes ? 2 : 1;
+        ok = mbar_wait(&bars->q_full, piece & 1);
+        for (int j = 0; ok && j < nt + LAG; ++j) {
+          if (j < nt) {
+            const int u = u0 + k_unit<LAG>(j), st = u % U;
+            if (!(ok = mbar_wait(&bars->full[st], (u / U) & 1))) break;
+            const uint32_t k_addr = ring_addr + st * UNIT;
+#pragma unroll
+            for (int h = 0; h < (PAIR ? 2 : 1); ++h) {
+              if (h >= groups) break;
+              const int g = PAIR ? h : j & 1;
+              int& n = s_count[g];
+              const int b = n & 1;
+              if (!(ok = mbar_wait(&bars->s_free[g][b], ((n >> 1) & 1) ^ 1))) break;
+              ++n;
+              tc_fence_after();
+#pragma unroll
+              for (int k = 0; k < DV / 16; ++k)
+                tc_mma_f16(tmem + g * 256 + b * 64, umma_desc_sw128(q_addr + h * C::Q_BYTES + (k >> 2) * Q_SLAB, (k & 3) * 32),
+                           umma_desc_sw128(k_addr + (k >> 2) * KV_SLAB, (k & 3) * 32), idesc_s, k != 0);
+              tc_commit(&bars->s_full[g][b]);
+            }
+            if (!ok) break;
+            tc_commit(&bars->empty[st]);
+            if (j == nt - 1) tc_commit(&bars->q_empty);
+          }
+          if (j >= LAG && j - LAG < nt) {
+            const int i = j - LAG, u = u0 + v_unit<LAG>(i, nt), st = u % U;
+            if (!(ok = mbar_wait(&bars->full[st], (u / U) & 1))) break;
+            const uint32_t v_addr = ring_addr + st * UNIT;
+#pragma unroll
+            for (int h = 0; h < (PAIR ? 2 : 1); ++h) {
+              if (h >= groups) break;
+              const int g = PAIR ? h : i & 1;
+              if (!(ok = mbar_wait(&bars->p_full[g], p_count[g] & 1))) break;
+              ++p_count[g];
+              tc_fence_after();
+#pragma unroll
+              for (int k = 0; k < BKV / 16; ++k)
+                tc_mma_f16(tmem + g * 256 + 128, umma_desc_sw128(p_addr + g * P_BYTES, k * 32),
+                           umma_desc_sw128_mn(v_addr + k * 2048, KV_SLAB, 1024), idesc_o, ((PAIR ? i : i >> 1) | k) != 0);
+              tc_commit(&bars->pv_done[g]);
+            }
+            if (!ok) break;
+            tc_commit(&bars->empty[st]);
+          }
+        }
+        u0 += 2 * nt;
+      }
+      if (!ok) atomicExch(p.status, XL_ERR_WAIT_FULL);
+    }
+  } else {
+    // ---------------------------------------------------------- softmax, one row per thread
+    const int g = (warp - 2) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    const int gt = (warp - 2 - 4 * g) * 32 + lane;                     // thread of the group
+    const uint32_t t_s = tmem + g * 256 + (uint32_t(quarter * 32) << 16), t_o = t_s + 128;
+    uint8_t* prow = sP + g * P_BYTES + r * 128;
+    const int node = r / p.group, head_in = r - node * p.group;
+    const float sc = p.scale_log2;
+    const int flags = PAIR ? 0 : g;                                    // whose flags hold for this group's keys
+    auto group_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory"); };
+    auto both_sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+    bool ok = true;
+    int u0 = 0, count = 0;                                             // units ahead of the piece; tiles of this group so far
+    for (int piece = 0; x.next(p, per_item); ++piece) {
+      const int nt = x.nt;
+      const bool idle = PAIR && g == 1 && x.q.n - x.node0 <= p.nodes;  // the second row tile is empty
+      const int my_node = x.node0 + (PAIR ? g * p.nodes : 0) + node;
+      const bool valid = node < p.nodes && my_node < x.q.n;
+      const bool warp_valid = __any_sync(0xffffffffu, valid);
+      const int t = x.q.q_start + (valid ? my_node : 0);
+      const int pos = valid ? a.positions[t] : 0;
+      float m_ref = -INFINITY, l_run = 0.f;
+      int done = 0;                                                    // tiles of this group in this piece
+      // (a group whose wait ran out goes on without waiting, so that the others still meet it at the barriers)
+      for (int j = PAIR ? 0 : g; j < nt && !idle; j += PAIR ? 1 : 2, ++done, ++count) {
+        const int b = count & 1, kv0 = x.key0(j);
+        if (ok && !__all_sync(0xffffffffu, mbar_wait(&bars->s_full[g][b], (count >> 1) & 1))) ok = false;
+        tc_fence_after();
+        uint32_t pk[32];
+        bool rescale = false;
+        float alpha = 1.f;
+        const bool partly = x.partly(a, kv0);
+        if (warp_valid) {
+          uint32_t s0[32], s1[32];
+          tmem_ld_32x32(t_s + b * 64, s0);
+          tmem_ld_32x32(t_s + b * 64 + 32, s1);
+          tc_wait_ld();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->s_free[g][b]);
+          float v[64];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            v[c] = __uint_as_float(s0[c]);
+            v[32 + c] = __uint_as_float(s1[c]);
+          }
+          if (partly) {
+            const uint64_t see = valid ? seen_keys(a, x.q, t, pos, kv0) : 0;
+            const uint32_t lo = uint32_t(see), hi = uint32_t(see >> 32);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              if (!(lo >> c & 1u)) v[c] = -INFINITY;
+              if (!(hi >> c & 1u)) v[32 + c] = -INFINITY;
+            }
+          }
+          float mx8[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) mx8[i] = v[i];
+#pragma unroll
+          for (int c = 8; c < 64; ++c) mx8[c & 7] = fmaxf(mx8[c & 7], v[c]);
+          const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])), fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+          // the reference stays unless the scaled maximum grew by more than 8: P stays below 2^8
+          const bool had = m_ref != -INFINITY;
+          const bool grow = (mx - m_ref) * sc > 8.f || (!had && mx != -INFINITY);
+          const float m_new = grow ? mx : m_ref;
+          rescale = grow && had;
+          alpha = rescale ? fast_exp2((m_ref - m_new) * sc) : 1.f;
+          m_ref = m_new;
+          const float mneg = m_ref == -INFINITY ? 0.f : -m_ref * sc;
+          float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 64; c += 2) {
+            const float e0 = fast_exp2(fmaf(v[c], sc, mneg)), e1 = fast_exp2(fmaf(v[c + 1], sc, mneg));
+            sum4[(c >> 1) & 3] += e0 + e1;
+            pk[c >> 1] = pack_bf16x2(e0, e1);
+          }
+          l_run = l_run * alpha + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+        } else {
+          tc_fence_before();
+          if (lane == 0) mbar_arrive(&bars->s_free[g][b]);
+        }
+        // P and O are touched only after P V of this group's tile before
+        if (ok && done > 0 && !__all_sync(0xffffffffu, mbar_wait(&bars->pv_done[g], (count - 1) & 1))) ok = false;
+        tc_fence_after();
+        if (done > 0 && __any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+          for (int c = 0; c < DV; c += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32(t_o + c, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st_32x32(t_o + c, o);
+          }
+          tc_wait_st();
+        }
+        if (warp_valid) {
+          // 16-byte chunk c of row r at chunk c ^ (r & 7)
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            *reinterpret_cast<uint4*>(prow + ((c ^ (r & 7)) << 4)) = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+        }
+        if (partly && flags == g) {
+          // two threads look at the values of one key
+          const int u = u0 + v_unit<LAG>(j, nt), st = u % U, key = gt >> 1;
+          if (ok && !__all_sync(0xffffffffu, mbar_wait(&bars->full[st], (u / U) & 1))) ok = false;
+          uint4* row = reinterpret_cast<uint4*>(ring + st * UNIT + key * 128 + (gt & 1) * 64);
+          bool bad = false;
+          if (ok) {
+#pragma unroll
+            for (int sl = 0; sl < QS; ++sl)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                uint4* at = row + sl * (KV_SLAB / 16) + i;
+                if (kv0 + key >= x.q.kv_len) {
+                  *at = make_uint4(0, 0, 0, 0);
+                } else {
+                  uint4 w = *at;
+                  if (not_finite(w.x) || not_finite(w.y) || not_finite(w.z) || not_finite(w.w)) {
+                    auto clean = [](uint32_t v) { return ((v & 0x7F800000u) == 0x7F800000u ? 0 : v & 0xFFFF0000u) | ((v & 0x7F80u) == 0x7F80u ? 0 : v & 0xFFFFu); };
+                    *at = make_uint4(clean(w.x), clean(w.y), clean(w.z), clean(w.w));
+                    bad = true;
+                  }
+                }
+              }
+          }
+          if (bad) {
+            atomicOr(&bars->bad[piece & 3][g][x.tile_number(kv0)][key >> 5], 1u << (key & 31));
+            bars->any_bad[piece & 3] = 1;
+          }
+          group_sync();
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->p_full[g]);
+      }
+      if (ok && done > 0 && !__all_sync(0xffffffffu, mbar_wait(&bars->pv_done[g], (count - 1) & 1))) ok = false;
+      tc_fence_after();
+      u0 += 2 * nt;
+      // ------------------------------------------------ end of a piece
+      if (ok && done > 0 && warp_valid && bars->any_bad[piece & 3]) {
+        // values that are not finite join the rows that see them
+        for (int i = 0; i < 16 * 64; ++i) {
+          const int tile = i >> 6, k = i & 63;
+          if (!(bars->bad[piece & 3][flags][tile][k >> 5] >> (k & 31) & 1u)) continue;
+          const int kv0 = tile >= 8 ? x.q.base / BKV * BKV + (tile - 8) * BKV : x.q.kv_begin + tile * BKV, key = kv0 + k;
+          const bool see = valid && (seen_keys(a, x.q, t, pos, kv0) >> k & 1ull);
+          const long slot = long(a.block_tables[size_t(x.seq) * a.max_blocks + key / a.block_size]) * a.block_size + key % a.block_size;
+          if (slot < 0 || slot >= a.num_slots) continue;
+          const __nv_bfloat16* from = static_cast<const __nv_bfloat16*>(a.v_cache) + (size_t(slot) * a.n_kv + x.head) * a.D;
+          for (int c = 0; c < DV; c += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32(t_o + c, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float f = c + e < a.D ? __bfloat162float(from[c + e]) : 0.f;
+              if (see && !(fabsf(f) <= 3.4e38f)) o[e] = __float_as_uint(__uint_as_float(o[e]) + f);
+            }
+            tmem_st_32x32(t_o + c, o);
+          }
+          tc_wait_st();
+        }
+      }
+      const bool whole = x.whole();
+      const int slot = 2 * blockIdx.x + (piece > 0);
+      const int ws_row = PAIR ? g * BQ + r : r;
+      const float m_log2 = m_ref == -INFINITY ? -INFINITY : m_ref * sc;
+      // the weights of the two groups' sums (PAIR: its own alone), and the columns that this group stores
+      float wa = 1.f, wb = 0.f, m_all = m_log2, l_all = l_run;
+      int c_lo = 0, c_hi = DV;
+      bool use_a = done > 0, use_b = false;                            // a: group 0 (PAIR: this group)
+      uint32_t t_oa = t_o;
+      const uint32_t t_ob = tmem + 256 + 128 + (uint32_t(quarter * 32) << 16);
+      if (!PAIR) {
+        bars->ml[g][r] = make_float2(m_log2, l_run);
+        tc_fence_before();
+        both_sync();
+        tc_fence_after();
+        const float2 other = bars->ml[g ^ 1][r];
+        const float ma = g == 0 ? m_log2 : other.x, mb = g == 0 ? other.x : m_log2, la = g == 0 ? l_run : other.y, lb = g == 0 ? other.y : l_run;
+        m_all = fmaxf(ma, mb);
+        wa = ma == -INFINITY ? (la != la ? la : 0.f) : fast_exp2(ma - m_all);
+        wb = mb == -INFINITY ? (lb != lb ? lb : 0.f) : fast_exp2(mb - m_all);
+        l_all = la * wa + lb * wb;
+        use_a = true;
+        use_b = nt > 1;
+        t_oa = tmem + 128 + (uint32_t(quarter * 32) << 16);
+        c_lo = g * (DV / 2);
+        c_hi = c_lo + DV / 2;
+      }
+      if (ok && use_a && warp_valid) {
+        const float inv = l_all != 0.f ? 1.f / l_all : 0.f;            // a row that sees nothing: zeros
+        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + size_t(t) * (size_t(a.n_q) * a.D) + (x.head * p.group + head_in) * a.D;
+        float4* wo = p.ws_o + size_t(slot) * (DV / 4) * C::kRows + ws_row;
+        const float fa = whole ? wa * inv : wa, fb = whole ? wb * inv : wb;
+#pragma unroll
+        for (int c = c_lo; c < c_hi; c += 32) {
+          uint32_t oa[32];
+          tmem_ld_32x32(t_oa + c, oa);
+          tc_wait_ld();
+          float f[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(oa[i]) * fa;
+          if (use_b) {
+            tmem_ld_32x32(t_ob + c, oa);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = fmaf(__uint_as_float(oa[i]), fb, f[i]);
+          }
+          if (valid) {
+            if (whole) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (c + 8 * i < a.D)
+                  *reinterpret_cast<uint4*>(dst + c + 8 * i) = make_uint4(pack_bf16x2(f[8 * i], f[8 * i + 1]), pack_bf16x2(f[8 * i + 2], f[8 * i + 3]),
+                                                                          pack_bf16x2(f[8 * i + 4], f[8 * i + 5]), pack_bf16x2(f[8 * i + 6], f[8 * i + 7]));
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) wo[size_t(c / 4 + i) * C::kRows] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+            }
+          }
+        }
+        if (valid && !whole && (PAIR || g == 0)) p.ws_ml[size_t(slot) * C::kRows + ws_row] = make_float2(m_all, l_all);
+      }
+      // the next piece's flags were last read three pieces ago
+      if (flags == g) {
+        for (int i = gt; i < 32; i += 128) (&bars->bad[(piece + 1) & 3][g][0][0])[i] = 0;
+        if (gt == 0 && g == 0) bars->any_bad[(piece + 1) & 3] = 0;
+        group_sync();
+      }
+      if (!PAIR) {
+        tc_fence_before();
+        both_sync();                                                   // both groups have read O and the maxima
+      }
+      if (piece == 0 && tid == 64) {
+        int* d = p.ws_desc + blockIdx.x * 8;
+        const bool merge = x.j0 > 0 && x.j0 + nt == x.q.key_tiles;
+        d[DESC_MERGE] = merge;
+        if (merge) {
+          const long start = x.w - x.j0;                               // the item's first tile
+          const long first = ((start + 1) * ctas - 1) / total;
+          d[DESC_FIRST] = int(first);
+          d[DESC_SLOT] = int(2 * first + (first * total / ctas == start ? 0 : 1));
+          d[DESC_START] = x.q.q_start + x.node0;
+          d[DESC_NODES] = min(per_item, x.q.n - x.node0);
+          d[DESC_HEAD] = x.head;
+        }
+      }
+    }
+    if (!ok && lane == 0) atomicExch(p.status, XL_ERR_WAIT_TMEM_FULL);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+// Joins the partials of the item that ends in CTA blockIdx.x's first piece: o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i.
+template <int QS, bool PAIR>
+__global__ void __launch_bounds__(256) attention_tree_merge_kernel(const TcParams p) {
+  using C = Cfg<QS, PAIR>;
+  const Params& a = p.a;
+  grid_dep_wait();
+  const int* d = p.ws_desc + blockIdx.x * 8;
+  if (!d[DESC_MERGE]) return;
+  const int first = d[DESC_FIRST], slot0 = d[DESC_SLOT], parts = int(blockIdx.x) - first + 1, nodes = d[DESC_NODES], rows = nodes * p.group;
+  const int c4 = a.D / 4, items = rows * c4;
+  for (int i = blockIdx.y * 256 + threadIdx.x; i < items; i += gridDim.y * 256) {
+    const int row = i % rows, c = i / rows;                            // neighbours share a column group: partials are read side by side
+    const int node = row / p.group, h = row - node * p.group;
+    const int tile = PAIR ? node / p.nodes : 0;
+    const int ws_row = tile * BQ + (node - tile * p.nodes) * p.group + h;
+    float m = -INFINITY;
+    for (int k = 0; k < parts; ++k) m = fmaxf(m, __ldcg(&p.ws_ml[size_t(k == 0 ? slot0 : 2 * (first + k)) * C::kRows + ws_row]).x);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < parts; ++k) {
+      const size_t slot = k == 0 ? slot0 : 2 * (first + k);
+      const float2 ml = __ldcg(&p.ws_ml[slot * C::kRows + ws_row]);
+      if (ml.x == -INFINITY && ml.y == 0.f) continue;                  // sees no key of that part
+      const float w = ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - m);
+      const float4 v = __ldcg(&p.ws_o[(slot * (C::DV / 4) + c) * C::kRows + ws_row]);
+      l += w * ml.y;
+      o.x += w * v.x; o.y += w * v.y; o.z += w * v.z; o.w += w * v.w;
+    }
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + size_t(d[DESC_START] + node) * (size_t(a.n_q) * a.D) + (d[DESC_HEAD] * p.group + h) * a.D + 4 * c;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+  }
+}
+
+template <int QS, bool PAIR>
+int launch_tc(const TcParams& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, int ctas, cudaStream_t s) {
+  using C = Cfg<QS, PAIR>;
+  auto* kernel = attention_tree_tc_kernel<QS, PAIR>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess) return -1;
+  kernel<<<ctas, kTcThreads, C::kSmem, s>>>(q, k, v, p);
+  if (cudaGetLastError() != cudaSuccess) return -1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas, 4);
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attention_tree_merge_kernel<QS, PAIR>, p) == cudaSuccess ? 0 : -1;
+}
+
 }  // namespace xl_at
+
+static bool tc_serves(const void* q, const void* k, const void* v, int block_size, int n_q, int n_kv, int D, long q_row, long q_head,
+                      float scale, int f32) {
+  const int box = block_size & -block_size;                 // largest power of two that divides it
+  return !f32 && D % 8 == 0 && D <= 128 && n_q / n_kv <= xl_at::BQ && box >= 8 && scale > 0.f && q_row % 8 == 0 && q_head % 8 == 0 && q_head > 0 &&
+         q_row % q_head == 0 && (reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 == 0;
+}
+
+// Bytes of the workspace for `ctas` CTAs (0: the tensor-core kernel does not serve these sizes).  max_q: rows of a sequence at most.
+XL_API long xl_attention_tree_workspace(int block_size, int n_q, int n_kv, int D, int max_q, int f32, int ctas) {
+  if (!tc_serves(nullptr, nullptr, nullptr, block_size, n_q, n_kv, D, 8, 8, 1.f, f32)) return 0;
+  const long rows = long(max_q) * (n_q / n_kv) > xl_at::BQ ? 256 : 128, DV = (D + 63) / 64 * 64;
+  return 2l * ctas * rows * (DV * 4 + 8) + 32l * ctas;
+}
 
 XL_API int xl_attention_tree(const void* q, const void* k_cache, const void* v_cache, void* out, const void* q_cu, const void* kv_lens,
                              const void* block_tables, const void* token_seq, const void* positions, const void* tree, int T, int B,
                              int max_blocks, int block_size, int num_blocks, int n_q, int n_kv, int D, int words, long q_row, long q_head,
-                             float scale, int window, int f32, void* stream) {
+                             float scale, int window, int f32, int max_q, int ctas, void* workspace, long workspace_bytes, void* stream) {
   using namespace xl_at;
   if (T < 0 || B < 0 || n_kv < 1 || n_q % n_kv || D < 1 || D > 32 * kMaxCols || words < 1 || block_size < 1 || max_blocks < 1) return -2;
   if (T == 0) return 0;
@@ -116,10 +796,39 @@ XL_API int xl_attention_tree(const void* q, const void* k_cache, const void* v_c
   p.q_row = q_row; p.q_head = q_head;
   p.num_slots = long(num_blocks) * block_size;
   p.scale = scale; p.window = window;
-  const long items = long(T) * n_q, ctas = (items + 3) / 4;
-  if (ctas > 0x7fffffffl) return -2;
   auto s = static_cast<cudaStream_t>(stream);
-  if (f32) attention_tree_simt_kernel<float><<<unsigned(ctas), 128, 4 * D * sizeof(float), s>>>(p);
-  else attention_tree_simt_kernel<__nv_bfloat16><<<unsigned(ctas), 128, 4 * D * sizeof(float), s>>>(p);
+  if (workspace && B > 0 && tc_serves(q, k_cache, v_cache, block_size, n_q, n_kv, D, q_row, q_head, scale, f32)) {
+    const bool pair = long(max_q) * (n_q / n_kv) > BQ;
+    if (ctas < 1 || workspace_bytes < xl_attention_tree_workspace(block_size, n_q, n_kv, D, max_q, f32, ctas)) return -2;
+    TcParams t{};
+    t.a = p;
+    t.group = n_q / n_kv;
+    t.nodes = BQ / t.group;
+    t.box_tokens = min(block_size & -block_size, BKV);
+    t.min_tiles = 4;
+    t.scale_log2 = scale * 1.4426950408889634f;
+    const int rows = pair ? 256 : 128, DV = (D + 63) / 64 * 64;
+    t.ws_o = static_cast<float4*>(workspace);
+    t.ws_ml = reinterpret_cast<float2*>(t.ws_o + size_t(2) * ctas * rows * (DV / 4));
+    t.ws_desc = reinterpret_cast<int*>(t.ws_ml + size_t(2) * ctas * rows);
+    t.status = xl_host::status_word();
+    CUtensorMap mq, mk, mv;
+    const uint64_t q_dims[3] = {uint64_t(D), uint64_t(n_q), uint64_t(T)}, q_strides[2] = {uint64_t(q_head) * 2, uint64_t(q_row) * 2};
+    const uint32_t q_box[3] = {64, uint32_t(t.group), uint32_t(t.nodes)};
+    const uint64_t kv_dims[3] = {uint64_t(D), uint64_t(n_kv), uint64_t(p.num_slots)}, kv_strides[2] = {uint64_t(D) * 2, uint64_t(n_kv) * D * 2};
+    const uint32_t kv_box[3] = {64, 1, uint32_t(t.box_tokens)};
+    const auto bf16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const auto swz = CU_TENSOR_MAP_SWIZZLE_128B;
+    if (xl_host::encode_tiled(&mq, bf16, 3, q, q_dims, q_strides, q_box, swz) != CUDA_SUCCESS ||
+        xl_host::encode_tiled(&mk, bf16, 3, k_cache, kv_dims, kv_strides, kv_box, swz) != CUDA_SUCCESS ||
+        xl_host::encode_tiled(&mv, bf16, 3, v_cache, kv_dims, kv_strides, kv_box, swz) != CUDA_SUCCESS)
+      return -4;
+    if (D <= 64) return pair ? launch_tc<1, true>(t, mq, mk, mv, ctas, s) : launch_tc<1, false>(t, mq, mk, mv, ctas, s);
+    return pair ? launch_tc<2, true>(t, mq, mk, mv, ctas, s) : launch_tc<2, false>(t, mq, mk, mv, ctas, s);
+  }
+  const long items = long(T) * n_q, grid = (items + 3) / 4;
+  if (grid > 0x7fffffffl) return -2;
+  if (f32) attention_tree_simt_kernel<float><<<unsigned(grid), 128, 4 * D * sizeof(float), s>>>(p);
+  else attention_tree_simt_kernel<__nv_bfloat16><<<unsigned(grid), 128, 4 * D * sizeof(float), s>>>(p);
   return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }

@@ -381,6 +381,7 @@ def tree_attention(q, k_cache, v_cache, inp, tree, scale, sliding_window=-1):
     assert Hq % k_cache.shape[2] == 0 and k_cache.is_contiguous() and v_cache.is_contiguous()
     dev, i32, B = q.device, torch.int32, inp.n_seqs
     assert k_cache.device == v_cache.device == dev
+    assert inp.max_q <= TREE_MAX_ROWS, f"trees have at most {TREE_MAX_ROWS} rows a sequence"
     assert tree.dim() == 2 and 1 <= tree.shape[1] <= TREE_MAX_ROWS // 64, "tree: one to four words a row"
     _like(tree, torch.int64, (T, None), dev, "tree")
     _like(inp.q_cu, i32, (B + 1,), dev, "q_cu")

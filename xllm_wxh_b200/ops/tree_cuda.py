@@ -13,7 +13,7 @@ _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
 _SIGNATURES = {
     "xl_step_rows": [_P] * 12 + [_I] * 8 + [_P],
     "xl_accept_tree": [_P] * 9 + [_I] * 5 + [_P] * 3 + [_I] * 2 + [_P],
-    "xl_attention_tree": [_P] * 10 + [_I] * 9 + [_L] * 2 + [_F] + [_I] * 2 + [_P],
+    "xl_attention_tree": [_P] * 10 + [_I] * 9 + [_L] * 2 + [_F] + [_I] * 4 + [_P, _L, _P],
     "xl_adjust_logits": [_P] + [_I] * 3 + [_L] + [_P] * 2 + [_I] * 3 + [_P, _L, _I] + [_P] * 10 + [_I, _P, _I, _I, _P, _P],
 }
 _ready = set()
@@ -29,6 +29,16 @@ def _launch(device: torch.device, name: str, *args) -> None:
     with contextlib.nullcontext() if here else torch.cuda.device(device):
         cuda_ops._check(getattr(L, name)(*args, torch.cuda.current_stream().cuda_stream), name)
     cuda_ops.launch_count += 1
+
+
+_sm_counts = {}
+
+
+def _sms(device: torch.device) -> int:
+    n = _sm_counts.get(device)
+    if n is None:
+        n = _sm_counts[device] = torch.cuda.get_device_properties(device).multi_processor_count
+    return n
 
 
 def _ptr(t):
@@ -52,13 +62,25 @@ def step_rows(tables, lens, seqs, counts, n_rows, block_size, parents, max_q, ma
 def tree_attention(q, k_cache, v_cache, inp, tree, scale, window) -> torch.Tensor:
     T, Hq, D = q.shape
     out = torch.empty((T, Hq * D), dtype=q.dtype, device=q.device)
-    if q.stride(2) != 1:
+    block, Hkv = k_cache.shape[1], k_cache.shape[2]
+    f32, work, ctas, size = q.dtype == torch.float32, None, 0, 0
+    if not f32 and scale > 0:
+        # one CTA per SM, fewer where there are fewer key tiles (of 64 keys for up to 128 rows) than it takes to be worth one
+        tiles = (inp.max_kv // 64 + 1) * Hkv * (inp.n_seqs + T * (Hq // Hkv) // 128)
+        ctas = max(1, min(_sms(q.device), tiles // 4))
+        size = cuda_ops.lib().xl_attention_tree_workspace(block, Hq, Hkv, D, inp.max_q, 0, ctas)
+    if size:
+        if q.stride(2) != 1 or q.stride(1) % 8 or q.stride(0) % max(8, q.stride(1)) or q.data_ptr() % 16:
+            q = q.contiguous()
+        work = torch.empty(size, dtype=torch.uint8, device=q.device)
+    elif q.stride(2) != 1:
         q = q.contiguous()
     bt = inp.block_tables
     _launch(q.device, "xl_attention_tree", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), inp.q_cu.data_ptr(),
             inp.kv_lens.data_ptr(), bt.data_ptr(), inp.token_seq.data_ptr(), inp.positions.data_ptr(), tree.data_ptr(), T, inp.n_seqs, bt.shape[1],
-            k_cache.shape[1], k_cache.shape[0], Hq, k_cache.shape[2], D, tree.shape[1], q.stride(0), q.stride(1), scale, window,
-            int(q.dtype == torch.float32))
+            block, k_cache.shape[0], Hq, Hkv, D, tree.shape[1], q.stride(0), q.stride(1), scale, window, int(f32), inp.max_q, ctas, _ptr(work), size)
+    if size:
+        cuda_ops.launch_count += 1                               # the join of pieces
     return out
 
 
