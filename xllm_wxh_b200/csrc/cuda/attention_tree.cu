@@ -98,19 +98,21 @@ __global__ void __launch_bounds__(128) attention_tree_simt_kernel(const Params p
 
 // ---------------------------------------------------------------- tensor-core kernel
 // bf16, up to 128 columns a head.  A key head's query heads times a tree's nodes are the rows of one product: 128 rows (TMEM lanes) take in
-// 128 / G nodes of G heads each, so that a key is read once for all of them (PAIR: for 256 rows).  Reading K and V bounds the kernel up to
-// about 256 rows; above, exponentials and products do.
+// 128 / G nodes of G heads each, so that a key is read once for all of them (two row tiles: for 256 rows).  Reading K and V bounds the
+// kernel up to about 256 rows; above, exponentials and products do.
 //
-//   work      : the key tiles (64 keys) of every (sequence, key head, rows) one behind the other, cut into equal stretches, one per CTA
-//               (one CTA per SM): ragged lengths leave no SM idle.  A stretch begins and ends anywhere; the at most two pieces of it
-//               that are not whole leave fp32 partials (sums, maximum, denominator) that the merge kernel joins.
-//   warp 0    : TMA producer - query rows of a piece (box: 64 columns x G heads x nodes), then a ring of units in the order of use, each
-//               64 tokens of K or of V through the block table;
-//   warp 1    : MMA issuer   - S = Q K^T (128 x 64 x D, fp32 in TMEM, two buffers a group), O += P V;
-//   warps 2-5 and 6-9: two softmax groups, one row per thread: running maximum and sum in the log2 domain, P as bf16 through shared
-//               memory, O rescaled only when the maximum grew by more than 2^8.
-//               PAIR: each group has 128 rows of its own, both read the same keys.  Otherwise the groups take the key tiles in turn
-//               for the same rows, each with its own O, and join at the end of a piece: a single group could not keep up with memory.
+//   work      : the key tiles (64 keys) of every item (sequence, key head, rows) one behind the other, each item with kItemCost tiles'
+//               worth of work ahead of it, cut into equal stretches, one per CTA (one CTA per SM): ragged lengths leave no SM idle.
+//               A stretch begins and ends anywhere; the at most two pieces of it that are not whole items leave fp32 partials (sums,
+//               maximum, denominator) that the merge kernel joins.
+//   warp 0    : TMA producer - says what the next piece is, fetches its query rows (box: 64 columns x G heads x nodes), then a ring of units
+//               in the order of use, each 64 tokens of K or of V through the block table;
+//   warp 1    : MMA issuer   - S = Q K^T (128 x 64 x D, fp32 in TMEM, two buffers a group), O += P V with P from TMEM;
+//   warps 2-5 and 6-9: two softmax groups, one row per thread: running maximum and sum in the log2 domain, P as bf16 over the
+//               scores it comes from, O rescaled only when the maximum grew by more than 2^8.
+//               An item of two row tiles gives each group one; otherwise the groups take the key tiles in turn for the same rows, each
+//               with its own O, and join at the end of a piece: a single group could not keep up with memory.
+// Products run in the order of their issue, so S of a tile may overwrite P of the tile two before as soon as that one's P V is issued.
 //
 // Masks: keys ahead of the tree are seen by all rows (within the window), the tree's by the row's words; only tiles that hold either
 // border look at them.  There, values behind the last row are cleared, and values that are not finite are taken out of the tile and
@@ -118,36 +120,55 @@ __global__ void __launch_bounds__(128) attention_tree_simt_kernel(const Params p
 // Every wait is bounded; on expiry the kernel records a status code and leaves.
 constexpr int BQ = 128, BKV = 64;
 constexpr int kTcThreads = 320;
-constexpr int Q_SLAB = BQ * 128, KV_SLAB = BKV * 128, P_BYTES = BQ * BKV * 2;
-constexpr int kMaxUnits = 16;
+constexpr int Q_SLAB = BQ * 128, KV_SLAB = BKV * 128;
+constexpr int kMaxUnits = 20, kPieces = 8, kItemCost = 3;
+
+struct Seq {
+  int q_start, n, kv_len, base, kv_begin, row_tiles, key_tiles;
+  __device__ __forceinline__ int item() const { return key_tiles + kItemCost; }
+  __device__ __forceinline__ long work(int n_kv) const { return long(row_tiles) * n_kv * item(); }
+};
+struct Piece {
+  Seq q;
+  int seq, head, node0, j0, nt;            // node0: first node of the piece's rows; its key tiles j0 .. j0 + nt - 1 (0: no more pieces)
+  int pair, whole, slot;                   // pair: two row tiles; slot: of its partials
+  __device__ __forceinline__ int key0(int j) const { return q.kv_begin + (j0 + j) * BKV; }
+  // tiles in which some row may see only a part: the window's border, the tree, the end
+  __device__ __forceinline__ bool partly(const Params& p, int kv0) const {
+    return kv0 + BKV > q.base || (p.window > 0 && kv0 < q.base + q.n - p.window);
+  }
+  __device__ __forceinline__ int tile_number(int kv0) const {        // of such a tile among its item's
+    return kv0 + BKV > q.base ? min(8 + (kv0 - q.base / BKV * BKV) / BKV, 15) : min((kv0 - q.kv_begin) / BKV, 7);
+  }
+};
 struct TcBarriers {
   uint64_t full[kMaxUnits], empty[kMaxUnits];
-  uint64_t q_full, q_empty;
-  uint64_t s_full[2][2], s_free[2][2];                       // [group][buffer]
-  uint64_t p_full[2], pv_done[2];
+  uint64_t q_full, q_empty, info[kPieces];
+  // [group][buffer]: softmax may be two tiles ahead of the products and need not look at each one's end, so that a barrier a group
+  // would be a phase off
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];
   uint32_t tmem_base;
-  int seq, any_bad[4];
-  long seq_tiles;                                            // tiles ahead of `seq`
-  long part[kTcThreads / 32];
+  int seq;
+  int any_bad[4][2];                                         // [piece & 3][group]
+  long seq_work, part[kTcThreads / 32];                      // work ahead of `seq`
   uint32_t bad[4][2][16][2];                                 // [piece & 3][group][tile][key]: keys whose values are not all finite
   float2 ml[2][BQ];
+  Piece piece[kPieces];
 };
-
-template <int QS, bool PAIR> struct Cfg {
+template <int QS, int NQ> struct Cfg {                       // NQ: row tiles of an item at most
   static constexpr int DV = 64 * QS;                         // padded columns
-  static constexpr int Q_BYTES = QS * Q_SLAB, UNIT = QS * KV_SLAB, NQ = PAIR ? 2 : 1;
-  static constexpr int kFit = (227 * 1024 - int(sizeof(TcBarriers)) - NQ * Q_BYTES - 2 * P_BYTES) / UNIT;
+  static constexpr int Q_BYTES = QS * Q_SLAB, UNIT = QS * KV_SLAB;
+  static constexpr int kFit = (227 * 1024 - int(sizeof(TcBarriers)) - NQ * Q_BYTES) / UNIT;
   static constexpr int U = kFit < kMaxUnits ? kFit : kMaxUnits;
-  static constexpr int LAG = PAIR ? 1 : 2;                   // S of a tile is issued ahead of P V of the tile LAG before it
-  static constexpr int kSmem = NQ * Q_BYTES + U * UNIT + 2 * P_BYTES + int(sizeof(TcBarriers));
-  static_assert(U >= 6 && kSmem <= 227 * 1024, "a piece's next units fit the ring");
-  static constexpr int kRows = PAIR ? 256 : 128;
+  static constexpr int kSmem = NQ * Q_BYTES + U * UNIT + int(sizeof(TcBarriers));
+  static constexpr int kRows = NQ * BQ;
+  static_assert(U >= 6 && kSmem <= 227 * 1024, "the units up to a tile's values fit the ring");
 };
 
 struct TcParams {
   Params a;
   int group, nodes;             // query heads per key head, nodes of one row tile
-  int box_tokens, min_tiles;
+  int box_tokens, block_shift, min_work;   // block_shift: -1 where the block size is no power of two
   float scale_log2;
   float4* ws_o;                 // [2 * CTA + which][D / 4][rows]
   float2* ws_ml;                // [2 * CTA + which][rows]: (maximum in the log2 domain, sum)
@@ -156,15 +177,11 @@ struct TcParams {
 };
 enum { DESC_MERGE, DESC_FIRST, DESC_SLOT, DESC_START, DESC_NODES, DESC_HEAD };   // of the item that ends in a CTA's first piece
 
-struct Seq {
-  int q_start, n, kv_len, base, kv_begin, row_tiles, key_tiles;
-  __device__ __forceinline__ long tiles(int n_kv) const { return long(row_tiles) * key_tiles * n_kv; }
-};
 __device__ __forceinline__ Seq load_seq(const Params& p, int s, int per_item) {
   Seq q;
   q.q_start = p.q_cu[s];
   q.n = min(p.q_cu[s + 1], p.T) - q.q_start;
-  q.kv_len = min(long(p.kv_lens[s]), long(p.max_blocks) * p.block_size);
+  q.kv_len = int(min(long(p.kv_lens[s]), long(p.max_blocks) * p.block_size));
   q.base = max(q.kv_len - q.n, 0);
   q.kv_begin = p.window > 0 ? max(0, q.base - p.window + 1) / BKV * BKV : 0;
   q.row_tiles = q.n > 0 && q.kv_len > 0 ? (q.n + per_item - 1) / per_item : 0;
@@ -172,50 +189,11 @@ __device__ __forceinline__ Seq load_seq(const Params& p, int s, int per_item) {
   return q;
 }
 
-// The pieces of a CTA's stretch [w, w1) of the tiles; every role walks them by itself.
-struct Walk {
-  Seq q;
-  int seq, head, node0, j0, nt;            // node0: first node of the piece's rows; its key tiles j0 .. j0 + nt - 1
-  long w, w1, ahead;                       // ahead: tiles in front of `seq`
-  __device__ __forceinline__ void start(const TcParams& p, const TcBarriers* b, long w0, long w_end, int per_item) {
-    w = w0;
-    w1 = w_end;
-    seq = b->seq;
-    ahead = b->seq_tiles;
-    q = load_seq(p.a, seq, per_item);
-    nt = 0;
-  }
-  __device__ __forceinline__ bool next(const TcParams& p, int per_item) {
-    w += nt;
-    if (w >= w1) return false;
-    while (w >= ahead + q.tiles(p.a.n_kv)) {
-      ahead += q.tiles(p.a.n_kv);
-      q = load_seq(p.a, ++seq, per_item);
-    }
-    const long at = w - ahead;
-    const int item = int(at / q.key_tiles);
-    j0 = int(at - long(item) * q.key_tiles);
-    nt = int(min(long(q.key_tiles - j0), w1 - w));
-    head = item / q.row_tiles;
-    node0 = item % q.row_tiles * per_item;
-    return true;
-  }
-  __device__ __forceinline__ bool whole() const { return nt == q.key_tiles; }
-  __device__ __forceinline__ int key0(int j) const { return q.kv_begin + (j0 + j) * BKV; }
-  // tiles in which some row may see only a part: the window's border, the tree, the end
-  __device__ __forceinline__ bool partly(const Params& p, int kv0) const {
-    return kv0 + BKV > q.base || (p.window > 0 && kv0 < q.base + q.n - p.window);
-  }
-  __device__ __forceinline__ int tile_number(int kv0) const {        // of such a tile among its piece's (at most 16)
-    return kv0 + BKV > q.base ? min(8 + (kv0 - q.base / BKV * BKV) / BKV, 15) : min((kv0 - q.kv_begin) / BKV, 7);
-  }
-};
+// S of a tile is issued `lag` tiles ahead of P V: by one tile of the same group.  Unit (within its piece) of the keys and values of tile j.
+__device__ __forceinline__ int k_unit(int j, int lag) { return j < lag ? j : 2 * j - lag; }
+__device__ __forceinline__ int v_unit(int j, int lag, int nt) { return j + lag < nt ? 2 * j + lag + 1 : nt + j; }
 
-// unit (within its piece) of the keys and values of tile j
-template <int LAG> __device__ __forceinline__ int k_unit(int j) { return j < LAG ? j : 2 * j - LAG; }
-template <int LAG> __device__ __forceinline__ int v_unit(int j, int nt) { return j + LAG < nt ? 2 * j + LAG + 1 : nt + j; }
-
-// keys of the tile at kv0 that row t (node of its sequence, at position pos) sees
+// keys of the tile at kv0 that row t (at position pos) sees
 __device__ __forceinline__ uint64_t seen_keys(const Params& p, const Seq& q, int t, int pos, int kv0) {
   const int c = q.base - kv0;
   uint64_t see = c >= 64 ? ~0ull : c > 0 ? (1ull << c) - 1 : 0;
@@ -248,37 +226,79 @@ __device__ __forceinline__ uint64_t seen_keys(const Params& p, const Seq& q, int
 __device__ __forceinline__ bool not_finite(uint32_t pair) {
   return (pair & 0x7F800000u) == 0x7F800000u || (pair & 0x7F80u) == 0x7F80u;
 }
+__device__ __forceinline__ uint32_t finite_part(uint32_t pair) {
+  return ((pair & 0x7F800000u) == 0x7F800000u ? 0 : pair & 0xFFFF0000u) | ((pair & 0x7F80u) == 0x7F80u ? 0 : pair & 0xFFFFu);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// D[tmem] (+)= A[tmem] * B[smem desc]: row i of A in lane i, two bf16 per column
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 
-template <int QS, bool PAIR>
+template <int QS, int NQ>
 __global__ void __launch_bounds__(kTcThreads, 1)
 attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                          const TcParams p) {
-  using C = Cfg<QS, PAIR>;
-  constexpr int U = C::U, UNIT = C::UNIT, DV = C::DV, LAG = C::LAG;
+  using C = Cfg<QS, NQ>;
+  constexpr int U = C::U, UNIT = C::UNIT, DV = C::DV;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sQ = smem;
-  uint8_t* ring = sQ + C::NQ * C::Q_BYTES;
-  uint8_t* sP = ring + U * UNIT;
-  TcBarriers* bars = reinterpret_cast<TcBarriers*>(sP + 2 * P_BYTES);
+  uint8_t* ring = sQ + NQ * C::Q_BYTES;
+  TcBarriers* bars = reinterpret_cast<TcBarriers*>(ring + U * UNIT);
   const Params& a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   grid_dep_launch();                                         // the merge kernel may take its place; it waits for this one's end
   if (smem_u32(smem) & 1023u) {
-    if (tid == 0) atomicExch(p.status, XL_ERR_BOUNDS);
+    if (tid == 0) {
+      atomicExch(p.status, XL_ERR_BOUNDS);
+      p.ws_desc[blockIdx.x * 8 + DESC_MERGE] = 0;
+    }
     return;
   }
-  // rows of no sequence
-  {
-    const int behind = max(a.q_cu[a.B], 0), width = a.n_q * a.D;
-    for (long t = long(behind) + blockIdx.x; t < a.T; t += gridDim.x)
-      for (int c = tid; c < width / 8; c += kTcThreads) reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + t * width)[c] = make_uint4(0, 0, 0, 0);
-  }
-  // ------------------------------------------------------------ this CTA's stretch of the tiles
-  const int per_item = (PAIR ? 2 : 1) * p.nodes;
+  // ------------------------------------------------------------ this CTA's stretch of the work
+  const int per_item = NQ * p.nodes;
   const int share = (a.B + kTcThreads - 1) / kTcThreads;
   const int s0 = min(tid * share, a.B), s1 = min(s0 + share, a.B);
   long mine = 0;
-  for (int s = s0; s < s1; ++s) mine += load_seq(a, s, per_item).tiles(a.n_kv);
+  for (int s = s0; s < s1; ++s) mine += load_seq(a, s, per_item).work(a.n_kv);
+  if (warp == 0 && lane < 3) prefetch_tmap(lane == 0 ? &tmQ : lane == 1 ? &tmK : &tmV);
+  if (tid == 64) {
+    for (int u = 0; u < U; ++u) {
+      mbar_init(&bars->full[u], 1);
+      mbar_init(&bars->empty[u], 1);
+    }
+    mbar_init(&bars->q_full, 1);
+    mbar_init(&bars->q_empty, 1);
+    for (int i = 0; i < kPieces; ++i) mbar_init(&bars->info[i], 1);
+    for (int g = 0; g < 2; ++g) {
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&bars->s_full[g][b], 1);
+        mbar_init(&bars->p_full[g][b], 4);
+        mbar_init(&bars->pv_done[g][b], 1);
+      }
+    }
+    mbar_fence_init();
+  }
+  if (tid < 4 * 2 * 16 * 2) (&bars->bad[0][0][0][0])[tid] = 0;
+  if (tid < 8) bars->any_bad[tid >> 1][tid & 1] = 0;
+  if (warp == 1) {
+    tmem_alloc(&bars->tmem_base, 512);
+    tmem_relinquish();
+  }
   long incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -286,167 +306,208 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
     if (lane >= o) incl += v;
   }
   if (lane == 31) bars->part[warp] = incl;
+  tc_fence_before();
   __syncthreads();
+  tc_fence_after();
   long total = 0;
 #pragma unroll
   for (int i = 0; i < kTcThreads / 32; ++i) {
     if (i < warp) incl += bars->part[i];
     total += bars->part[i];
   }
-  const long ctas = max(1l, min(long(gridDim.x), total / p.min_tiles));
-  const long w0 = blockIdx.x * total / ctas, w1 = (blockIdx.x + 1) * total / ctas;
-  if (long(blockIdx.x) >= ctas || w0 >= w1) {
-    if (tid == 0) p.ws_desc[blockIdx.x * 8 + DESC_MERGE] = 0;
-    return;
-  }
-  if (incl - mine <= w0 && w0 < incl) {
+  const long ctas = max(1l, min(long(gridDim.x), total / p.min_work));
+  const long w0 = blockIdx.x * total / ctas, w1 = min(total, (blockIdx.x + 1) * total / ctas);
+  const bool busy = long(blockIdx.x) < ctas && w0 < w1;
+  if (!busy && tid == 0) p.ws_desc[blockIdx.x * 8 + DESC_MERGE] = 0;
+  if (busy && incl - mine <= w0 && w0 < incl) {
     long at = incl - mine;
     for (int s = s0; s < s1; ++s) {
-      const long n = load_seq(a, s, per_item).tiles(a.n_kv);
+      const long n = load_seq(a, s, per_item).work(a.n_kv);
       if (w0 < at + n) {
         bars->seq = s;
-        bars->seq_tiles = at;
+        bars->seq_work = at;
         break;
       }
       at += n;
     }
   }
-  if (tid == 0) {
-    for (int u = 0; u < U; ++u) {
-      mbar_init(&bars->full[u], 1);
-      mbar_init(&bars->empty[u], 1);
-    }
-    mbar_init(&bars->q_full, 1);
-    mbar_init(&bars->q_empty, 1);
-    for (int g = 0; g < 2; ++g) {
-      for (int b = 0; b < 2; ++b) {
-        mbar_init(&bars->s_full[g][b], 1);
-        mbar_init(&bars->s_free[g][b], 4);
-      }
-      mbar_init(&bars->p_full[g], 4);
-      mbar_init(&bars->pv_done[g], 1);
-    }
-    mbar_fence_init();
-  }
-  for (int i = tid; i < 4 * 2 * 16 * 2; i += kTcThreads) (&bars->bad[0][0][0][0])[i] = 0;
-  if (tid < 4) bars->any_bad[tid] = 0;
-  if (warp == 1) {
-    tmem_alloc(&bars->tmem_base, 512);
-    tmem_relinquish();
-  }
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = bars->tmem_base;                     // group g: S buffers at g * 256 + {0, 64}, O at g * 256 + 128
-  Walk x;
-  x.start(p, bars, w0, w1, per_item);
+  const uint32_t tmem = bars->tmem_base;                     // group g: S / P buffers at g * 256 + {0, 64}, O at g * 256 + 128
 
   if (warp == 0) {
     // ---------------------------------------------------------- TMA producer (whole warp: lanes share the boxes)
-    if (lane == 0) {
-      prefetch_tmap(&tmQ);
-      prefetch_tmap(&tmK);
-      prefetch_tmap(&tmV);
-    }
     const int boxes = BKV / p.box_tokens, per_unit = boxes * QS;       // boxes of a 64-column slab; at most 8 x 2
     const int slab = lane / boxes, bx = lane % boxes;
-    const long num_slots = a.num_slots;
     bool ok = true;
-    int u = 0;
-    for (int piece = 0; ok && x.next(p, per_item); ++piece) {
-      if (lane == 0) {
-        ok = mbar_wait(&bars->q_empty, (piece & 1) ^ 1);
-        if (ok) {
-          const int tiles = PAIR && x.q.n - x.node0 > p.nodes ? 2 : 1;
-          mbar_arrive_expect_tx(&bars->q_full, uint32_t(tiles * QS * 128 * p.group * p.nodes));
-          for (int h = 0; h < tiles; ++h)
-#pragma unroll
-            for (int sl = 0; sl < QS; ++sl)
-              tma_load_3d(sQ + h * C::Q_BYTES + sl * Q_SLAB, &tmQ, &bars->q_full, sl * 64, x.head * p.group, x.q.q_start + x.node0 + h * p.nodes);
-        }
-      }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      const int* bt = a.block_tables + size_t(x.seq) * a.max_blocks;
-      auto unit = [&](const CUtensorMap* map, int j) {
-        long slot = 0;
-        if (lane < per_unit) {
-          const int tok = x.key0(j) + bx * p.box_tokens, bi = min(tok / a.block_size, a.max_blocks - 1);
-          slot = long(bt[bi]) * a.block_size + tok % a.block_size;
-          if (slot < 0 || slot + p.box_tokens > num_slots) slot = 0;   // places behind the last row
-        }
-        const int st = u % U;
+    int st = 0, phase = 0, count = 0;
+    Piece x;
+    long w = w0;                                                       // work ahead of the current item
+    int row = 0;
+    if (busy) {
+      x.seq = bars->seq;
+      x.q = load_seq(a, x.seq, per_item);
+      const int item = int((w0 - bars->seq_work) / x.q.item());
+      w = bars->seq_work + long(item) * x.q.item();
+      x.head = item / x.q.row_tiles;
+      row = item - x.head * x.q.row_tiles;
+    }
+    while (ok && busy && w < w1) {
+      // the part of the item that lies in the stretch
+      const long ahead = w0 - w - kItemCost, behind = w1 - w - kItemCost;
+      x.j0 = int(max(ahead, 0l));
+      x.nt = int(min(behind, long(x.q.key_tiles))) - x.j0;
+      if (x.nt > 0) {
+        x.node0 = row * per_item;
+        x.pair = NQ == 2 && x.q.n - x.node0 > p.nodes;
+        x.whole = x.nt == x.q.key_tiles;
+        x.slot = 2 * blockIdx.x + (count > 0);
+        const int info = count % kPieces;
         if (lane == 0) {
-          ok = mbar_wait(&bars->empty[st], ((u / U) & 1) ^ 1);
-          if (ok) mbar_arrive_expect_tx(&bars->full[st], UNIT);
+          if (count == 0) {
+            int* d = p.ws_desc + blockIdx.x * 8;
+            const bool merge = x.j0 > 0 && x.j0 + x.nt == x.q.key_tiles;
+            d[DESC_MERGE] = merge;
+            if (merge) {
+              const long first = ((w + kItemCost + 1) * ctas - 1) / total;      // CTA of the item's first tile
+              d[DESC_FIRST] = int(first);
+              d[DESC_SLOT] = int(2 * first + (first * total / ctas < w ? 1 : 0));
+              d[DESC_START] = x.q.q_start + x.node0;
+              d[DESC_NODES] = min(per_item, x.q.n - x.node0);
+              d[DESC_HEAD] = x.head;
+            }
+          }
+          ok = mbar_wait(&bars->q_empty, (count & 1) ^ 1);
+          if (ok) {
+            bars->piece[info] = x;
+            mbar_arrive(&bars->info[info]);
+            const int tiles = x.pair ? 2 : 1;
+            mbar_arrive_expect_tx(&bars->q_full, uint32_t(tiles * QS * 128 * p.group * p.nodes));
+            for (int h = 0; h < tiles; ++h)
+#pragma unroll
+              for (int sl = 0; sl < QS; ++sl)
+                tma_load_3d(sQ + h * C::Q_BYTES + sl * Q_SLAB, &tmQ, &bars->q_full, sl * 64, x.head * p.group, x.q.q_start + x.node0 + h * p.nodes);
+          }
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (ok && lane < per_unit)
-          tma_load_3d(ring + st * UNIT + slab * KV_SLAB + bx * p.box_tokens * 128, map, &bars->full[st], slab * 64, x.head, int(slot));
-        __syncwarp();
-        ++u;
-      };
-      for (int j = 0; ok && j < x.nt + LAG; ++j) {
-        if (j < x.nt) unit(&tmK, j);
-        if (ok && j >= LAG) unit(&tmV, j - LAG);
+        ++count;
+        // a lane's place in tile j; the values of a tile are fetched `lag` tiles after its keys, from the same places
+        const int* bt = a.block_tables + size_t(x.seq) * a.max_blocks;
+        auto place = [&](int j) {
+          const int tok = x.key0(j) + bx * p.box_tokens;
+          const int blk = p.block_shift >= 0 ? tok >> p.block_shift : tok / a.block_size;
+          const long slot = long(bt[min(blk, a.max_blocks - 1)]) * a.block_size + (tok - blk * a.block_size);
+          return slot < 0 || slot + p.box_tokens > a.num_slots ? 0 : int(slot);  // places behind the last row
+        };
+        auto unit = [&](const CUtensorMap* map, int slot) {
+          if (lane == 0) {
+            ok = mbar_wait(&bars->empty[st], phase ^ 1);
+            if (ok) mbar_arrive_expect_tx(&bars->full[st], UNIT);
+          }
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+          if (ok && lane < per_unit)
+            tma_load_3d(ring + st * UNIT + slab * KV_SLAB + bx * p.box_tokens * 128, map, &bars->full[st], slab * 64, x.head, slot);
+          if (++st == U) {
+            st = 0;
+            phase ^= 1;
+          }
+        };
+        const int lag = x.pair ? 1 : 2;
+        int next = lane < per_unit ? place(0) : 0, held0 = 0, held1 = 0;
+        for (int j = 0; ok && j < x.nt + lag; ++j) {
+          const int slot = next;
+          if (j < x.nt) {
+            if (lane < per_unit && j + 1 < x.nt) next = place(j + 1);
+            unit(&tmK, slot);
+          }
+          if (ok && j >= lag && j - lag < x.nt) unit(&tmV, lag == 1 ? held0 : held1);
+          held1 = held0;
+          held0 = slot;
+        }
+      }
+      w += x.q.item();
+      if (++row == x.q.row_tiles) {
+        row = 0;
+        if (++x.head == a.n_kv) {
+          x.head = 0;
+          if (w < w1)
+            do x.q = load_seq(a, ++x.seq, per_item);
+            while (x.q.row_tiles == 0);
+        }
       }
     }
-    if (!ok && lane == 0) atomicExch(p.status, XL_ERR_WAIT_EMPTY);
+    if (lane == 0) {
+      bars->piece[count % kPieces].nt = 0;
+      mbar_arrive(&bars->info[count % kPieces]);
+      if (busy && count == 0) p.ws_desc[blockIdx.x * 8 + DESC_MERGE] = 0;
+      if (!ok) atomicExch(p.status, XL_ERR_WAIT_EMPTY);
+    }
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
     if (elect_one_sync()) {
       const uint32_t idesc_s = umma_idesc_f16(BQ, BKV, 1), idesc_o = umma_idesc_f16(BQ, DV, 1) | (1u << 16);   // V is MN-major
-      const uint32_t q_addr = smem_u32(sQ), ring_addr = smem_u32(ring), p_addr = smem_u32(sP);
+      // descriptors count in units of 16 bytes: a step along a tile is an addition
+      const uint64_t q_desc = umma_desc_sw128(smem_u32(sQ), 0), k_desc = umma_desc_sw128(smem_u32(ring), 0);
+      const uint64_t v_desc = umma_desc_sw128_mn(smem_u32(ring), KV_SLAB, 1024);
       bool ok = true;
-      int u0 = 0, s_count[2] = {0, 0}, p_count[2] = {0, 0};
-      for (int piece = 0; ok && x.next(p, per_item); ++piece) {
-        const int nt = x.nt, groups = PAIR && x.q.n - x.node0 > p.nodes ? 2 : 1;
-        ok = mbar_wait(&bars->q_full, piece & 1);
-        for (int j = 0; ok && j < nt + LAG; ++j) {
+      int st = 0, phase = 0, s_count[2] = {0, 0}, p_count[2] = {0, 0};
+      auto take = [&] {                                                // the next unit
+        ok = mbar_wait(&bars->full[st], phase);
+        return ok;
+      };
+      auto leave = [&] {
+        tc_commit(&bars->empty[st]);
+        if (++st == U) {
+          st = 0;
+          phase ^= 1;
+        }
+      };
+      for (int count = 0;; ++count) {
+        const int info = count % kPieces;
+        if (!(ok = mbar_wait(&bars->info[info], (count / kPieces) & 1))) break;
+        const int nt = bars->piece[info].nt;
+        if (nt == 0) break;
+        const bool pair = NQ == 2 && bars->piece[info].pair;
+        const int lag = pair ? 1 : 2;
+        ok = mbar_wait(&bars->q_full, count & 1);
+        for (int j = 0; ok && j < nt + lag; ++j) {
           if (j < nt) {
-            const int u = u0 + k_unit<LAG>(j), st = u % U;
-            if (!(ok = mbar_wait(&bars->full[st], (u / U) & 1))) break;
-            const uint32_t k_addr = ring_addr + st * UNIT;
+            if (!take()) break;
+            tc_fence_after();
+            const uint64_t k0 = k_desc + st * (UNIT / 16);
 #pragma unroll
-            for (int h = 0; h < (PAIR ? 2 : 1); ++h) {
-              if (h >= groups) break;
-              const int g = PAIR ? h : j & 1;
-              int& n = s_count[g];
-              const int b = n & 1;
-              if (!(ok = mbar_wait(&bars->s_free[g][b], ((n >> 1) & 1) ^ 1))) break;
-              ++n;
-              tc_fence_after();
+            for (int h = 0; h < NQ; ++h) {
+              if (h == 1 && !pair) break;
+              const int g = pair ? h : j & 1, b = s_count[g]++ & 1;
 #pragma unroll
               for (int k = 0; k < DV / 16; ++k)
-                tc_mma_f16(tmem + g * 256 + b * 64, umma_desc_sw128(q_addr + h * C::Q_BYTES + (k >> 2) * Q_SLAB, (k & 3) * 32),
-                           umma_desc_sw128(k_addr + (k >> 2) * KV_SLAB, (k & 3) * 32), idesc_s, k != 0);
+                tc_mma_f16(tmem + g * 256 + b * 64, q_desc + (h * C::Q_BYTES + (k >> 2) * Q_SLAB) / 16 + (k & 3) * 2,
+                           k0 + (k >> 2) * (KV_SLAB / 16) + (k & 3) * 2, idesc_s, k != 0);
               tc_commit(&bars->s_full[g][b]);
             }
-            if (!ok) break;
-            tc_commit(&bars->empty[st]);
+            leave();
             if (j == nt - 1) tc_commit(&bars->q_empty);
           }
-          if (j >= LAG && j - LAG < nt) {
-            const int i = j - LAG, u = u0 + v_unit<LAG>(i, nt), st = u % U;
-            if (!(ok = mbar_wait(&bars->full[st], (u / U) & 1))) break;
-            const uint32_t v_addr = ring_addr + st * UNIT;
+          if (j >= lag && j - lag < nt) {
+            const int i = j - lag;
+            if (!take()) break;
+            const uint64_t v0 = v_desc + st * (UNIT / 16);
 #pragma unroll
-            for (int h = 0; h < (PAIR ? 2 : 1); ++h) {
-              if (h >= groups) break;
-              const int g = PAIR ? h : i & 1;
-              if (!(ok = mbar_wait(&bars->p_full[g], p_count[g] & 1))) break;
+            for (int h = 0; h < NQ; ++h) {
+              if (h == 1 && !pair) break;
+              const int g = pair ? h : i & 1, b = p_count[g] & 1;
+              if (!(ok = mbar_wait(&bars->p_full[g][b], (p_count[g] >> 1) & 1))) break;
               ++p_count[g];
               tc_fence_after();
 #pragma unroll
               for (int k = 0; k < BKV / 16; ++k)
-                tc_mma_f16(tmem + g * 256 + 128, umma_desc_sw128(p_addr + g * P_BYTES, k * 32),
-                           umma_desc_sw128_mn(v_addr + k * 2048, KV_SLAB, 1024), idesc_o, ((PAIR ? i : i >> 1) | k) != 0);
-              tc_commit(&bars->pv_done[g]);
+                tc_mma_f16_ts(tmem + g * 256 + 128, tmem + g * 256 + b * 64 + k * 8, v0 + k * (2048 / 16), idesc_o, ((pair ? i : i >> 1) | k) != 0);
+              tc_commit(&bars->pv_done[g][b]);
             }
             if (!ok) break;
-            tc_commit(&bars->empty[st]);
+            leave();
           }
         }
-        u0 += 2 * nt;
+        if (!ok) break;
       }
       if (!ok) atomicExch(p.status, XL_ERR_WAIT_FULL);
     }
@@ -454,42 +515,47 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
     // ---------------------------------------------------------- softmax, one row per thread
     const int g = (warp - 2) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const int gt = (warp - 2 - 4 * g) * 32 + lane;                     // thread of the group
-    const uint32_t t_s = tmem + g * 256 + (uint32_t(quarter * 32) << 16), t_o = t_s + 128;
-    uint8_t* prow = sP + g * P_BYTES + r * 128;
+    const uint32_t t_lane = tmem + (uint32_t(quarter * 32) << 16), t_s = t_lane + g * 256, t_o = t_s + 128;
     const int node = r / p.group, head_in = r - node * p.group;
     const float sc = p.scale_log2;
-    const int flags = PAIR ? 0 : g;                                    // whose flags hold for this group's keys
     auto group_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory"); };
     auto both_sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+    // rows of no sequence
+    {
+      const int behind = max(a.q_cu[a.B], 0), width = a.n_q * a.D;
+      for (long t = long(behind) + blockIdx.x; t < a.T; t += gridDim.x)
+        for (int c = tid - 64; c < width / 8; c += 256) reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + t * width)[c] = make_uint4(0, 0, 0, 0);
+    }
     bool ok = true;
     int u0 = 0, count = 0;                                             // units ahead of the piece; tiles of this group so far
-    for (int piece = 0; x.next(p, per_item); ++piece) {
+    for (int piece = 0;; ++piece) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&bars->info[piece % kPieces], (piece / kPieces) & 1))) {
+        ok = false;
+        break;
+      }
+      const Piece& x = bars->piece[piece % kPieces];
       const int nt = x.nt;
-      const bool idle = PAIR && g == 1 && x.q.n - x.node0 <= p.nodes;  // the second row tile is empty
-      const int my_node = x.node0 + (PAIR ? g * p.nodes : 0) + node;
+      if (nt == 0) break;
+      const bool pair = NQ == 2 && x.pair;
+      const int lag = pair ? 1 : 2, owner = pair ? 0 : g;              // owner: whose flags hold for this group's keys
+      const int my_node = x.node0 + (pair ? g * p.nodes : 0) + node;
       const bool valid = node < p.nodes && my_node < x.q.n;
       const bool warp_valid = __any_sync(0xffffffffu, valid);
       const int t = x.q.q_start + (valid ? my_node : 0);
-      const int pos = valid ? a.positions[t] : 0;
+      const int pos = valid && a.window > 0 ? a.positions[t] : 0;
       float m_ref = -INFINITY, l_run = 0.f;
       int done = 0;                                                    // tiles of this group in this piece
       // (a group whose wait ran out goes on without waiting, so that the others still meet it at the barriers)
-      for (int j = PAIR ? 0 : g; j < nt && !idle; j += PAIR ? 1 : 2, ++done, ++count) {
+      for (int j = pair ? 0 : g; j < nt; j += pair ? 1 : 2, ++done, ++count) {
         const int b = count & 1, kv0 = x.key0(j);
         if (ok && !__all_sync(0xffffffffu, mbar_wait(&bars->s_full[g][b], (count >> 1) & 1))) ok = false;
         tc_fence_after();
-        uint32_t pk[32];
-        bool rescale = false;
-        float alpha = 1.f;
         const bool partly = x.partly(a, kv0);
         if (warp_valid) {
           uint32_t s0[32], s1[32];
           tmem_ld_32x32(t_s + b * 64, s0);
           tmem_ld_32x32(t_s + b * 64 + 32, s1);
           tc_wait_ld();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->s_free[g][b]);
           float v[64];
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
@@ -505,97 +571,90 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
               if (!(hi >> c & 1u)) v[32 + c] = -INFINITY;
             }
           }
-          float mx8[8];
+          float mx4[4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) mx8[i] = v[i];
+          for (int i = 0; i < 4; ++i) mx4[i] = fmaxf(v[i], v[i + 4]);
 #pragma unroll
-          for (int c = 8; c < 64; ++c) mx8[c & 7] = fmaxf(mx8[c & 7], v[c]);
-          const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])), fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+          for (int c = 8; c < 64; c += 8)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx4[i] = max3(mx4[i], v[c + i], v[c + 4 + i]);
+          const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]);
           // the reference stays unless the scaled maximum grew by more than 8: P stays below 2^8
           const bool had = m_ref != -INFINITY;
           const bool grow = (mx - m_ref) * sc > 8.f || (!had && mx != -INFINITY);
           const float m_new = grow ? mx : m_ref;
-          rescale = grow && had;
-          alpha = rescale ? fast_exp2((m_ref - m_new) * sc) : 1.f;
+          const bool rescale = grow && had;
+          const float alpha = rescale ? fast_exp2((m_ref - m_new) * sc) : 1.f;
           m_ref = m_new;
           const float mneg = m_ref == -INFINITY ? 0.f : -m_ref * sc;
-          float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint64_t sc2 = pack2(sc, sc), mneg2 = pack2(mneg, mneg);
+          uint64_t sum2[4] = {0, 0, 0, 0};
+          uint32_t pk[32];
 #pragma unroll
           for (int c = 0; c < 64; c += 2) {
-            const float e0 = fast_exp2(fmaf(v[c], sc, mneg)), e1 = fast_exp2(fmaf(v[c + 1], sc, mneg));
-            sum4[(c >> 1) & 3] += e0 + e1;
+            const float2 z = unpack2(fma2(pack2(v[c], v[c + 1]), sc2, mneg2));
+            const float e0 = fast_exp2(z.x), e1 = fast_exp2(z.y);
+            sum2[(c >> 1) & 3] = add2(sum2[(c >> 1) & 3], pack2(e0, e1));
             pk[c >> 1] = pack_bf16x2(e0, e1);
           }
-          l_run = l_run * alpha + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
-        } else {
-          tc_fence_before();
-          if (lane == 0) mbar_arrive(&bars->s_free[g][b]);
-        }
-        // P and O are touched only after P V of this group's tile before
-        if (ok && done > 0 && !__all_sync(0xffffffffu, mbar_wait(&bars->pv_done[g], (count - 1) & 1))) ok = false;
-        tc_fence_after();
-        if (done > 0 && __any_sync(0xffffffffu, rescale)) {
+          const float2 sum = unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])));
+          l_run = l_run * alpha + (sum.x + sum.y);
+          tmem_st_32x32(t_s + b * 64, pk);
+          if (done > 0 && __any_sync(0xffffffffu, rescale)) {
+            // O is at rest once P V of this group's tile before has run
+            if (ok && !__all_sync(0xffffffffu, mbar_wait(&bars->pv_done[g][(count - 1) & 1], ((count - 1) >> 1) & 1))) ok = false;
+            tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < DV; c += 32) {
-            uint32_t o[32];
-            tmem_ld_32x32(t_o + c, o);
-            tc_wait_ld();
+            for (int c = 0; c < DV; c += 32) {
+              uint32_t o[32];
+              tmem_ld_32x32(t_o + c, o);
+              tc_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            tmem_st_32x32(t_o + c, o);
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st_32x32(t_o + c, o);
+            }
           }
           tc_wait_st();
         }
-        if (warp_valid) {
-          // 16-byte chunk c of row r at chunk c ^ (r & 7)
-#pragma unroll
-          for (int c = 0; c < 8; ++c)
-            *reinterpret_cast<uint4*>(prow + ((c ^ (r & 7)) << 4)) = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
-        }
-        if (partly && flags == g) {
+        if (partly && owner == g) {
           // two threads look at the values of one key
-          const int u = u0 + v_unit<LAG>(j, nt), st = u % U, key = gt >> 1;
+          const int u = u0 + v_unit(j, lag, nt), st = u % U, key = gt >> 1;
           if (ok && !__all_sync(0xffffffffu, mbar_wait(&bars->full[st], (u / U) & 1))) ok = false;
           uint4* row = reinterpret_cast<uint4*>(ring + st * UNIT + key * 128 + (gt & 1) * 64);
           bool bad = false;
-          if (ok) {
 #pragma unroll
-            for (int sl = 0; sl < QS; ++sl)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                uint4* at = row + sl * (KV_SLAB / 16) + i;
-                if (kv0 + key >= x.q.kv_len) {
-                  *at = make_uint4(0, 0, 0, 0);
-                } else {
-                  uint4 w = *at;
-                  if (not_finite(w.x) || not_finite(w.y) || not_finite(w.z) || not_finite(w.w)) {
-                    auto clean = [](uint32_t v) { return ((v & 0x7F800000u) == 0x7F800000u ? 0 : v & 0xFFFF0000u) | ((v & 0x7F80u) == 0x7F80u ? 0 : v & 0xFFFFu); };
-                    *at = make_uint4(clean(w.x), clean(w.y), clean(w.z), clean(w.w));
-                    bad = true;
-                  }
-                }
+          for (int i = 0; i < 4 * QS; ++i) {
+            uint4* at = row + (i >> 2) * (KV_SLAB / 16) + (i & 3);
+            if (kv0 + key >= x.q.kv_len) {
+              *at = make_uint4(0, 0, 0, 0);
+            } else {
+              const uint4 v = *at;
+              if (not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w)) {
+                *at = make_uint4(finite_part(v.x), finite_part(v.y), finite_part(v.z), finite_part(v.w));
+                bad = true;
               }
+            }
           }
           if (bad) {
             atomicOr(&bars->bad[piece & 3][g][x.tile_number(kv0)][key >> 5], 1u << (key & 31));
-            bars->any_bad[piece & 3] = 1;
+            bars->any_bad[piece & 3][g] = 1;
           }
+          fence_proxy_async_smem();
           group_sync();
         }
-        fence_proxy_async_smem();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->p_full[g]);
+        if (lane == 0) mbar_arrive(&bars->p_full[g][b]);
       }
-      if (ok && done > 0 && !__all_sync(0xffffffffu, mbar_wait(&bars->pv_done[g], (count - 1) & 1))) ok = false;
+      if (ok && done > 0 && !__all_sync(0xffffffffu, mbar_wait(&bars->pv_done[g][(count - 1) & 1], ((count - 1) >> 1) & 1))) ok = false;
       tc_fence_after();
       u0 += 2 * nt;
       // ------------------------------------------------ end of a piece
-      if (ok && done > 0 && warp_valid && bars->any_bad[piece & 3]) {
+      if (ok && done > 0 && warp_valid && bars->any_bad[piece & 3][owner]) {
         // values that are not finite join the rows that see them
         for (int i = 0; i < 16 * 64; ++i) {
           const int tile = i >> 6, k = i & 63;
-          if (!(bars->bad[piece & 3][flags][tile][k >> 5] >> (k & 31) & 1u)) continue;
+          if (!(bars->bad[piece & 3][owner][tile][k >> 5] >> (k & 31) & 1u)) continue;
           const int kv0 = tile >= 8 ? x.q.base / BKV * BKV + (tile - 8) * BKV : x.q.kv_begin + tile * BKV, key = kv0 + k;
           const bool see = valid && (seen_keys(a, x.q, t, pos, kv0) >> k & 1ull);
           const long slot = long(a.block_tables[size_t(x.seq) * a.max_blocks + key / a.block_size]) * a.block_size + key % a.block_size;
@@ -615,91 +674,68 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
           tc_wait_st();
         }
       }
-      const bool whole = x.whole();
-      const int slot = 2 * blockIdx.x + (piece > 0);
-      const int ws_row = PAIR ? g * BQ + r : r;
       const float m_log2 = m_ref == -INFINITY ? -INFINITY : m_ref * sc;
-      // the weights of the two groups' sums (PAIR: its own alone), and the columns that this group stores
+      // weights of the two groups' sums (two row tiles: its own alone), and the columns that this group stores
       float wa = 1.f, wb = 0.f, m_all = m_log2, l_all = l_run;
       int c_lo = 0, c_hi = DV;
-      bool use_a = done > 0, use_b = false;                            // a: group 0 (PAIR: this group)
       uint32_t t_oa = t_o;
-      const uint32_t t_ob = tmem + 256 + 128 + (uint32_t(quarter * 32) << 16);
-      if (!PAIR) {
+      if (!pair) {
         bars->ml[g][r] = make_float2(m_log2, l_run);
         tc_fence_before();
         both_sync();
         tc_fence_after();
-        const float2 other = bars->ml[g ^ 1][r];
-        const float ma = g == 0 ? m_log2 : other.x, mb = g == 0 ? other.x : m_log2, la = g == 0 ? l_run : other.y, lb = g == 0 ? other.y : l_run;
-        m_all = fmaxf(ma, mb);
-        wa = ma == -INFINITY ? (la != la ? la : 0.f) : fast_exp2(ma - m_all);
-        wb = mb == -INFINITY ? (lb != lb ? lb : 0.f) : fast_exp2(mb - m_all);
-        l_all = la * wa + lb * wb;
-        use_a = true;
-        use_b = nt > 1;
-        t_oa = tmem + 128 + (uint32_t(quarter * 32) << 16);
+        const float2 fa = bars->ml[0][r], fb = bars->ml[1][r];
+        m_all = fmaxf(fa.x, fb.x);
+        // a group whose row saw nothing has nothing to add, unless its scores were not numbers
+        wa = fa.x == -INFINITY ? (fa.y != fa.y ? fa.y : 0.f) : fast_exp2(fa.x - m_all);
+        wb = fb.x == -INFINITY ? (fb.y != fb.y ? fb.y : 0.f) : fast_exp2(fb.x - m_all);
+        l_all = fa.y * wa + fb.y * wb;
+        t_oa = t_lane + 128;
         c_lo = g * (DV / 2);
         c_hi = c_lo + DV / 2;
       }
-      if (ok && use_a && warp_valid) {
+      if (ok && warp_valid) {
+        const bool whole = x.whole, two = !pair && nt > 1;
+        const int ws_row = pair ? g * BQ + r : r;
         const float inv = l_all != 0.f ? 1.f / l_all : 0.f;            // a row that sees nothing: zeros
         __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + size_t(t) * (size_t(a.n_q) * a.D) + (x.head * p.group + head_in) * a.D;
-        float4* wo = p.ws_o + size_t(slot) * (DV / 4) * C::kRows + ws_row;
+        float4* wo = p.ws_o + size_t(x.slot) * (DV / 4) * C::kRows + ws_row;
         const float fa = whole ? wa * inv : wa, fb = whole ? wb * inv : wb;
-#pragma unroll
+#pragma unroll 1
         for (int c = c_lo; c < c_hi; c += 32) {
-          uint32_t oa[32];
+          uint32_t oa[32], ob[32];
           tmem_ld_32x32(t_oa + c, oa);
+          if (two) tmem_ld_32x32(t_lane + 256 + 128 + c, ob);
           tc_wait_ld();
           float f[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(oa[i]) * fa;
-          if (use_b) {
-            tmem_ld_32x32(t_ob + c, oa);
-            tc_wait_ld();
+          if (two) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) f[i] = fmaf(__uint_as_float(oa[i]), fb, f[i]);
+            for (int i = 0; i < 32; ++i) f[i] = fmaf(__uint_as_float(ob[i]), fb, f[i]);
           }
-          if (valid) {
-            if (whole) {
+          if (valid && whole) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (c + 8 * i < a.D)
-                  *reinterpret_cast<uint4*>(dst + c + 8 * i) = make_uint4(pack_bf16x2(f[8 * i], f[8 * i + 1]), pack_bf16x2(f[8 * i + 2], f[8 * i + 3]),
-                                                                          pack_bf16x2(f[8 * i + 4], f[8 * i + 5]), pack_bf16x2(f[8 * i + 6], f[8 * i + 7]));
-            } else {
+            for (int i = 0; i < 32; i += 8)
+              if (c + i < a.D)
+                *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(pack_bf16x2(f[i], f[i + 1]), pack_bf16x2(f[i + 2], f[i + 3]),
+                                                                    pack_bf16x2(f[i + 4], f[i + 5]), pack_bf16x2(f[i + 6], f[i + 7]));
+          } else if (valid) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) wo[size_t(c / 4 + i) * C::kRows] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
-            }
+            for (int i = 0; i < 32; i += 4) wo[size_t((c + i) / 4) * C::kRows] = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
           }
         }
-        if (valid && !whole && (PAIR || g == 0)) p.ws_ml[size_t(slot) * C::kRows + ws_row] = make_float2(m_all, l_all);
+        if (valid && !whole && (pair || g == 0)) p.ws_ml[size_t(x.slot) * C::kRows + ws_row] = make_float2(m_all, l_all);
       }
       // the next piece's flags were last read three pieces ago
-      if (flags == g) {
-        for (int i = gt; i < 32; i += 128) (&bars->bad[(piece + 1) & 3][g][0][0])[i] = 0;
-        if (gt == 0 && g == 0) bars->any_bad[(piece + 1) & 3] = 0;
+      if (bars->any_bad[(piece + 1) & 3][g]) {
+        if (gt < 32) (&bars->bad[(piece + 1) & 3][g][0][0])[gt] = 0;
+        group_sync();
+        if (gt == 0) bars->any_bad[(piece + 1) & 3][g] = 0;
         group_sync();
       }
-      if (!PAIR) {
-        tc_fence_before();
-        both_sync();                                                   // both groups have read O and the maxima
-      }
-      if (piece == 0 && tid == 64) {
-        int* d = p.ws_desc + blockIdx.x * 8;
-        const bool merge = x.j0 > 0 && x.j0 + nt == x.q.key_tiles;
-        d[DESC_MERGE] = merge;
-        if (merge) {
-          const long start = x.w - x.j0;                               // the item's first tile
-          const long first = ((start + 1) * ctas - 1) / total;
-          d[DESC_FIRST] = int(first);
-          d[DESC_SLOT] = int(2 * first + (first * total / ctas == start ? 0 : 1));
-          d[DESC_START] = x.q.q_start + x.node0;
-          d[DESC_NODES] = min(per_item, x.q.n - x.node0);
-          d[DESC_HEAD] = x.head;
-        }
-      }
+      tc_fence_before();
+      if (!pair) both_sync();                                          // both groups have read O and the maxima
     }
     if (!ok && lane == 0) atomicExch(p.status, XL_ERR_WAIT_TMEM_FULL);
   }
@@ -709,56 +745,72 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
 }
 
 // Joins the partials of the item that ends in CTA blockIdx.x's first piece: o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i.
-template <int QS, bool PAIR>
-__global__ void __launch_bounds__(256) attention_tree_merge_kernel(const TcParams p) {
-  using C = Cfg<QS, PAIR>;
+// Four parts at a time are fetched together, so that the chain of loads is short.
+template <int QS, int NQ>
+__global__ void __launch_bounds__(128) attention_tree_merge_kernel(const TcParams p) {
+  using C = Cfg<QS, NQ>;
   const Params& a = p.a;
   grid_dep_wait();
-  const int* d = p.ws_desc + blockIdx.x * 8;
-  if (!d[DESC_MERGE]) return;
-  const int first = d[DESC_FIRST], slot0 = d[DESC_SLOT], parts = int(blockIdx.x) - first + 1, nodes = d[DESC_NODES], rows = nodes * p.group;
-  const int c4 = a.D / 4, items = rows * c4;
-  for (int i = blockIdx.y * 256 + threadIdx.x; i < items; i += gridDim.y * 256) {
+  const int4 d0 = __ldcg(reinterpret_cast<const int4*>(p.ws_desc) + blockIdx.x * 2), d1 = __ldcg(reinterpret_cast<const int4*>(p.ws_desc) + blockIdx.x * 2 + 1);
+  if (!d0.x) return;
+  const int first = d0.y, slot0 = d0.z, start = d0.w, rows = d1.x * p.group, head = d1.y;
+  const int parts = int(blockIdx.x) - first + 1, items = rows * (a.D / 4);
+  for (int i = blockIdx.y * 128 + threadIdx.x; i < items; i += gridDim.y * 128) {
     const int row = i % rows, c = i / rows;                            // neighbours share a column group: partials are read side by side
     const int node = row / p.group, h = row - node * p.group;
-    const int tile = PAIR ? node / p.nodes : 0;
+    const int tile = NQ == 2 && node >= p.nodes ? 1 : 0;
     const int ws_row = tile * BQ + (node - tile * p.nodes) * p.group + h;
-    float m = -INFINITY;
-    for (int k = 0; k < parts; ++k) m = fmaxf(m, __ldcg(&p.ws_ml[size_t(k == 0 ? slot0 : 2 * (first + k)) * C::kRows + ws_row]).x);
-    float l = 0.f;
+    float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < parts; ++k) {
-      const size_t slot = k == 0 ? slot0 : 2 * (first + k);
-      const float2 ml = __ldcg(&p.ws_ml[slot * C::kRows + ws_row]);
-      if (ml.x == -INFINITY && ml.y == 0.f) continue;                  // sees no key of that part
-      const float w = ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - m);
-      const float4 v = __ldcg(&p.ws_o[(slot * (C::DV / 4) + c) * C::kRows + ws_row]);
-      l += w * ml.y;
-      o.x += w * v.x; o.y += w * v.y; o.z += w * v.z; o.w += w * v.w;
+    for (int k0 = 0; k0 < parts; k0 += 4) {
+      float2 ml[4];
+      float4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const size_t slot = k0 + k == 0 ? slot0 : 2 * (first + k0 + k);
+        ml[k] = make_float2(-INFINITY, 0.f);
+        if (k0 + k < parts) {
+          ml[k] = __ldcg(&p.ws_ml[slot * C::kRows + ws_row]);
+          v[k] = __ldcg(&p.ws_o[(slot * (C::DV / 4) + c) * C::kRows + ws_row]);
+        }
+      }
+      const float m_new = fmaxf(fmaxf(m, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
+      const float w0 = m == -INFINITY ? 1.f : fast_exp2(m - m_new);
+      l *= w0;
+      o.x *= w0; o.y *= w0; o.z *= w0; o.w *= w0;
+      m = m_new;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (ml[k].x == -INFINITY && ml[k].y == 0.f) continue;          // sees no key of that part
+        const float w = ml[k].x == -INFINITY ? 1.f : fast_exp2(ml[k].x - m);
+        l += w * ml[k].y;
+        o.x += w * v[k].x; o.y += w * v[k].y; o.z += w * v[k].z; o.w += w * v[k].w;
+      }
     }
     const float inv = l != 0.f ? 1.f / l : 0.f;
-    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + size_t(d[DESC_START] + node) * (size_t(a.n_q) * a.D) + (d[DESC_HEAD] * p.group + h) * a.D + 4 * c;
+    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + size_t(start + node) * (size_t(a.n_q) * a.D) + (head * p.group + h) * a.D + 4 * c;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
   }
 }
 
-template <int QS, bool PAIR>
+template <int QS, int NQ>
 int launch_tc(const TcParams& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, int ctas, cudaStream_t s) {
-  using C = Cfg<QS, PAIR>;
-  auto* kernel = attention_tree_tc_kernel<QS, PAIR>;
+  using C = Cfg<QS, NQ>;
+  auto* kernel = attention_tree_tc_kernel<QS, NQ>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess) return -1;
   kernel<<<ctas, kTcThreads, C::kSmem, s>>>(q, k, v, p);
   if (cudaGetLastError() != cudaSuccess) return -1;
+  if (ctas == 1) return 0;                                             // nothing was split
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(ctas, 4);
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3(ctas, 8);
+  cfg.blockDim = dim3(128);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attention_tree_merge_kernel<QS, PAIR>, p) == cudaSuccess ? 0 : -1;
+  return cudaLaunchKernelEx(&cfg, attention_tree_merge_kernel<QS, NQ>, p) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace xl_at
@@ -805,12 +857,13 @@ XL_API int xl_attention_tree(const void* q, const void* k_cache, const void* v_c
     t.group = n_q / n_kv;
     t.nodes = BQ / t.group;
     t.box_tokens = min(block_size & -block_size, BKV);
-    t.min_tiles = 4;
+    t.block_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
+    t.min_work = 4 + kItemCost;
     t.scale_log2 = scale * 1.4426950408889634f;
     const int rows = pair ? 256 : 128, DV = (D + 63) / 64 * 64;
     t.ws_o = static_cast<float4*>(workspace);
     t.ws_ml = reinterpret_cast<float2*>(t.ws_o + size_t(2) * ctas * rows * (DV / 4));
-    t.ws_desc = reinterpret_cast<int*>(t.ws_ml + size_t(2) * ctas * rows);
+    t.ws_desc = reinterpret_cast<int*>(t.ws_ml + size_t(2) * ctas * rows);          // on 16 bytes: rows is even
     t.status = xl_host::status_word();
     CUtensorMap mq, mk, mv;
     const uint64_t q_dims[3] = {uint64_t(D), uint64_t(n_q), uint64_t(T)}, q_strides[2] = {uint64_t(q_head) * 2, uint64_t(q_row) * 2};
@@ -823,8 +876,8 @@ XL_API int xl_attention_tree(const void* q, const void* k_cache, const void* v_c
         xl_host::encode_tiled(&mk, bf16, 3, k_cache, kv_dims, kv_strides, kv_box, swz) != CUDA_SUCCESS ||
         xl_host::encode_tiled(&mv, bf16, 3, v_cache, kv_dims, kv_strides, kv_box, swz) != CUDA_SUCCESS)
       return -4;
-    if (D <= 64) return pair ? launch_tc<1, true>(t, mq, mk, mv, ctas, s) : launch_tc<1, false>(t, mq, mk, mv, ctas, s);
-    return pair ? launch_tc<2, true>(t, mq, mk, mv, ctas, s) : launch_tc<2, false>(t, mq, mk, mv, ctas, s);
+    if (D <= 64) return pair ? launch_tc<1, 2>(t, mq, mk, mv, ctas, s) : launch_tc<1, 1>(t, mq, mk, mv, ctas, s);
+    return pair ? launch_tc<2, 2>(t, mq, mk, mv, ctas, s) : launch_tc<2, 1>(t, mq, mk, mv, ctas, s);
   }
   const long items = long(T) * n_q, grid = (items + 3) / 4;
   if (grid > 0x7fffffffl) return -2;
