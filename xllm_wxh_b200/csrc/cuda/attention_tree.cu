@@ -3,6 +3,8 @@
 //
 // The fp32-pipe kernel serves every type and size: one warp per (row, query head), 32 keys at a time, one key per lane for the scores, then
 // one slice of the value columns per lane for the weighted sum, with a running maximum and sum.
+#include <atomic>
+
 #include "attention_tc.cuh"
 #include "vec8.cuh"
 
@@ -797,7 +799,13 @@ template <int QS, int NQ>
 int launch_tc(const TcParams& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, int ctas, cudaStream_t s) {
   using C = Cfg<QS, NQ>;
   auto* kernel = attention_tree_tc_kernel<QS, NQ>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess) return -1;
+  static std::atomic<bool> ready[64];                                  // per device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess) return -1;
+    ready[dev].store(true, std::memory_order_release);
+  }
   kernel<<<ctas, kTcThreads, C::kSmem, s>>>(q, k, v, p);
   if (cudaGetLastError() != cudaSuccess) return -1;
   if (ctas == 1) return 0;                                             // nothing was split
@@ -823,8 +831,8 @@ static bool tc_serves(const void* q, const void* k, const void* v, int block_siz
 }
 
 // Bytes of the workspace for `ctas` CTAs (0: the tensor-core kernel does not serve these sizes).  max_q: rows of a sequence at most.
-XL_API long xl_attention_tree_workspace(int block_size, int n_q, int n_kv, int D, int max_q, int f32, int ctas) {
-  if (!tc_serves(nullptr, nullptr, nullptr, block_size, n_q, n_kv, D, 8, 8, 1.f, f32)) return 0;
+XL_API long xl_attention_tree_workspace(int block_size, int n_q, int n_kv, int D, int max_q, int ctas) {
+  if (!tc_serves(nullptr, nullptr, nullptr, block_size, n_q, n_kv, D, 8, 8, 1.f, 0)) return 0;
   const long rows = long(max_q) * (n_q / n_kv) > xl_at::BQ ? 256 : 128, DV = (D + 63) / 64 * 64;
   return 2l * ctas * rows * (DV * 4 + 8) + 32l * ctas;
 }
@@ -851,14 +859,14 @@ XL_API int xl_attention_tree(const void* q, const void* k_cache, const void* v_c
   auto s = static_cast<cudaStream_t>(stream);
   if (workspace && B > 0 && tc_serves(q, k_cache, v_cache, block_size, n_q, n_kv, D, q_row, q_head, scale, f32)) {
     const bool pair = long(max_q) * (n_q / n_kv) > BQ;
-    if (ctas < 1 || workspace_bytes < xl_attention_tree_workspace(block_size, n_q, n_kv, D, max_q, f32, ctas)) return -2;
+    if (ctas < 1 || workspace_bytes < xl_attention_tree_workspace(block_size, n_q, n_kv, D, max_q, ctas)) return -2;
     TcParams t{};
     t.a = p;
     t.group = n_q / n_kv;
     t.nodes = BQ / t.group;
     t.box_tokens = min(block_size & -block_size, BKV);
     t.block_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
-    t.min_work = 4 + kItemCost;
+    t.min_work = 3;
     t.scale_log2 = scale * 1.4426950408889634f;
     const int rows = pair ? 256 : 128, DV = (D + 63) / 64 * 64;
     t.ws_o = static_cast<float4*>(workspace);

@@ -4,6 +4,8 @@ a CPU tensor runs the PyTorch statement of the same op from `reference`, which i
 the kernels are tested against."""
 from __future__ import annotations
 
+import torch
+
 from . import reference as ref
 
 
@@ -333,12 +335,10 @@ def _tree():
     return tree_cuda
 
 
-def _like(t, dtype, shape, device, name):
-    """Checks one argument: element type, sizes (None: any), dense, on the same device."""
-    import torch
-    assert isinstance(t, torch.Tensor) and t.dtype == dtype, f"{name}: a tensor of {dtype}"
-    assert t.dim() == len(shape) and all(n is None or n == m for n, m in zip(shape, t.shape)), f"{name}: shape {tuple(t.shape)}, not {shape}"
-    assert t.is_contiguous() and t.device == device, f"{name}: contiguous, on {device}"
+def _like(t, dtype, shape, dev, name):
+    """Checks one argument: element type, sizes, dense, on the device of that number."""
+    assert t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous(), \
+        f"{name}: {dtype} {tuple(shape)}, contiguous, beside the others; not {t.dtype} {tuple(t.shape)}"
 
 
 def step_rows(tables, lens, seqs, counts, n_rows, block_size, parents=None, max_q=None, max_blocks=None):
@@ -351,16 +351,16 @@ def step_rows(tables, lens, seqs, counts, n_rows, block_size, parents=None, max_
     the reserved block 0.  max_q bounds counts (trees: at most 256); max_blocks: columns of the new tables (all), unused ones 0.
     Sequences outside the pool (padding: -1) add nothing.  Returns StepRows (positions, slots, token_seq, q_cu, kv_lens,
     block_tables, tree)."""
-    import torch
-    dev, i32 = tables.device, torch.int32
-    assert tables.dim() == 2 and tables.dtype == i32 and (tables.stride(1) == 1 or tables.shape[1] <= 1), "tables: int32 [pool, blocks]"
-    pool, B = tables.shape[0], seqs.numel()
+    dev, i32 = tables.get_device(), torch.int32
+    assert tables.dtype is i32 and tables.dim() == 2 and (tables.stride(1) == 1 or tables.shape[1] <= 1), "tables: int32 [pool, blocks]"
+    pool, blocks = tables.shape
+    B = (seqs.numel(),)
     _like(lens, i32, (pool,), dev, "lens")
-    _like(seqs, i32, (B,), dev, "seqs")
-    _like(counts, i32, (B,), dev, "counts")
+    _like(seqs, i32, B, dev, "seqs")
+    _like(counts, i32, B, dev, "counts")
     max_q = max(1, n_rows) if max_q is None else max_q
-    max_blocks = tables.shape[1] if max_blocks is None else max_blocks
-    assert n_rows >= 0 and block_size >= 1 and max_q >= 1 and 0 <= max_blocks <= tables.shape[1] and B < 65535
+    max_blocks = blocks if max_blocks is None else max_blocks
+    assert n_rows >= 0 and block_size >= 1 and max_q >= 1 and 0 <= max_blocks <= blocks and B[0] < 65535
     if parents is not None:
         _like(parents, i32, (n_rows,), dev, "parents")
         assert max_q <= TREE_MAX_ROWS, f"trees have at most {TREE_MAX_ROWS} rows a sequence: give max_q"
@@ -374,19 +374,20 @@ def tree_attention(q, k_cache, v_cache, inp, tree, scale, sliding_window=-1):
     block, Hkv, D] that hold the step's rows already; `inp` has q_cu, kv_lens, block_tables, token_seq, positions, n_seqs, and max_q and
     max_kv as bounds.  `sliding_window`: only keys at positions above the row's own - window.  Rows that see nothing and rows of no
     sequence are zero.  Returns [T, Hq * D].  bf16 or fp32, up to 512 columns a head."""
-    import torch
     T, Hq, D = q.shape
-    assert q.dtype in (torch.bfloat16, torch.float32) and k_cache.dtype == v_cache.dtype == q.dtype, "q and caches: one type, bf16 or fp32"
+    dev, i32, B = q.get_device(), torch.int32, inp.n_seqs
+    assert q.dtype is k_cache.dtype is v_cache.dtype and q.dtype in (torch.bfloat16, torch.float32), "q and caches: one type, bf16 or fp32"
     assert k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.shape[3] == D and D <= 512, "caches: [blocks, block, Hkv, D]"
-    assert Hq % k_cache.shape[2] == 0 and k_cache.is_contiguous() and v_cache.is_contiguous()
-    dev, i32, B = q.device, torch.int32, inp.n_seqs
-    assert k_cache.device == v_cache.device == dev
+    assert Hq % k_cache.shape[2] == 0 and k_cache.is_contiguous() and v_cache.is_contiguous(), "caches: contiguous, key heads that divide q's"
+    assert k_cache.get_device() == v_cache.get_device() == dev, "caches: on q's device"
     assert inp.max_q <= TREE_MAX_ROWS, f"trees have at most {TREE_MAX_ROWS} rows a sequence"
+    tables = inp.block_tables
     assert tree.dim() == 2 and 1 <= tree.shape[1] <= TREE_MAX_ROWS // 64, "tree: one to four words a row"
-    _like(tree, torch.int64, (T, None), dev, "tree")
+    assert tables.dim() == 2, "block_tables: [B, blocks]"
+    _like(tree, torch.int64, (T, tree.shape[1]), dev, "tree")
     _like(inp.q_cu, i32, (B + 1,), dev, "q_cu")
     _like(inp.kv_lens, i32, (B,), dev, "kv_lens")
-    _like(inp.block_tables, i32, (B, None), dev, "block_tables")
+    _like(tables, i32, (B, tables.shape[1]), dev, "block_tables")
     _like(inp.token_seq, i32, (T,), dev, "token_seq")
     _like(inp.positions, i32, (T,), dev, "positions")
     f = _tree().tree_attention if q.is_cuda else ref.tree_attention
@@ -404,24 +405,23 @@ def adjust_logits(logits, q_cu, seqs=None, history=None, penalties=None, tokens=
     bias = (cu int32 [pool + 1], ids int32, values fp32): added; the last entry of an id holds.
     mask = (words int32 [masks, >= V / 32], rows int32 [S]): ids whose bit is 0 in the row's mask become -inf (rows: -1 for none).
     Ids outside the vocabulary are passed over.  Returns logits."""
-    import torch
     S, V = logits.shape
-    dev, i32, f32 = logits.device, torch.int32, torch.float32
+    dev, i32, f32 = logits.get_device(), torch.int32, torch.float32
     assert logits.dtype in (f32, torch.bfloat16) and (logits.stride(1) == 1 or V == 1) and (logits.stride(0) >= V or S <= 1), "logits: fp32 or bf16 rows"
-    assert q_cu.numel() >= 1
-    _like(q_cu, i32, (None,), dev, "q_cu")
+    assert q_cu.dim() == 1 and q_cu.numel() >= 1, "q_cu: [B + 1]"
     B = q_cu.numel() - 1
+    _like(q_cu, i32, (B + 1,), dev, "q_cu")
     pool = None
     if history is not None:
         ids, lens, prompts = history
         pool = lens.numel()
-        assert ids.dtype == i32 and ids.dim() == 2 and ids.shape[0] == pool and (ids.stride(1) == 1 or ids.shape[1] <= 1) and ids.device == dev, \
+        assert ids.dtype is i32 and ids.dim() == 2 and ids.shape[0] == pool and (ids.stride(1) == 1 or ids.shape[1] <= 1) and ids.get_device() == dev, \
             "history: int32 [pool, cap]"
+        assert penalties is not None and len(penalties) == 3, "history needs (repetition, frequency, presence)"
         _like(lens, i32, (pool,), dev, "lens")
         _like(prompts, i32, (pool,), dev, "prompt_lens")
-        assert penalties is not None and len(penalties) == 3, "history needs (repetition, frequency, presence)"
-        for t, name in zip(penalties, ("repetition", "frequency", "presence")):
-            _like(t, f32, (pool,), dev, name)
+        for t in penalties:
+            _like(t, f32, (pool,), dev, "penalties")
     else:
         assert penalties is None and tokens is None, "penalties and tokens need a history"
     if tokens is not None:
@@ -431,15 +431,15 @@ def adjust_logits(logits, q_cu, seqs=None, history=None, penalties=None, tokens=
         _like(parents, i32, (S,), dev, "parents")
     if bias is not None:
         cu, ids, values = bias
-        _like(cu, i32, (None,) if pool is None else (pool + 1,), dev, "bias cu")
-        pool = cu.numel() - 1
-        _like(ids, i32, (None,), dev, "bias ids")
-        _like(values, f32, (ids.numel(),), dev, "bias values")
+        n = (ids.numel(),)
+        _like(cu, i32, (max(1, cu.numel()) if pool is None else pool + 1,), dev, "bias cu")
+        _like(ids, i32, n, dev, "bias ids")
+        _like(values, f32, n, dev, "bias values")
     if seqs is not None:
         _like(seqs, i32, (B,), dev, "seqs")
     if mask is not None:
         words, rows = mask
-        assert words.dim() == 2 and words.dtype == i32 and words.stride(1) == 1 and words.shape[1] * 32 >= V and words.device == dev, \
+        assert words.dtype is i32 and words.dim() == 2 and words.stride(1) == 1 and words.shape[1] * 32 >= V and words.get_device() == dev, \
             "mask: int32 [masks, V / 32]"
         _like(rows, i32, (S,), dev, "mask rows")
     max_q = max(1, S) if max_q is None else max_q
@@ -455,22 +455,29 @@ def accept_tree(target, inp, parents, caches=(), max_depth=None):
     target's tokens along the path, then -1; accepted [B]: drafted rows on the path; path [B, max_depth + 1]: their numbers, then -1).
     In every tensor of `caches` ([blocks, block, ...], contiguous, no tensor twice) the path's rows move to the positions behind the
     sequence's earlier tokens, which then has 1 + accepted more; the other drafted rows' places hold what they held."""
-    import torch
-    T, dev, i32, B = target.numel(), target.device, torch.int32, inp.n_seqs
-    _like(target, i32, (T,), dev, "target")
-    _like(inp.tokens, i32, (T,), dev, "tokens")
-    _like(parents, i32, (T,), dev, "parents")
+    dev, i32, B, tables, block = target.get_device(), torch.int32, inp.n_seqs, inp.block_tables, inp.block_size
+    T = (target.numel(),)
+    _like(target, i32, T, dev, "target")
+    _like(inp.tokens, i32, T, dev, "tokens")
+    _like(parents, i32, T, dev, "parents")
     _like(inp.q_cu, i32, (B + 1,), dev, "q_cu")
     _like(inp.kv_lens, i32, (B,), dev, "kv_lens")
-    _like(inp.block_tables, i32, (B, None), dev, "block_tables")
+    assert tables.dim() == 2, "block_tables: [B, blocks]"
+    _like(tables, i32, (B, tables.shape[1]), dev, "block_tables")
     assert inp.max_q <= TREE_MAX_ROWS, f"trees have at most {TREE_MAX_ROWS} rows a sequence"
     depth = max(0, inp.max_q - 1) if max_depth is None else max_depth
     assert 0 <= depth < TREE_MAX_ROWS and B < 65536
+    at, shape = [], None
     for c in caches:
-        assert c.dim() >= 2 and c.shape[1] == inp.block_size and c.is_contiguous() and c.device == dev, "caches: [blocks, block, ...], contiguous"
-    assert len({c.data_ptr() for c in caches if c.numel()}) == sum(c.numel() > 0 for c in caches), "a cache may be named once"
-    f = _tree().accept_tree if target.is_cuda else ref.accept_tree
-    return f(target, inp, parents, caches, depth)
+        if c.shape != shape:
+            shape = c.shape
+            assert len(shape) >= 2 and shape[1] == block, "caches: [blocks, block, ...]"
+        assert c.is_contiguous() and c.get_device() == dev, "caches: contiguous, beside the others"
+        at.append(c.data_ptr())
+    assert len(set(at)) == len(at) or len({c.data_ptr() for c in caches if c.numel()}) == sum(c.numel() > 0 for c in caches), "a cache may be named once"
+    if target.is_cuda:
+        return _tree().accept_tree(target, inp, parents, caches, at, depth)
+    return ref.accept_tree(target, inp, parents, caches, depth)
 
 
 # ----------------------------------------------------------------------------- MLA (DeepSeek)
