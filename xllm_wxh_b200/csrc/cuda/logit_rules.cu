@@ -1,24 +1,27 @@
-// Penalties for repeated tokens, biases and grammar masks on the logits of a step's rows, in place and in one launch.
+// Penalties for repeated tokens, biases and grammar masks on the logits of a step's rows, in place.
 //
 // For an id that the row has behind it (its sequence's history, or the tokens on the row's way from the root of its drafted tree),
 // made of them generated ones: x -= made freq + (made > 0) pres, then x *= rep below zero and x /= rep above.  Biases are
 // added; ids that the row's mask forbids become -inf.  Everything is computed in fp32 and rounded once.
 //
-// The kernel reads the history itself, so that nothing of it has to be counted and sent by the host.  Two kinds of CTAs share the launch
-// and never write the same logit:
-//   penalties: (sequence, part, rows) - counts the history's ids in a table in shared memory, which the sequence's rows share, and
-//              touches only the logits whose ids are in it; forbidden ids are left to the other kind;
-//   masks:     (row, columns) - writes -inf where the mask forbids and reads no logit.
-// The table is a hash table when the history, the path and the biases fit three quarters of it, otherwise it holds a slice of the
-// vocabulary at a time, so that any length works.  Counts are whole numbers and the last bias of an id wins by its index: the
-// order in which threads arrive changes nothing.
+// Two kernels that never write the same logit, so that they may run side by side:
+//   masks    : (row, columns) - writes -inf where the mask forbids and reads no logit; bound by the bytes written;
+//   penalties: (sequence, part, rows) - counts the history's ids in a table in shared memory, so that nothing of the history has to be
+//              counted and sent by the host, and touches only the logits whose ids are in it (one sector each); forbidden ids are left
+//              to the other kernel.  Bound by the latency of a few dependent loads when there are few rows.
+// The table is a hash table (linear probing) where history and biases are sure to fit.  Longer ones are tried, since text has far fewer
+// distinct ids than tokens; where an id finds no place within kProbes, or the history is longer still, the CTA goes through the
+// vocabulary slice by slice with the table as a plain array, so that any history works.  Counts are whole
+// numbers and the last bias of an id wins by its index: the order in which threads arrive changes nothing.
+#include <atomic>
+
 #include "vec8.cuh"
 
 namespace xl_lr {
 using namespace xl;
 
-constexpr int kThreads = 512;
-constexpr int kPathRows = 256;
+constexpr int kThreads = 512, kMaskThreads = 256;
+constexpr int kPathRows = 256, kProbes = 64, kMaxSlots = 7680;   // two such tables fit an SM
 constexpr uint32_t kPrompt = 0x80000000u, kOnPath = 0x40000000u, kMade = 0x3FFFFFFFu;
 
 struct Params {
@@ -41,11 +44,54 @@ struct Params {
   const int* mask_of;           // [S]
   int words_ld, n_masks;
   int slots;                    // entries of the table
-  int parts, row_parts;
-  int penalty_ctas;             // parts * row_parts * B
-  int columns, mask_parts;      // columns of a mask CTA, such CTAs of a row
+  int parts, row_parts;         // CTAs that share a sequence's vocabulary slices, and its rows
 };
 
+// ---------------------------------------------------------------- masks
+// Groups of 16 bytes start on 16-byte boundaries of the row's address.  A group's bits straddle two words of the mask.
+template <typename T>
+__global__ void __launch_bounds__(kMaskThreads) mask_logits_kernel(const Params p, int parts) {
+  grid_dep_launch();
+  const int row = blockIdx.x / parts;
+  const int m = p.mask_of[row];
+  if (m < 0 || m >= p.n_masks) return;
+  constexpr int G = 16 / sizeof(T);
+  constexpr uint32_t kAll = (1u << G) - 1, kLow = sizeof(T) == 2 ? 0xFF80FF80u : 0xFF800000u;
+  T* x = static_cast<T*>(p.logits) + size_t(row) * p.ld;
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(p.words) + size_t(m) * p.words_ld;
+  const int n_words = (p.V + 31) / 32;
+  const int shift = int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % G), groups = (p.V + shift + G - 1) / G;
+  T low;
+  from_f32(&low, -INFINITY);
+  const int share = (groups + parts - 1) / parts, g1 = min(groups, int(blockIdx.x % parts + 1) * share);
+  for (int g0 = blockIdx.x % parts * share + threadIdx.x; g0 < g1; g0 += 4 * kMaskThreads) {
+    uint32_t bits[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int g = g0 + i * kMaskThreads, t = g * G - shift, at = t >> 5;        // t may start below 0
+      bits[i] = kAll;
+      if (g < g1) {
+        const uint32_t lo = at >= 0 ? w[at] : ~0u, hi = at + 1 < n_words && (t & 31) > 32 - G ? w[at + 1] : ~0u;
+        bits[i] = __funnelshift_r(lo, hi, t & 31) & kAll;
+        if (t < 0) bits[i] |= (1u << -t) - 1;
+        if (t + G > p.V) bits[i] |= kAll & ~((1u << (p.V - t)) - 1);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = (g0 + i * kMaskThreads) * G - shift;
+      if (bits[i] == 0) {
+        *reinterpret_cast<uint4*>(x + t) = make_uint4(kLow, kLow, kLow, kLow);
+      } else if (bits[i] != kAll) {
+#pragma unroll
+        for (int e = 0; e < G; ++e)
+          if (!(bits[i] >> e & 1u)) x[t + e] = low;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- penalties and biases
 __device__ __forceinline__ float adjusted(float x, uint32_t word, float bias, bool biased, float rep, float freq, float pres) {
   if (word != 0) {
     const float made = float(word & kMade);
@@ -55,84 +101,57 @@ __device__ __forceinline__ float adjusted(float x, uint32_t word, float bias, bo
   return biased ? x + bias : x;
 }
 
-template <typename T>
-__device__ void mask_columns(const Params& p, int row, int c0) {
-  const int m = p.mask_of[row];
-  if (m < 0 || m >= p.n_masks) return;
-  constexpr int kPer16 = 16 / sizeof(T);
-  T* x = static_cast<T*>(p.logits) + size_t(row) * p.ld;
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(p.words) + size_t(m) * p.words_ld;
-  const int n_words = (p.V + 31) / 32;
-  // groups of eight columns start on 16-byte boundaries of the row's address
-  const int shift = int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % kPer16);
-  T low;
-  from_f32(&low, -INFINITY);
-  const int hi = min(c0 + p.columns, p.V + shift);
-  for (int g = c0 + 8 * int(threadIdx.x); g < hi; g += 8 * kThreads) {
-    const int t = g - shift, at = t >> 5;                          // may start below 0
-    const uint32_t a = at >= 0 && at < n_words ? w[at] : ~0u, b = at + 1 < n_words ? w[at + 1] : ~0u;
-    const uint32_t bits = __funnelshift_r(a, b, t & 31) & 0xFFu;
-    if (bits == 0xFFu) continue;
-    if (bits == 0 && t >= 0 && t + 8 <= p.V) {
-      const uint32_t pair = sizeof(T) == 2 ? 0xFF80FF80u : 0xFF800000u;
-      uint4* to = reinterpret_cast<uint4*>(x + t);
-      to[0] = make_uint4(pair, pair, pair, pair);
-      if (sizeof(T) == 4) to[1] = make_uint4(pair, pair, pair, pair);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (!(bits >> e & 1u) && t + e >= 0 && t + e < p.V) x[t + e] = low;
-    }
-  }
-}
+struct PathSmem {                // of a row of the sequence (only where rows have tokens)
+  unsigned long long anc[4];     // the row and its ancestors
+  unsigned long long same[4];    // rows with the same token
+  int up, token, first;          // first: list of the rows that are the first with their token
+  uint32_t word;                 // what the table had for the token
+  int bias;
+  int pad;
+};
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) adjust_logits_kernel(const Params p) {
-  extern __shared__ __align__(16) uint32_t smem[];
-  if (int(blockIdx.x) >= p.penalty_ctas) {
-    const int i = blockIdx.x - p.penalty_ctas;
-    mask_columns<T>(p, i / p.mask_parts, i % p.mask_parts * p.columns);
-    return;
-  }
+__global__ void __launch_bounds__(kThreads) penalise_logits_kernel(const Params p) {
+  extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x, C = p.slots;
   int* s_id = reinterpret_cast<int*>(smem);                        // [C]
-  uint32_t* s_word = smem + C;                                     // [C]
-  int* s_bias = reinterpret_cast<int*>(smem + 2 * C);              // [C] index of the bias, then its value's bits
-  __shared__ unsigned long long s_anc[kPathRows][4], s_same[kPathRows][4];
-  __shared__ int s_up[kPathRows], s_tok[kPathRows], s_first[kPathRows];
-  __shared__ uint32_t s_pword[kPathRows];
-  __shared__ float s_pbias[kPathRows];
-  __shared__ int s_pbiased[kPathRows];
-  __shared__ unsigned long long s_made[4];                          // rows whose tokens lie behind the prompt
-  __shared__ int s_count, s_firsts;
+  uint32_t* s_word = reinterpret_cast<uint32_t*>(s_id + C);        // [C]
+  int* s_bias = reinterpret_cast<int*>(s_word + C);                // [C] index of the bias
+  uint16_t* s_list = reinterpret_cast<uint16_t*>(s_bias + C);      // [C] entries that change something
+  PathSmem* path_of = reinterpret_cast<PathSmem*>(s_list + C);     // [max_q]
+  __shared__ unsigned long long s_made[4];                         // rows whose tokens lie behind the prompt
+  __shared__ int s_count, s_firsts, s_full;
 
   const int part = blockIdx.x % p.parts, rp = blockIdx.x / p.parts % p.row_parts, b = blockIdx.x / p.parts / p.row_parts;
   const int src = p.seqs ? p.seqs[b] : b;
-  if (unsigned(src) >= unsigned(p.pool)) return;
   const int start = max(p.q_cu[b], 0), n = min(min(p.q_cu[b + 1], p.S) - start, p.max_q);
   const int share = (max(n, 0) + p.row_parts - 1) / p.row_parts;
   const int r0 = rp * share, r1 = min(n, r0 + share);
-  if (r0 >= r1) return;
+  if (unsigned(src) >= unsigned(p.pool) || r0 >= r1) {
+    grid_dep_wait();
+    return;
+  }
   float rep = 1.f, freq = 0.f, pres = 0.f;
-  int len = 0, prompt = 0;
+  int given = 0, prompt = 0, e0 = 0, e1 = 0;
   if (p.text) {
     rep = p.rep[src]; freq = p.freq[src]; pres = p.pres[src];
-    if (rep != 1.f || freq != 0.f || pres != 0.f) {                // otherwise the history changes nothing
-      len = min(max(p.lens[src], 0), p.text_cap);
-      prompt = p.prompts[src];
-    }
+    given = max(p.lens[src], 0);
+    prompt = p.prompts[src];
   }
-  const bool penal = p.text && (rep != 1.f || freq != 0.f || pres != 0.f);
-  int e0 = 0, e1 = 0;
   if (p.bias_cu) {
     e0 = max(p.bias_cu[src], 0);
-    e1 = min(p.bias_cu[src + 1], p.n_bias);
+    e1 = max(e0, min(p.bias_cu[src + 1], p.n_bias));
   }
+  const bool penal = rep != 1.f || freq != 0.f || pres != 0.f;     // otherwise the history changes nothing
+  const int len = penal ? min(given, p.text_cap) : 0;
   const int path = penal && p.tokens ? r1 : 0;                     // rows whose tokens can be on a way to the rows r0 .. r1 - 1
-  if (len == 0 && path == 0 && e1 <= e0) return;
+  if (len == 0 && path == 0 && e1 == e0) {
+    grid_dep_wait();
+    return;
+  }
   const int* text = p.text + size_t(src) * p.text_ld;
 
-  // ancestors of the rows, as sets of rows (by doubling), and the rows with the same token as each
+  // ancestors of the rows, as sets of rows (by doubling)
   if (path > 0) {
     unsigned long long a[4] = {0, 0, 0, 0};
     int up = -1;
@@ -140,159 +159,219 @@ __global__ void __launch_bounds__(kThreads) adjust_logits_kernel(const Params p)
     if (tid < path) {
       up = p.parents ? p.parents[start + tid] : tid - 1;
       if (up < 0 || up >= tid) up = -1;
-      s_up[tid] = up;
-      s_tok[tid] = p.tokens[start + tid];
+      path_of[tid].up = up;
+      path_of[tid].token = p.tokens[start + tid];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) s_anc[tid][w] = a[w] = w == (tid >> 6) ? 1ull << (tid & 63) : 0;
+      for (int w = 0; w < 4; ++w) path_of[tid].anc[w] = a[w] = w == (tid >> 6) ? 1ull << (tid & 63) : 0;
     }
     while (__syncthreads_or(tid < path && up >= 0)) {
       int next = -1;
       if (tid < path && up >= 0) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) a[w] |= s_anc[up][w];
-        next = s_up[up];
+        for (int w = 0; w < 4; ++w) a[w] |= path_of[up].anc[w];
+        next = path_of[up].up;
       }
       __syncthreads();
       if (tid < path) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) s_anc[tid][w] = a[w];
-        s_up[tid] = up = next;
+        for (int w = 0; w < 4; ++w) path_of[tid].anc[w] = a[w];
+        path_of[tid].up = up = next;
       }
     }
     if (tid < path) {
       const int depth = __popcll(a[0]) + __popcll(a[1]) + __popcll(a[2]) + __popcll(a[3]) - 1;
-      if (long(max(p.lens[src], 0)) + depth >= prompt) atomicOr(&s_made[tid >> 6], 1ull << (tid & 63));
+      if (long(given) + depth >= prompt) atomicOr(&s_made[tid >> 6], 1ull << (tid & 63));
     }
   }
 
-  const bool hashed = long(len) + max(e1 - e0, 0) <= C / 4 * 3;
-  const int slices = hashed ? 1 : (p.V + C - 1) / C;
-  for (int slice = part; slice < slices; slice += p.parts) {
-    const int v0 = hashed ? 0 : slice * C, v1 = hashed ? p.V : min(p.V, v0 + C);
-    __syncthreads();
-    for (int i = tid; i < C; i += kThreads) {
-      s_id[i] = hashed ? -1 : v0 + i;
-      s_word[i] = 0;
-      s_bias[i] = -1;
-    }
-    if (tid == 0) s_count = s_firsts = 0;
-    __syncthreads();
-    auto first_slot = [&](int id) { return int((uint32_t(id) * 2654435761u) >> 16) & (C - 1); };
-    // the table has free entries (it is at most three quarters full), so the search ends
-    auto entry = [&](int id) {
-      if (!hashed) return id - v0;
-      int at = first_slot(id);
-      while (true) {
-        const int was = atomicCAS(&s_id[at], -1, id);
-        if (was == -1 || was == id) return at;
-        at = (at + 1) & (C - 1);
+  // Attempt 0 hashes, attempt 1 goes through slices.  Parts that share a sequence's slices must not differ on it: they hash only what
+  // is sure to fit, and leave that to the first of them.
+  const long most = long(len) + (e1 - e0);
+  const bool sure = most <= C / 8 * 7;
+  const int probes = sure ? C : kProbes;
+  for (int attempt = sure || (p.parts == 1 && most <= 4l * C) ? 0 : 1; attempt < 2; ++attempt) {
+    const bool hashed = attempt == 0;
+    if (hashed && part > 0) break;
+    const int slices = hashed ? 1 : (p.V + C - 1) / C;
+    bool full = false;
+    for (int slice = hashed ? 0 : part; slice < slices; slice += p.parts) {
+      const int v0 = hashed ? 0 : slice * C, v1 = hashed ? p.V : min(p.V, v0 + C);
+      __syncthreads();
+      for (int i = 4 * tid; i < C; i += 4 * kThreads) {
+        *reinterpret_cast<int4*>(s_id + i) = hashed ? make_int4(-1, -1, -1, -1) : make_int4(v0 + i, v0 + i + 1, v0 + i + 2, v0 + i + 3);
+        *reinterpret_cast<int4*>(s_word + i) = make_int4(0, 0, 0, 0);
+        *reinterpret_cast<int4*>(s_bias + i) = make_int4(-1, -1, -1, -1);
       }
-    };
-    auto find = [&](int id) {
-      if (!hashed) return id - v0;
-      int at = first_slot(id);
-      while (s_id[at] != id) {
-        if (s_id[at] == -1) return -1;
-        at = (at + 1) & (C - 1);
-      }
-      return at;
-    };
-    for (int i = tid; i < len; i += kThreads) {
-      const int id = text[i];
-      if (id < v0 || id >= v1) continue;
-      uint32_t* w = &s_word[entry(id)];
-      if (i < prompt) atomicOr(w, kPrompt);
-      else atomicAdd(w, 1u);
-    }
-    for (int e = e0 + tid; e < e1; e += kThreads) {
-      const int id = p.bias_ids[e];
-      if (id >= v0 && id < v1) atomicMax(&s_bias[entry(id)], e);
-    }
-    __syncthreads();
-    // ids on the path: one entry for each distinct one, with the set of the rows that hold it; their counts differ from row to row
-    if (tid < path) {
-      const int id = s_tok[tid];
-      bool first = id >= v0 && id < v1;
-      unsigned long long same[4] = {0, 0, 0, 0};
-      for (int i = 0; i < path; ++i) {
-        const bool eq = s_tok[i] == id;
-        first = first && !(eq && i < tid);
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          if (eq && w == (i >> 6)) same[w] |= 1ull << (i & 63);
-      }
-      if (first) {
-        const int at = find(id);
-        uint32_t word = 0;
-        int e = -1;
-        if (at >= 0) {
-          word = s_word[at];
-          e = s_bias[at];
-          s_word[at] = word | kOnPath;
+      if (tid == 0) s_count = s_firsts = s_full = 0;
+      __syncthreads();
+      auto first_slot = [&](int id) { return int(__umulhi(uint32_t(id) * 2654435761u, uint32_t(C))); };
+      auto entry = [&](int id) {                                   // -1: no place
+        if (!hashed) return id - v0;
+        int at = first_slot(id);
+        for (int k = 0; k < probes; ++k) {
+          const int was = atomicCAS(&s_id[at], -1, id);
+          if (was == -1 || was == id) return at;
+          at = at + 1 < C ? at + 1 : 0;
         }
-        s_pword[tid] = word;
-        s_pbiased[tid] = e >= 0;
-        s_pbias[tid] = e >= 0 ? p.bias_values[e] : 0.f;
+        s_full = 1;
+        return -1;
+      };
+      auto find = [&](int id) {
+        if (!hashed) return id - v0;
+        int at = first_slot(id);
+        for (int k = 0; k < probes && s_id[at] != -1; ++k) {
+          if (s_id[at] == id) return at;
+          at = at + 1 < C ? at + 1 : 0;
+        }
+        return -1;
+      };
+      for (int i0 = tid; i0 < len; i0 += 8 * kThreads) {
+        int id[8];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) s_same[tid][w] = same[w];
-        s_first[atomicAdd(&s_firsts, 1)] = tid;
-      }
-    }
-    __syncthreads();
-    // the other entries that change something move to the front of the table
-    for (int base = 0; base < C; base += kThreads) {
-      const int i = base + tid;
-      int id = -1, e = -1;
-      uint32_t word = 0;
-      if (i < C) {
-        id = s_id[i];
-        word = s_word[i];
-        e = s_bias[i];
-      }
-      const bool keep = id >= 0 && !(word & kOnPath) && (word != 0 || e >= 0);
-      const uint32_t votes = __ballot_sync(0xffffffffu, keep);
-      int at = 0;
-      if ((tid & 31) == 0) at = atomicAdd(&s_count, __popc(votes));
-      at = __shfl_sync(0xffffffffu, at, 0) + __popc(votes & ((1u << (tid & 31)) - 1));
-      const float value = keep && e >= 0 ? p.bias_values[e] : 0.f;
-      __syncthreads();                                             // everything below base + kThreads has been read
-      if (keep) {
-        s_id[at] = e >= 0 ? ~id : id;                              // ids with a bias are stored complemented
-        s_word[at] = word;
-        s_bias[at] = __float_as_int(value);
-      }
-    }
-    __syncthreads();
-    const int count = s_count, firsts = s_firsts, rows = r1 - r0;
-    T* x0 = static_cast<T*>(p.logits);
-    auto allowed = [&](int row, int id) {
-      if (!p.words) return true;
-      const int m = p.mask_of[row];
-      return m < 0 || m >= p.n_masks || (p.words[size_t(m) * p.words_ld + (id >> 5)] >> (id & 31) & 1);
-    };
-    for (int i = tid; i < count * rows; i += kThreads) {
-      const int r = i / count, e = i - r * count, row = start + r0 + r;
-      const int raw = s_id[e], id = raw < 0 ? ~raw : raw;
-      if (!allowed(row, id)) continue;
-      T* x = x0 + size_t(row) * p.ld + id;
-      from_f32(x, adjusted(to_f32(*x), s_word[e], __int_as_float(s_bias[e]), raw < 0, rep, freq, pres));
-    }
-    for (int i = tid; i < firsts * rows; i += kThreads) {
-      const int r = i / firsts, f = s_first[i - r * firsts], row = start + r0 + r, id = s_tok[f];
-      int more = 0;
-      bool given = false;
+        for (int k = 0; k < 8; ++k) id[k] = i0 + k * kThreads < len ? text[i0 + k * kThreads] : -1;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const unsigned long long mine = s_anc[r0 + r][w] & s_same[f][w];
-        more += __popcll(mine & s_made[w]);
-        given = given || (mine & ~s_made[w]);
+        for (int k = 0; k < 8; ++k) {
+          if (id[k] < v0 || id[k] >= v1) continue;
+          const int at = entry(id[k]);
+          if (at < 0) continue;
+          if (i0 + k * kThreads < prompt) atomicOr(&s_word[at], kPrompt);
+          else atomicAdd(&s_word[at], 1u);
+        }
       }
-      const uint32_t word = (s_pword[f] + uint32_t(more)) | (given ? kPrompt : 0u);
-      if ((word == 0 && !s_pbiased[f]) || !allowed(row, id)) continue;
-      T* x = x0 + size_t(row) * p.ld + id;
-      from_f32(x, adjusted(to_f32(*x), word, s_pbias[f], s_pbiased[f], rep, freq, pres));
+      for (int e = e0 + tid; e < e1; e += kThreads) {
+        const int id = p.bias_ids[e];
+        if (id < v0 || id >= v1) continue;
+        const int at = entry(id);
+        if (at >= 0) atomicMax(&s_bias[at], e);
+      }
+      __syncthreads();
+      full = s_full;
+      if (full) break;                                             // (only a hash table fills up)
+      // ids on the path: one entry for each distinct one, with the set of the rows that hold it; their counts differ from row to row
+      if (tid < path) {
+        const int id = path_of[tid].token;
+        bool first = id >= v0 && id < v1;
+        unsigned long long same[4] = {0, 0, 0, 0};
+        for (int i = 0; i < path; ++i) {
+          const bool eq = path_of[i].token == id;
+          first = first && !(eq && i < tid);
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            if (eq && w == (i >> 6)) same[w] |= 1ull << (i & 63);
+        }
+        if (first) {
+          const int at = find(id);
+          uint32_t word = 0;
+          int e = -1;
+          if (at >= 0) {
+            word = s_word[at];
+            e = s_bias[at];
+            s_word[at] = word | kOnPath;
+          }
+          path_of[tid].word = word;
+          path_of[tid].bias = e;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) path_of[tid].same[w] = same[w];
+          path_of[atomicAdd(&s_firsts, 1)].first = tid;
+        }
+      }
+      __syncthreads();
+      for (int i = tid; i < C; i += kThreads) {
+        const uint32_t word = s_word[i];
+        const bool keep = !(word & kOnPath) && (word != 0 || s_bias[i] >= 0);
+        const uint32_t votes = __ballot_sync(0xffffffffu, keep);
+        int at = 0;
+        if ((tid & 31) == 0 && votes) at = atomicAdd(&s_count, __popc(votes));
+        at = __shfl_sync(0xffffffffu, at, 0) + __popc(votes & ((1u << (tid & 31)) - 1));
+        if (keep) s_list[at] = uint16_t(i);
+      }
+      __syncthreads();
+      const int count = s_count, firsts = s_firsts, rows = r1 - r0;
+      T* x0 = static_cast<T*>(p.logits);
+      auto allowed = [&](int row, int id) {
+        if (!p.words) return true;
+        const int m = p.mask_of[row];
+        return m < 0 || m >= p.n_masks || (p.words[size_t(m) * p.words_ld + (id >> 5)] >> (id & 31) & 1);
+      };
+      // four logits at a time, so that their loads are under way together
+      for (int i0 = tid; i0 < count * rows; i0 += 4 * kThreads) {
+        T* at[4];
+        float x[4];
+        int slot[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int i = i0 + k * kThreads;
+          at[k] = nullptr;
+          x[k] = 0.f;
+          slot[k] = 0;
+          if (i < count * rows) {
+            const int r = i / count, row = start + r0 + r;
+            slot[k] = s_list[i - r * count];
+            const int id = s_id[slot[k]];
+            T* to = x0 + size_t(row) * p.ld + id;
+            x[k] = to_f32(*to);
+            if (allowed(row, id)) at[k] = to;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (at[k]) {
+            const int e = s_bias[slot[k]];
+            from_f32(at[k], adjusted(x[k], s_word[slot[k]], e >= 0 ? p.bias_values[e] : 0.f, e >= 0, rep, freq, pres));
+          }
+      }
+      for (int i = tid; i < firsts * rows; i += kThreads) {
+        const int r = i / firsts, f = path_of[i - r * firsts].first, row = start + r0 + r, id = path_of[f].token;
+        int more = 0;
+        bool before = false;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const unsigned long long mine = path_of[r0 + r].anc[w] & path_of[f].same[w];
+          more += __popcll(mine & s_made[w]);
+          before = before || (mine & ~s_made[w]);
+        }
+        const uint32_t word = (path_of[f].word + uint32_t(more)) | (before ? kPrompt : 0u);
+        const int e = path_of[f].bias;
+        if ((word == 0 && e < 0) || !allowed(row, id)) continue;
+        T* x = x0 + size_t(row) * p.ld + id;
+        from_f32(x, adjusted(to_f32(*x), word, e >= 0 ? p.bias_values[e] : 0.f, e >= 0, rep, freq, pres));
+      }
     }
+    if (hashed && !full) break;
   }
+  grid_dep_wait();                                                 // what follows on the stream waits for this kernel only
+}
+
+template <typename T>
+int launch(const Params& p, bool penalties, int mask_parts, cudaStream_t s) {
+  if (p.words) {
+    const long grid = long(p.S) * mask_parts;
+    if (grid > 0x7fffffffl) return -2;
+    mask_logits_kernel<T><<<unsigned(grid), kMaskThreads, 0, s>>>(p, mask_parts);
+    if (cudaGetLastError() != cudaSuccess) return -1;
+  }
+  if (!penalties) return 0;
+  const long grid = long(p.B) * p.parts * p.row_parts;
+  if (grid > 0x7fffffffl) return -2;
+  auto* kernel = penalise_logits_kernel<T>;
+  static std::atomic<bool> ready[64];                              // per device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 14 * kMaxSlots + int(sizeof(PathSmem)) * kPathRows) != cudaSuccess) return -1;
+    ready[dev].store(true, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(grid));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = 14 * p.slots + (p.tokens ? sizeof(PathSmem) * p.max_q : 0);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.words ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace xl_lr
@@ -304,7 +383,7 @@ XL_API int xl_adjust_logits(void* logits, int f32, int S, int V, long ld, const 
                             const void* mask_of, void* stream) {
   using namespace xl_lr;
   if (S < 0 || V < 1 || B < 0 || max_q < 1 || (tokens && max_q > kPathRows) || (words && words_ld < (V + 31) / 32)) return -2;
-  if (S == 0 || B == 0) return 0;
+  if (S == 0) return 0;
   Params p{};
   p.logits = logits;
   p.ld = ld;
@@ -327,21 +406,18 @@ XL_API int xl_adjust_logits(void* logits, int f32, int S, int V, long ld, const 
   p.words = static_cast<const int*>(words);
   p.mask_of = static_cast<const int*>(mask_of);
   p.words_ld = words_ld; p.n_masks = n_masks;
-  p.slots = 8192;
-  p.parts = 1;
-  p.row_parts = 1;
-  const bool penalties = text || bias_cu;
-  const long ctas = penalties ? long(B) * p.parts * p.row_parts : 0;
-  p.columns = 16384;
-  p.mask_parts = (V + 16 + p.columns - 1) / p.columns;
-  const long grid = ctas + (words ? long(S) * p.mask_parts : 0);
-  if (grid == 0) return 0;
-  if (grid > 0x7fffffffl) return -2;
-  p.penalty_ctas = int(ctas);
-  const int smem = penalties ? 12 * p.slots : 0;
-  auto* kernel = f32 ? adjust_logits_kernel<float> : adjust_logits_kernel<__nv_bfloat16>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 12 * 8192);
-  if (e != cudaSuccess) return -1;
-  kernel<<<unsigned(grid), kThreads, smem, static_cast<cudaStream_t>(stream)>>>(p);
-  return cudaGetLastError() == cudaSuccess ? 0 : -1;
+  const int sms = xl_host::sm_count();
+  // a table that holds any history of the given length; long ones go by their distinct ids, which text has far fewer of
+  p.slots = int(min(long(kMaxSlots), (long(text ? text_cap : 0) + 64) / 448 * 512 + 512));
+  // rows of a sequence over several CTAs (each counts the history again), as long as there are SMs without one; slices of the
+  // vocabulary, where histories are too long to be hashed
+  p.row_parts = B > 0 ? max(1, min(min(max_q, S), 2 * sms / B)) : 1;
+  p.parts = B > 0 && text && text_cap > 4l * p.slots ? max(1, min((V + p.slots - 1) / p.slots, 2 * sms / (B * p.row_parts))) : 1;
+  // 16-byte groups of a row over CTAs of up to 4 x 4 groups a thread, smaller ones where there are few rows
+  const int groups = V * (f32 ? 4 : 2) / 16 + 2;
+  const int mask_parts = max(1, min((groups + 4 * kMaskThreads - 1) / (4 * kMaskThreads),
+                                    max((groups + 16 * kMaskThreads - 1) / (16 * kMaskThreads), 4 * sms / S)));
+  auto s = static_cast<cudaStream_t>(stream);
+  const bool penalties = B > 0 && (text || bias_cu);
+  return f32 ? launch<float>(p, penalties, mask_parts, s) : launch<__nv_bfloat16>(p, penalties, mask_parts, s);
 }
