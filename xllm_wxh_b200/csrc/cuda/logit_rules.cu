@@ -9,10 +9,10 @@
 //   penalties: (sequence, part, rows) - counts the history's ids in a table in shared memory, so that nothing of the history has to be
 //              counted and sent by the host, and touches only the logits whose ids are in it (one sector each); forbidden ids are left
 //              to the other kernel.  Bound by the latency of a few dependent loads when there are few rows.
-// The table is a hash table (linear probing) where history and biases are sure to fit.  Longer ones are tried, since text has far fewer
-// distinct ids than tokens; where an id finds no place within kProbes, or the history is longer still, the CTA goes through the
-// vocabulary slice by slice with the table as a plain array, so that any history works.  Counts are whole
-// numbers and the last bias of an id wins by its index: the order in which threads arrive changes nothing.
+// The ids that a CTA has to do with (history, path, biases) are marked in a bitmap of the vocabulary; an id's rank in it is its place in
+// the table of counts, so that the table is as long as there are distinct ids, nothing is probed for, and the logits are visited in
+// the order of their addresses.  More ids than the table holds are taken window by window, larger vocabularies slice by slice.  Counts
+// are whole numbers and the last bias of an id wins by its index: the order in which threads arrive changes nothing.
 #include <atomic>
 
 #include "vec8.cuh"
@@ -20,8 +20,8 @@
 namespace xl_lr {
 using namespace xl;
 
-constexpr int kThreads = 512, kMaskThreads = 256;
-constexpr int kPathRows = 256, kProbes = 64, kMaxSlots = 7680;   // two such tables fit an SM
+constexpr int kThreads = 512, kWarps = kThreads / 32, kMaskThreads = 256;
+constexpr int kPathRows = 256, kMaxWords = 8192, kMaxSlots = 4608;   // ids of a bitmap / 32; entries of the table
 constexpr uint32_t kPrompt = 0x80000000u, kOnPath = 0x40000000u, kMade = 0x3FFFFFFFu;
 
 struct Params {
@@ -43,49 +43,48 @@ struct Params {
   const int* words;             // [n_masks, words_ld], bit 1: allowed (null: no masks)
   const int* mask_of;           // [S]
   int words_ld, n_masks;
-  int slots;                    // entries of the table
-  int parts, row_parts;         // CTAs that share a sequence's vocabulary slices, and its rows
+  int slots, bitmap_words;      // entries of the table, words of the bitmap
+  int parts, row_parts;         // CTAs that share a sequence's windows, and its rows
 };
 
 // ---------------------------------------------------------------- masks
-// Groups of 16 bytes start on 16-byte boundaries of the row's address.  A group's bits straddle two words of the mask.
+// A warp takes 32 words of the mask at a time, one a lane, and writes their columns in pieces of 512 bytes, 16 a lane, on 16-byte
+// boundaries of the row's address (so that a lane's columns may straddle two words).
 template <typename T>
 __global__ void __launch_bounds__(kMaskThreads) mask_logits_kernel(const Params p, int parts) {
   grid_dep_launch();
   const int row = blockIdx.x / parts;
   const int m = p.mask_of[row];
   if (m < 0 || m >= p.n_masks) return;
-  constexpr int G = 16 / sizeof(T);
+  constexpr int G = 16 / sizeof(T), kPer = 32 / G;                 // columns of a lane; lanes of a word
   constexpr uint32_t kAll = (1u << G) - 1, kLow = sizeof(T) == 2 ? 0xFF80FF80u : 0xFF800000u;
   T* x = static_cast<T*>(p.logits) + size_t(row) * p.ld;
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(p.words) + size_t(m) * p.words_ld;
-  const int n_words = (p.V + 31) / 32;
-  const int shift = int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % G), groups = (p.V + shift + G - 1) / G;
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(p.words) + size_t(m) * p.words_ld;
+  const int n_words = (p.V + 31) / 32, lane = threadIdx.x & 31;
+  const int shift = int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % G);       // the lanes' columns start `shift` ahead of the words'
   T low;
   from_f32(&low, -INFINITY);
-  const int share = (groups + parts - 1) / parts, g1 = min(groups, int(blockIdx.x % parts + 1) * share);
-  for (int g0 = blockIdx.x % parts * share + threadIdx.x; g0 < g1; g0 += 4 * kMaskThreads) {
-    uint32_t bits[4];
+  const int warp = (blockIdx.x % parts) * (kMaskThreads / 32) + (threadIdx.x >> 5), warps = parts * (kMaskThreads / 32);
+  for (int w0 = warp * 32; w0 < n_words + 1; w0 += warps * 32) {   // (the last columns may need a word's worth of lanes more)
+    auto word = [&](int w) {                                       // columns past the vocabulary count as allowed
+      if (w < 0 || w >= n_words) return ~0u;
+      const uint32_t v = words[w];
+      return w == n_words - 1 && (p.V & 31) ? v | (~0u << (p.V & 31)) : v;
+    };
+    const uint32_t mine = word(w0 + lane), before = word(w0 - 1);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int g = g0 + i * kMaskThreads, t = g * G - shift, at = t >> 5;        // t may start below 0
-      bits[i] = kAll;
-      if (g < g1) {
-        const uint32_t lo = at >= 0 ? w[at] : ~0u, hi = at + 1 < n_words && (t & 31) > 32 - G ? w[at + 1] : ~0u;
-        bits[i] = __funnelshift_r(lo, hi, t & 31) & kAll;
-        if (t < 0) bits[i] |= (1u << -t) - 1;
-        if (t + G > p.V) bits[i] |= kAll & ~((1u << (p.V - t)) - 1);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = (g0 + i * kMaskThreads) * G - shift;
-      if (bits[i] == 0) {
+    for (int k = 0; k < kPer; ++k) {
+      const int at = k * (32 / kPer) + lane / kPer, bit = lane % kPer * G - shift;
+      const uint32_t hi = __shfl_sync(0xffffffffu, mine, at), up = __shfl_sync(0xffffffffu, mine, (at + 31) & 31);
+      const uint32_t lo = at == 0 ? before : up;
+      const uint32_t bits = (bit >= 0 ? hi >> bit : __funnelshift_r(lo, hi, bit & 31)) & kAll;
+      const int t = (w0 + at) * 32 + bit;
+      if (bits == 0) {
         *reinterpret_cast<uint4*>(x + t) = make_uint4(kLow, kLow, kLow, kLow);
-      } else if (bits[i] != kAll) {
+      } else if (bits != kAll) {
 #pragma unroll
         for (int e = 0; e < G; ++e)
-          if (!(bits[i] >> e & 1u)) x[t + e] = low;
+          if (!(bits >> e & 1u)) x[t + e] = low;
       }
     }
   }
@@ -113,14 +112,15 @@ struct PathSmem {                // of a row of the sequence (only where rows ha
 template <typename T>
 __global__ void __launch_bounds__(kThreads) penalise_logits_kernel(const Params p) {
   extern __shared__ __align__(16) uint8_t smem[];
-  const int tid = threadIdx.x, C = p.slots;
-  int* s_id = reinterpret_cast<int*>(smem);                        // [C]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, C = p.slots, W = p.bitmap_words;
+  uint32_t* s_bits = reinterpret_cast<uint32_t*>(smem);            // [W] ids of the slice that are there
+  int* s_rank = reinterpret_cast<int*>(s_bits + W);                // [W] how many ahead of the word
+  int* s_id = s_rank + W;                                          // [C]
   uint32_t* s_word = reinterpret_cast<uint32_t*>(s_id + C);        // [C]
   int* s_bias = reinterpret_cast<int*>(s_word + C);                // [C] index of the bias
-  uint16_t* s_list = reinterpret_cast<uint16_t*>(s_bias + C);      // [C] entries that change something
-  PathSmem* path_of = reinterpret_cast<PathSmem*>(s_list + C);     // [max_q]
+  PathSmem* path_of = reinterpret_cast<PathSmem*>(s_bias + C);     // [max_q]
   __shared__ unsigned long long s_made[4];                         // rows whose tokens lie behind the prompt
-  __shared__ int s_count, s_firsts, s_full;
+  __shared__ int s_firsts, s_total[kWarps];
 
   const int part = blockIdx.x % p.parts, rp = blockIdx.x / p.parts % p.row_parts, b = blockIdx.x / p.parts / p.row_parts;
   const int src = p.seqs ? p.seqs[b] : b;
@@ -184,140 +184,141 @@ __global__ void __launch_bounds__(kThreads) penalise_logits_kernel(const Params 
     }
   }
 
-  // Attempt 0 hashes, attempt 1 goes through slices.  Parts that share a sequence's slices must not differ on it: they hash only what
-  // is sure to fit, and leave that to the first of them.
-  const long most = long(len) + (e1 - e0);
-  const bool sure = most <= C / 8 * 7;
-  const int probes = sure ? C : kProbes;
-  for (int attempt = sure || (p.parts == 1 && most <= 4l * C) ? 0 : 1; attempt < 2; ++attempt) {
-    const bool hashed = attempt == 0;
-    if (hashed && part > 0) break;
-    const int slices = hashed ? 1 : (p.V + C - 1) / C;
-    bool full = false;
-    for (int slice = hashed ? 0 : part; slice < slices; slice += p.parts) {
-      const int v0 = hashed ? 0 : slice * C, v1 = hashed ? p.V : min(p.V, v0 + C);
-      __syncthreads();
-      for (int i = 4 * tid; i < C; i += 4 * kThreads) {
-        *reinterpret_cast<int4*>(s_id + i) = hashed ? make_int4(-1, -1, -1, -1) : make_int4(v0 + i, v0 + i + 1, v0 + i + 2, v0 + i + 3);
-        *reinterpret_cast<int4*>(s_word + i) = make_int4(0, 0, 0, 0);
-        *reinterpret_cast<int4*>(s_bias + i) = make_int4(-1, -1, -1, -1);
-      }
-      if (tid == 0) s_count = s_firsts = s_full = 0;
-      __syncthreads();
-      auto first_slot = [&](int id) { return int(__umulhi(uint32_t(id) * 2654435761u, uint32_t(C))); };
-      auto entry = [&](int id) {                                   // -1: no place
-        if (!hashed) return id - v0;
-        int at = first_slot(id);
-        for (int k = 0; k < probes; ++k) {
-          const int was = atomicCAS(&s_id[at], -1, id);
-          if (was == -1 || was == id) return at;
-          at = at + 1 < C ? at + 1 : 0;
-        }
-        s_full = 1;
-        return -1;
-      };
-      auto find = [&](int id) {
-        if (!hashed) return id - v0;
-        int at = first_slot(id);
-        for (int k = 0; k < probes && s_id[at] != -1; ++k) {
-          if (s_id[at] == id) return at;
-          at = at + 1 < C ? at + 1 : 0;
-        }
-        return -1;
-      };
+  int window = 0;                                                  // of all slices
+  for (int v0 = 0; v0 < p.V; v0 += 32 * W) {
+    const int v1 = min(p.V, v0 + 32 * W);
+    __syncthreads();
+    for (int i = tid; i < W; i += kThreads) s_bits[i] = 0;
+    __syncthreads();
+    auto mark = [&](int id) {
+      if (id < v0 || id >= v1) return;
+      uint32_t* w = &s_bits[(id - v0) >> 5];
+      const uint32_t bit = 1u << ((id - v0) & 31);
+      if (!(*reinterpret_cast<volatile uint32_t*>(w) & bit)) atomicOr(w, bit);   // frequent ids are there already
+    };
+    auto each_of_text = [&](auto&& f) {                            // eight loads at a time
       for (int i0 = tid; i0 < len; i0 += 8 * kThreads) {
         int id[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) id[k] = i0 + k * kThreads < len ? text[i0 + k * kThreads] : -1;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (id[k] < v0 || id[k] >= v1) continue;
-          const int at = entry(id[k]);
-          if (at < 0) continue;
-          if (i0 + k * kThreads < prompt) atomicOr(&s_word[at], kPrompt);
-          else atomicAdd(&s_word[at], 1u);
-        }
+        for (int k = 0; k < 8; ++k) f(id[k], i0 + k * kThreads);
       }
+    };
+    each_of_text([&](int id, int) { mark(id); });
+    for (int e = e0 + tid; e < e1; e += kThreads) mark(p.bias_ids[e]);
+    if (tid < path) mark(path_of[tid].token);
+    __syncthreads();
+    // ranks: a warp sums its stretch of the words, 32 at a time, then adds what lies ahead
+    const int stretch = (W + kThreads - 1) / kThreads * 32, b0 = warp * stretch, b1 = min(W, b0 + stretch);
+    int run = 0;
+    for (int w0 = b0; w0 < b1; w0 += 32) {
+      const int c = w0 + lane < b1 ? __popc(s_bits[w0 + lane]) : 0;
+      int incl = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (w0 + lane < b1) s_rank[w0 + lane] = run + incl - c;
+      run += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) s_total[warp] = run;
+    __syncthreads();
+    int ahead = 0, distinct = 0;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      if (i < warp) ahead += s_total[i];
+      distinct += s_total[i];
+    }
+    for (int w = b0 + lane; w < b1; w += 32) s_rank[w] += ahead;
+    __syncthreads();
+    auto rank = [&](int id) { return s_rank[(id - v0) >> 5] + __popc(s_bits[(id - v0) >> 5] & ((1u << ((id - v0) & 31)) - 1)); };
+
+    for (int k0 = 0; k0 < distinct; k0 += C, ++window) {
+      if (window % p.parts != part) continue;
+      const int count = min(C, distinct - k0);
+      __syncthreads();
+      for (int i = tid; i < count; i += kThreads) {
+        s_word[i] = 0;
+        s_bias[i] = -1;
+      }
+      for (int w = b0 + lane; w < b1; w += 32) {
+        int k = s_rank[w] - k0;
+        for (uint32_t todo = s_bits[w]; todo; todo &= todo - 1, ++k)
+          if (k >= 0 && k < C) s_id[k] = v0 + w * 32 + __ffs(todo) - 1;
+      }
+      if (tid == 0) s_firsts = 0;
+      __syncthreads();
+      each_of_text([&](int id, int i) {
+        if (id < v0 || id >= v1) return;
+        const int k = rank(id) - k0;
+        if (k < 0 || k >= count) return;
+        if (i >= prompt) atomicAdd(&s_word[k], 1u);
+        else if (!(*reinterpret_cast<volatile uint32_t*>(&s_word[k]) & kPrompt)) atomicOr(&s_word[k], kPrompt);
+      });
       for (int e = e0 + tid; e < e1; e += kThreads) {
         const int id = p.bias_ids[e];
         if (id < v0 || id >= v1) continue;
-        const int at = entry(id);
-        if (at >= 0) atomicMax(&s_bias[at], e);
+        const int k = rank(id) - k0;
+        if (k >= 0 && k < count) atomicMax(&s_bias[k], e);
       }
       __syncthreads();
-      full = s_full;
-      if (full) break;                                             // (only a hash table fills up)
       // ids on the path: one entry for each distinct one, with the set of the rows that hold it; their counts differ from row to row
       if (tid < path) {
         const int id = path_of[tid].token;
-        bool first = id >= v0 && id < v1;
-        unsigned long long same[4] = {0, 0, 0, 0};
-        for (int i = 0; i < path; ++i) {
-          const bool eq = path_of[i].token == id;
-          first = first && !(eq && i < tid);
+        const int k = id >= v0 && id < v1 ? rank(id) - k0 : -1;
+        if (k >= 0 && k < count) {
+          bool first = true;
+          unsigned long long same[4] = {0, 0, 0, 0};
+          for (int i = 0; i < path; ++i) {
+            const bool eq = path_of[i].token == id;
+            first = first && !(eq && i < tid);
 #pragma unroll
-          for (int w = 0; w < 4; ++w)
-            if (eq && w == (i >> 6)) same[w] |= 1ull << (i & 63);
-        }
-        if (first) {
-          const int at = find(id);
-          uint32_t word = 0;
-          int e = -1;
-          if (at >= 0) {
-            word = s_word[at];
-            e = s_bias[at];
-            s_word[at] = word | kOnPath;
+            for (int w = 0; w < 4; ++w)
+              if (eq && w == (i >> 6)) same[w] |= 1ull << (i & 63);
           }
-          path_of[tid].word = word;
-          path_of[tid].bias = e;
+          if (first) {
+            const uint32_t word = s_word[k];
+            path_of[tid].word = word;
+            path_of[tid].bias = s_bias[k];
+            s_word[k] = word | kOnPath;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) path_of[tid].same[w] = same[w];
-          path_of[atomicAdd(&s_firsts, 1)].first = tid;
+            for (int w = 0; w < 4; ++w) path_of[tid].same[w] = same[w];
+            path_of[atomicAdd(&s_firsts, 1)].first = tid;
+          }
         }
       }
       __syncthreads();
-      for (int i = tid; i < C; i += kThreads) {
-        const uint32_t word = s_word[i];
-        const bool keep = !(word & kOnPath) && (word != 0 || s_bias[i] >= 0);
-        const uint32_t votes = __ballot_sync(0xffffffffu, keep);
-        int at = 0;
-        if ((tid & 31) == 0 && votes) at = atomicAdd(&s_count, __popc(votes));
-        at = __shfl_sync(0xffffffffu, at, 0) + __popc(votes & ((1u << (tid & 31)) - 1));
-        if (keep) s_list[at] = uint16_t(i);
-      }
-      __syncthreads();
-      const int count = s_count, firsts = s_firsts, rows = r1 - r0;
+      const int firsts = s_firsts, rows = r1 - r0;
       T* x0 = static_cast<T*>(p.logits);
-      auto allowed = [&](int row, int id) {
-        if (!p.words) return true;
+      // what a row's mask says of an id: word and bit, looked up ahead of the logit, which a forbidden id leaves alone
+      auto mask_word = [&](int row, int id) {
+        if (!p.words) return ~0u;
         const int m = p.mask_of[row];
-        return m < 0 || m >= p.n_masks || (p.words[size_t(m) * p.words_ld + (id >> 5)] >> (id & 31) & 1);
+        return m < 0 || m >= p.n_masks ? ~0u : uint32_t(p.words[size_t(m) * p.words_ld + (id >> 5)]);
       };
       // four logits at a time, so that their loads are under way together
       for (int i0 = tid; i0 < count * rows; i0 += 4 * kThreads) {
         T* at[4];
         float x[4];
-        int slot[4];
+        int entry[4];
+        uint32_t open[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int i = i0 + k * kThreads;
-          at[k] = nullptr;
-          x[k] = 0.f;
-          slot[k] = 0;
-          if (i < count * rows) {
-            const int r = i / count, row = start + r0 + r;
-            slot[k] = s_list[i - r * count];
-            const int id = s_id[slot[k]];
-            T* to = x0 + size_t(row) * p.ld + id;
-            x[k] = to_f32(*to);
-            if (allowed(row, id)) at[k] = to;
-          }
+          const int i = min(i0 + k * kThreads, count * rows - 1), r = i / count, row = start + r0 + r;
+          entry[k] = i - r * count;
+          const int id = s_id[entry[k]];
+          at[k] = x0 + size_t(row) * p.ld + id;
+          open[k] = i0 + k * kThreads < count * rows && !(s_word[entry[k]] & kOnPath) ? mask_word(row, id) >> (id & 31) & 1u : 0u;
         }
 #pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = open[k] ? to_f32(*at[k]) : 0.f;
+#pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (at[k]) {
-            const int e = s_bias[slot[k]];
-            from_f32(at[k], adjusted(x[k], s_word[slot[k]], e >= 0 ? p.bias_values[e] : 0.f, e >= 0, rep, freq, pres));
+          if (open[k]) {
+            const int e = s_bias[entry[k]];
+            from_f32(at[k], adjusted(x[k], s_word[entry[k]], e >= 0 ? p.bias_values[e] : 0.f, e >= 0, rep, freq, pres));
           }
       }
       for (int i = tid; i < firsts * rows; i += kThreads) {
@@ -332,12 +333,11 @@ __global__ void __launch_bounds__(kThreads) penalise_logits_kernel(const Params 
         }
         const uint32_t word = (path_of[f].word + uint32_t(more)) | (before ? kPrompt : 0u);
         const int e = path_of[f].bias;
-        if ((word == 0 && e < 0) || !allowed(row, id)) continue;
+        if ((word == 0 && e < 0) || !(mask_word(row, id) >> (id & 31) & 1u)) continue;
         T* x = x0 + size_t(row) * p.ld + id;
         from_f32(x, adjusted(to_f32(*x), word, e >= 0 ? p.bias_values[e] : 0.f, e >= 0, rep, freq, pres));
       }
     }
-    if (hashed && !full) break;
   }
   grid_dep_wait();                                                 // what follows on the stream waits for this kernel only
 }
@@ -358,13 +358,13 @@ int launch(const Params& p, bool penalties, int mask_parts, cudaStream_t s) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
   if (!ready[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 14 * kMaxSlots + int(sizeof(PathSmem)) * kPathRows) != cudaSuccess) return -1;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * kMaxWords + 12 * kMaxSlots + int(sizeof(PathSmem)) * kPathRows) != cudaSuccess) return -1;
     ready[dev].store(true, std::memory_order_release);
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(grid));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = 14 * p.slots + (p.tokens ? sizeof(PathSmem) * p.max_q : 0);
+  cfg.dynamicSmemBytes = 8 * p.bitmap_words + 12 * p.slots + (p.tokens ? sizeof(PathSmem) * p.max_q : 0);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -407,16 +407,16 @@ XL_API int xl_adjust_logits(void* logits, int f32, int S, int V, long ld, const 
   p.mask_of = static_cast<const int*>(mask_of);
   p.words_ld = words_ld; p.n_masks = n_masks;
   const int sms = xl_host::sm_count();
-  // a table that holds any history of the given length; long ones go by their distinct ids, which text has far fewer of
-  p.slots = int(min(long(kMaxSlots), (long(text ? text_cap : 0) + 64) / 448 * 512 + 512));
-  // rows of a sequence over several CTAs (each counts the history again), as long as there are SMs without one; slices of the
-  // vocabulary, where histories are too long to be hashed
+  // a table that holds any history of the given length; of long ones their distinct ids, which text has far fewer of, at a time
+  p.bitmap_words = (min((V + 31) / 32, kMaxWords) + 1) & ~1;
+  p.slots = int(min(long(kMaxSlots), ((text ? text_cap : 0) + long(n_bias) + max_q + 31) / 32 * 32));
+  // rows of a sequence over several CTAs (each counts the history again), as long as there are SMs without one; windows, where
+  // histories are long enough to need several
   p.row_parts = B > 0 ? max(1, min(min(max_q, S), 2 * sms / B)) : 1;
-  p.parts = B > 0 && text && text_cap > 4l * p.slots ? max(1, min((V + p.slots - 1) / p.slots, 2 * sms / (B * p.row_parts))) : 1;
-  // 16-byte groups of a row over CTAs of up to 4 x 4 groups a thread, smaller ones where there are few rows
-  const int groups = V * (f32 ? 4 : 2) / 16 + 2;
-  const int mask_parts = max(1, min((groups + 4 * kMaskThreads - 1) / (4 * kMaskThreads),
-                                    max((groups + 16 * kMaskThreads - 1) / (16 * kMaskThreads), 4 * sms / S)));
+  p.parts = B > 0 && text && text_cap > 4l * p.slots ? max(1, min(text_cap / p.slots + 1, 2 * sms / (B * p.row_parts))) : 1;
+  // a row's mask over CTAs of eight warps: four times 32 words a warp, fewer where there are few rows
+  const int per_cta = kMaskThreads, n_words = (V + 31) / 32 + 1;
+  const int mask_parts = max(1, min((n_words + per_cta - 1) / per_cta, max((n_words + 4 * per_cta - 1) / (4 * per_cta), 8 * sms / S)));
   auto s = static_cast<cudaStream_t>(stream);
   const bool penalties = B > 0 && (text || bias_cu);
   return f32 ? launch<float>(p, penalties, mask_parts, s) : launch<__nv_bfloat16>(p, penalties, mask_parts, s);
