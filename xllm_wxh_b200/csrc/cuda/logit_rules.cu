@@ -65,26 +65,38 @@ __global__ void __launch_bounds__(kMaskThreads) mask_logits_kernel(const Params 
   T low;
   from_f32(&low, -INFINITY);
   const int warp = (blockIdx.x % parts) * (kMaskThreads / 32) + (threadIdx.x >> 5), warps = parts * (kMaskThreads / 32);
+  auto word = [&](int w) {                                         // columns past the vocabulary count as allowed
+    if (w < 0 || w >= n_words) return ~0u;
+    const uint32_t v = words[w];
+    return w == n_words - 1 && (p.V & 31) ? v | (~0u << (p.V & 31)) : v;
+  };
+  auto put = [&](uint32_t bits, int t) {
+    if (bits == 0) {
+      *reinterpret_cast<uint4*>(x + t) = make_uint4(kLow, kLow, kLow, kLow);
+    } else if (bits != kAll) {
+#pragma unroll
+      for (int e = 0; e < G; ++e)
+        if (!(bits >> e & 1u)) x[t + e] = low;
+    }
+  };
+  const int bit = lane % kPer * G - shift;
+  uint32_t next = word(warp * 32 + lane), next_before = word(warp * 32 - 1);
   for (int w0 = warp * 32; w0 < n_words + 1; w0 += warps * 32) {   // (the last columns may need a word's worth of lanes more)
-    auto word = [&](int w) {                                       // columns past the vocabulary count as allowed
-      if (w < 0 || w >= n_words) return ~0u;
-      const uint32_t v = words[w];
-      return w == n_words - 1 && (p.V & 31) ? v | (~0u << (p.V & 31)) : v;
-    };
-    const uint32_t mine = word(w0 + lane), before = word(w0 - 1);
+    const uint32_t mine = next, before = next_before;
+    next = word(w0 + warps * 32 + lane);
+    next_before = word(w0 + warps * 32 - 1);
+    if (__all_sync(0xffffffffu, mine == ~0u) && before == ~0u) continue;
+    const int t0 = (w0 + lane / kPer) * 32 + bit;
+    if (shift == 0) {                                              // (of the whole row)
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int at = k * (32 / kPer) + lane / kPer, bit = lane % kPer * G - shift;
-      const uint32_t hi = __shfl_sync(0xffffffffu, mine, at), up = __shfl_sync(0xffffffffu, mine, (at + 31) & 31);
-      const uint32_t lo = at == 0 ? before : up;
-      const uint32_t bits = (bit >= 0 ? hi >> bit : __funnelshift_r(lo, hi, bit & 31)) & kAll;
-      const int t = (w0 + at) * 32 + bit;
-      if (bits == 0) {
-        *reinterpret_cast<uint4*>(x + t) = make_uint4(kLow, kLow, kLow, kLow);
-      } else if (bits != kAll) {
+      for (int k = 0; k < kPer; ++k)
+        put(__shfl_sync(0xffffffffu, mine, k * (32 / kPer) + lane / kPer) >> bit & kAll, t0 + k * (32 / kPer) * 32);
+    } else {
 #pragma unroll
-        for (int e = 0; e < G; ++e)
-          if (!(bits >> e & 1u)) x[t + e] = low;
+      for (int k = 0; k < kPer; ++k) {
+        const int at = k * (32 / kPer) + lane / kPer;
+        const uint32_t hi = __shfl_sync(0xffffffffu, mine, at), up = __shfl_sync(0xffffffffu, mine, (at + 31) & 31);
+        put((bit >= 0 ? hi >> bit : __funnelshift_r(at == 0 ? before : up, hi, bit & 31)) & kAll, t0 + k * (32 / kPer) * 32);
       }
     }
   }
@@ -110,7 +122,7 @@ struct PathSmem {                // of a row of the sequence (only where rows ha
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) penalise_logits_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 2) penalise_logits_kernel(const Params p) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, C = p.slots, W = p.bitmap_words;
   uint32_t* s_bits = reinterpret_cast<uint32_t*>(smem);            // [W] ids of the slice that are there
@@ -209,29 +221,30 @@ __global__ void __launch_bounds__(kThreads) penalise_logits_kernel(const Params 
     for (int e = e0 + tid; e < e1; e += kThreads) mark(p.bias_ids[e]);
     if (tid < path) mark(path_of[tid].token);
     __syncthreads();
-    // ranks: a warp sums its stretch of the words, 32 at a time, then adds what lies ahead
-    const int stretch = (W + kThreads - 1) / kThreads * 32, b0 = warp * stretch, b1 = min(W, b0 + stretch);
-    int run = 0;
-    for (int w0 = b0; w0 < b1; w0 += 32) {
-      const int c = w0 + lane < b1 ? __popc(s_bits[w0 + lane]) : 0;
-      int incl = c;
+    // ranks: every thread sums its stretch of the words.  (Short loops: code that runs once per launch costs its fetch.)
+    const int each = (W + kThreads - 1) / kThreads, b0 = min(W, tid * each), b1 = min(W, b0 + each);
+    int sum = 0;
+#pragma unroll 1
+    for (int w = b0; w < b1; ++w) sum += __popc(s_bits[w]);
+    int incl = sum;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-      }
-      if (w0 + lane < b1) s_rank[w0 + lane] = run + incl - c;
-      run += __shfl_sync(0xffffffffu, incl, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
     }
-    if (lane == 0) s_total[warp] = run;
+    if (lane == 31) s_total[warp] = incl;
     __syncthreads();
-    int ahead = 0, distinct = 0;
-#pragma unroll
+    int run = incl - sum, distinct = 0;
+#pragma unroll 4
     for (int i = 0; i < kWarps; ++i) {
-      if (i < warp) ahead += s_total[i];
+      if (i < warp) run += s_total[i];
       distinct += s_total[i];
     }
-    for (int w = b0 + lane; w < b1; w += 32) s_rank[w] += ahead;
+#pragma unroll 1
+    for (int w = b0; w < b1; ++w) {
+      s_rank[w] = run;
+      run += __popc(s_bits[w]);
+    }
     __syncthreads();
     auto rank = [&](int id) { return s_rank[(id - v0) >> 5] + __popc(s_bits[(id - v0) >> 5] & ((1u << ((id - v0) & 31)) - 1)); };
 
@@ -243,17 +256,13 @@ __global__ void __launch_bounds__(kThreads) penalise_logits_kernel(const Params 
         s_word[i] = 0;
         s_bias[i] = -1;
       }
-      for (int w = b0 + lane; w < b1; w += 32) {
-        int k = s_rank[w] - k0;
-        for (uint32_t todo = s_bits[w]; todo; todo &= todo - 1, ++k)
-          if (k >= 0 && k < C) s_id[k] = v0 + w * 32 + __ffs(todo) - 1;
-      }
       if (tid == 0) s_firsts = 0;
       __syncthreads();
       each_of_text([&](int id, int i) {
         if (id < v0 || id >= v1) return;
         const int k = rank(id) - k0;
         if (k < 0 || k >= count) return;
+        s_id[k] = id;
         if (i >= prompt) atomicAdd(&s_word[k], 1u);
         else if (!(*reinterpret_cast<volatile uint32_t*>(&s_word[k]) & kPrompt)) atomicOr(&s_word[k], kPrompt);
       });
@@ -261,7 +270,9 @@ __global__ void __launch_bounds__(kThreads) penalise_logits_kernel(const Params 
         const int id = p.bias_ids[e];
         if (id < v0 || id >= v1) continue;
         const int k = rank(id) - k0;
-        if (k >= 0 && k < count) atomicMax(&s_bias[k], e);
+        if (k < 0 || k >= count) continue;
+        s_id[k] = id;
+        atomicMax(&s_bias[k], e);
       }
       __syncthreads();
       // ids on the path: one entry for each distinct one, with the set of the rows that hold it; their counts differ from row to row
@@ -414,9 +425,9 @@ XL_API int xl_adjust_logits(void* logits, int f32, int S, int V, long ld, const 
   // histories are long enough to need several
   p.row_parts = B > 0 ? max(1, min(min(max_q, S), 2 * sms / B)) : 1;
   p.parts = B > 0 && text && text_cap > 4l * p.slots ? max(1, min(text_cap / p.slots + 1, 2 * sms / (B * p.row_parts))) : 1;
-  // a row's mask over CTAs of eight warps: four times 32 words a warp, fewer where there are few rows
+  // a row's mask over CTAs of eight warps, 32 words a warp at a time: two rounds of resident CTAs where there are rows enough
   const int per_cta = kMaskThreads, n_words = (V + 31) / 32 + 1;
-  const int mask_parts = max(1, min((n_words + per_cta - 1) / per_cta, max((n_words + 4 * per_cta - 1) / (4 * per_cta), 8 * sms / S)));
+  const int mask_parts = max(1, min((n_words + per_cta - 1) / per_cta, 16 * sms / S));
   auto s = static_cast<cudaStream_t>(stream);
   const bool penalties = B > 0 && (text || bias_cu);
   return f32 ? launch<float>(p, penalties, mask_parts, s) : launch<__nv_bfloat16>(p, penalties, mask_parts, s);
