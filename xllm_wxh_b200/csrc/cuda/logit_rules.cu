@@ -52,11 +52,15 @@ struct Params {
 // boundaries of the row's address (so that a lane's columns may straddle two words).
 template <typename T>
 __global__ void __launch_bounds__(kMaskThreads) mask_logits_kernel(const Params p, int parts) {
-  grid_dep_launch();
   const int row = blockIdx.x / parts;
   const int m = p.mask_of[row];
-  if (m < 0 || m >= p.n_masks) return;
-  constexpr int G = 16 / sizeof(T), kPer = 32 / G;                 // columns of a lane; lanes of a word
+  // what follows on the stream waits for this kernel only, so its last CTA stays until the penalties are done
+  const bool last = blockIdx.x == gridDim.x - 1;
+  if (m < 0 || m >= p.n_masks) {
+    if (last) grid_dep_wait();
+    return;
+  }
+  constexpr int G = 16 / sizeof(T), kPer = 32 / G;                 // columns of a lane, and words of a piece; lanes of a word
   constexpr uint32_t kAll = (1u << G) - 1, kLow = sizeof(T) == 2 ? 0xFF80FF80u : 0xFF800000u;
   T* x = static_cast<T*>(p.logits) + size_t(row) * p.ld;
   const uint32_t* words = reinterpret_cast<const uint32_t*>(p.words) + size_t(m) * p.words_ld;
@@ -89,17 +93,26 @@ __global__ void __launch_bounds__(kMaskThreads) mask_logits_kernel(const Params 
     const int t0 = (w0 + lane / kPer) * 32 + bit;
     if (shift == 0) {                                              // (of the whole row)
 #pragma unroll
-      for (int k = 0; k < kPer; ++k)
-        put(__shfl_sync(0xffffffffu, mine, k * (32 / kPer) + lane / kPer) >> bit & kAll, t0 + k * (32 / kPer) * 32);
+      for (int k = 0; k < kPer; ++k) {
+        const uint32_t bits = __shfl_sync(0xffffffffu, mine, k * G + lane / kPer) >> bit & kAll;
+        if (__any_sync(0xffffffffu, bits != 0 && bits != kAll)) {  // column by column, a word at a time
+#pragma unroll
+          for (int e = 0; e < G; ++e)
+            if (!(__shfl_sync(0xffffffffu, mine, k * G + e) >> lane & 1u)) x[(w0 + k * G + e) * 32 + lane] = low;
+        } else if (bits == 0) {
+          *reinterpret_cast<uint4*>(x + t0 + k * G * 32) = make_uint4(kLow, kLow, kLow, kLow);
+        }
+      }
     } else {
 #pragma unroll
       for (int k = 0; k < kPer; ++k) {
-        const int at = k * (32 / kPer) + lane / kPer;
+        const int at = k * G + lane / kPer;
         const uint32_t hi = __shfl_sync(0xffffffffu, mine, at), up = __shfl_sync(0xffffffffu, mine, (at + 31) & 31);
-        put((bit >= 0 ? hi >> bit : __funnelshift_r(at == 0 ? before : up, hi, bit & 31)) & kAll, t0 + k * (32 / kPer) * 32);
+        put((bit >= 0 ? hi >> bit : __funnelshift_r(at == 0 ? before : up, hi, bit & 31)) & kAll, t0 + k * G * 32);
       }
     }
   }
+  if (last) grid_dep_wait();
 }
 
 // ---------------------------------------------------------------- penalties and biases
@@ -124,6 +137,7 @@ struct PathSmem {                // of a row of the sequence (only where rows ha
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) penalise_logits_kernel(const Params p) {
   extern __shared__ __align__(16) uint8_t smem[];
+  grid_dep_launch();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, C = p.slots, W = p.bitmap_words;
   uint32_t* s_bits = reinterpret_cast<uint32_t*>(smem);            // [W] ids of the slice that are there
   int* s_rank = reinterpret_cast<int*>(s_bits + W);                // [W] how many ahead of the word
@@ -139,10 +153,7 @@ __global__ void __launch_bounds__(kThreads, 2) penalise_logits_kernel(const Para
   const int start = max(p.q_cu[b], 0), n = min(min(p.q_cu[b + 1], p.S) - start, p.max_q);
   const int share = (max(n, 0) + p.row_parts - 1) / p.row_parts;
   const int r0 = rp * share, r1 = min(n, r0 + share);
-  if (unsigned(src) >= unsigned(p.pool) || r0 >= r1) {
-    grid_dep_wait();
-    return;
-  }
+  if (unsigned(src) >= unsigned(p.pool) || r0 >= r1) return;
   float rep = 1.f, freq = 0.f, pres = 0.f;
   int given = 0, prompt = 0, e0 = 0, e1 = 0;
   if (p.text) {
@@ -157,10 +168,7 @@ __global__ void __launch_bounds__(kThreads, 2) penalise_logits_kernel(const Para
   const bool penal = rep != 1.f || freq != 0.f || pres != 0.f;     // otherwise the history changes nothing
   const int len = penal ? min(given, p.text_cap) : 0;
   const int path = penal && p.tokens ? r1 : 0;                     // rows whose tokens can be on a way to the rows r0 .. r1 - 1
-  if (len == 0 && path == 0 && e1 == e0) {
-    grid_dep_wait();
-    return;
-  }
+  if (len == 0 && path == 0 && e1 == e0) return;
   const int* text = p.text + size_t(src) * p.text_ld;
 
   // ancestors of the rows, as sets of rows (by doubling)
@@ -350,39 +358,37 @@ __global__ void __launch_bounds__(kThreads, 2) penalise_logits_kernel(const Para
       }
     }
   }
-  grid_dep_wait();                                                 // what follows on the stream waits for this kernel only
 }
 
+// The penalties come first: they are latency, and leave room for the masks' CTAs, which start as soon as all of theirs run.
 template <typename T>
 int launch(const Params& p, bool penalties, int mask_parts, cudaStream_t s) {
-  if (p.words) {
-    const long grid = long(p.S) * mask_parts;
-    if (grid > 0x7fffffffl) return -2;
-    mask_logits_kernel<T><<<unsigned(grid), kMaskThreads, 0, s>>>(p, mask_parts);
+  const long grid = long(p.B) * p.parts * p.row_parts, mask_grid = long(p.S) * mask_parts;
+  if (grid > 0x7fffffffl || mask_grid > 0x7fffffffl) return -2;
+  if (penalties) {
+    auto* kernel = penalise_logits_kernel<T>;
+    static std::atomic<bool> ready[64];                            // per device
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
+    if (!ready[dev].load(std::memory_order_acquire)) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * kMaxWords + 12 * kMaxSlots + int(sizeof(PathSmem)) * kPathRows) != cudaSuccess)
+        return -1;
+      ready[dev].store(true, std::memory_order_release);
+    }
+    kernel<<<unsigned(grid), kThreads, 8 * p.bitmap_words + 12 * p.slots + (p.tokens ? sizeof(PathSmem) * p.max_q : 0), s>>>(p);
     if (cudaGetLastError() != cudaSuccess) return -1;
   }
-  if (!penalties) return 0;
-  const long grid = long(p.B) * p.parts * p.row_parts;
-  if (grid > 0x7fffffffl) return -2;
-  auto* kernel = penalise_logits_kernel<T>;
-  static std::atomic<bool> ready[64];                              // per device
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
-  if (!ready[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * kMaxWords + 12 * kMaxSlots + int(sizeof(PathSmem)) * kPathRows) != cudaSuccess) return -1;
-    ready[dev].store(true, std::memory_order_release);
-  }
+  if (!p.words) return 0;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(grid));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = 8 * p.bitmap_words + 12 * p.slots + (p.tokens ? sizeof(PathSmem) * p.max_q : 0);
+  cfg.gridDim = dim3(unsigned(mask_grid));
+  cfg.blockDim = dim3(kMaskThreads);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = p.words ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? 0 : -1;
+  cfg.numAttrs = penalties ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, mask_logits_kernel<T>, p, mask_parts) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace xl_lr
@@ -425,9 +431,9 @@ XL_API int xl_adjust_logits(void* logits, int f32, int S, int V, long ld, const 
   // histories are long enough to need several
   p.row_parts = B > 0 ? max(1, min(min(max_q, S), 2 * sms / B)) : 1;
   p.parts = B > 0 && text && text_cap > 4l * p.slots ? max(1, min(text_cap / p.slots + 1, 2 * sms / (B * p.row_parts))) : 1;
-  // a row's mask over CTAs of eight warps, 32 words a warp at a time: two rounds of resident CTAs where there are rows enough
-  const int per_cta = kMaskThreads, n_words = (V + 31) / 32 + 1;
-  const int mask_parts = max(1, min((n_words + per_cta - 1) / per_cta, 16 * sms / S));
+  // a row's mask over CTAs of eight warps, two times 32 words a warp: in more CTAs their start costs open rows more, in fewer what is
+  // written at a time lies further apart (1024 rows of 152064 fp32: 99 us with one, 102 with two, 107 with four, 122 with nineteen)
+  const int mask_parts = ((V + 31) / 32 + 1 + 2 * kMaskThreads - 1) / (2 * kMaskThreads);
   auto s = static_cast<cudaStream_t>(stream);
   const bool penalties = B > 0 && (text || bias_cu);
   return f32 ? launch<float>(p, penalties, mask_parts, s) : launch<__nv_bfloat16>(p, penalties, mask_parts, s);

@@ -31,41 +31,63 @@ struct RowsParams {
   const int* parents;           // [n_rows] or null
   int *positions, *slots, *token_seq, *q_cu, *kv_lens, *block_tables;
   unsigned long long* tree;     // [n_rows, words] or null
-  int pool, table_ld, B, n_rows, max_q, max_blocks, block_size, words, per_cta;
+  int pool, table_ld, B, n_rows, max_q, max_blocks, block_size, words, per_cta, table_parts, vectors;
 };
 
-// blockIdx.y = sequence (B: the rows behind the last one), blockIdx.x = a part of `per_cta` table entries and of as many rows.
+// blockIdx.y = sequence (B: the rows behind the last one); blockIdx.x = a part of `per_cta` entries of its table, or behind those a part of
+// as many rows.  The table does not wait for the sum of the sequences ahead, which only the rows need.
 __global__ void __launch_bounds__(kThreads) step_rows_kernel(const RowsParams p) {
   __shared__ long s_sum[kThreads / 32];
   __shared__ unsigned long long s_anc[kTreeRows * 4];
   __shared__ int s_up[kTreeRows];
   const int b = blockIdx.y, tid = threadIdx.x;
-  const int lo = blockIdx.x * p.per_cta;
   auto rows_of = [&](int i) { return unsigned(p.seqs[i]) < unsigned(p.pool) ? min(max(p.counts[i], 0), p.max_q) : 0; };
 
   int src = -1, mine = 0, len = 0;
   if (b < p.B) {
     src = p.seqs[b];
+    mine = p.counts[b];
     if (unsigned(src) >= unsigned(p.pool)) src = -1;
-    mine = rows_of(b);
+    mine = src >= 0 ? min(max(mine, 0), p.max_q) : 0;
     len = src >= 0 ? max(p.lens[src], 0) : 0;
-    // the table does not wait for the sum of the sequences ahead
-    const int used = min(long(p.max_blocks), (long(len) + mine + p.block_size - 1) / p.block_size);
-    const int* from = p.tables + size_t(max(src, 0)) * p.table_ld;
-    int* to = p.block_tables + size_t(b) * p.max_blocks;
-    const int hi = min(lo + p.per_cta, p.max_blocks);
-    for (int i = lo + tid; i < hi; i += kThreads) to[i] = i < used ? from[i] : 0;
   }
-  // rows are in the part of blockIdx.x = 0 alone when they form a tree
-  const bool has_rows = b == p.B || (p.parents ? blockIdx.x == 0 : lo < mine || blockIdx.x == 0);
-  if (!has_rows) return;
+  const int* from = p.tables + size_t(max(src, 0)) * p.table_ld;
+  if (int(blockIdx.x) < p.table_parts) {
+    if (b == p.B) return;
+    const int used = int(min(long(p.max_blocks), (long(len) + mine + p.block_size - 1) / p.block_size));
+    const int lo = blockIdx.x * p.per_cta, hi = min(lo + p.per_cta, p.max_blocks);
+    int* to = p.block_tables + size_t(b) * p.max_blocks;
+    if (p.vectors) {                                                   // rows on 16-byte boundaries: four entries at a time, four times
+      for (int i0 = lo + 4 * tid; i0 < hi; i0 += 16 * kThreads) {
+        int4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int i = i0 + k * 4 * kThreads;
+          v[k] = i < min(used, hi) ? *reinterpret_cast<const int4*>(from + i) : make_int4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int i = i0 + k * 4 * kThreads;
+          if (i + 1 >= used) v[k].y = 0;
+          if (i + 2 >= used) v[k].z = 0;
+          if (i + 3 >= used) v[k].w = 0;
+          if (i < hi) *reinterpret_cast<int4*>(to + i) = v[k];
+        }
+      }
+    } else {
+      for (int i = lo + tid; i < hi; i += kThreads) to[i] = i < used ? from[i] : 0;
+    }
+    return;
+  }
+  const int part = blockIdx.x - p.table_parts, lo = part * p.per_cta;
+  if (part > 0 && lo >= mine && b < p.B) return;
   long ahead = 0;
   for (int i = tid; i < b; i += kThreads) ahead += rows_of(i);
   const long sum = block_sum(ahead, s_sum);
   const int start = int(min(sum, long(p.n_rows)));
-  if (blockIdx.x == 0 && tid == 0) p.q_cu[b] = start;
+  if (part == 0 && tid == 0) p.q_cu[b] = start;
   if (b == p.B) {
-    for (long t = start + long(blockIdx.x) * kThreads + tid; t < p.n_rows; t += long(gridDim.x) * kThreads) {
+    for (long t = start + long(part) * kThreads + tid; t < p.n_rows; t += long(gridDim.x - p.table_parts) * kThreads) {
       p.positions[t] = 0;
       p.slots[t] = int(t % p.block_size);
       p.token_seq[t] = -1;
@@ -74,8 +96,7 @@ __global__ void __launch_bounds__(kThreads) step_rows_kernel(const RowsParams p)
     return;
   }
   const int n = min(mine, p.n_rows - start);
-  if (blockIdx.x == 0 && tid == 0) p.kv_lens[b] = len + n;
-  const int* from = p.tables + size_t(max(src, 0)) * p.table_ld;
+  if (part == 0 && tid == 0) p.kv_lens[b] = len + n;
   auto slot_of = [&](long at, int t) {
     const long blk = at / p.block_size;
     return blk < p.table_ld ? from[blk] * p.block_size + int(at % p.block_size) : t % p.block_size;   // past the table: the reserved block
@@ -232,10 +253,14 @@ XL_API int xl_step_rows(const void* tables, const void* lens, const void* seqs, 
   p.tree = static_cast<unsigned long long*>(tree);
   p.pool = pool; p.table_ld = table_ld; p.B = B; p.n_rows = n_rows; p.max_q = max_q; p.max_blocks = max_blocks;
   p.block_size = block_size; p.words = parents ? words : 0;
+  p.vectors = max_blocks % 4 == 0 && table_ld % 4 == 0 && (reinterpret_cast<uintptr_t>(tables) | reinterpret_cast<uintptr_t>(block_tables)) % 16 == 0;
+  // table entries of a CTA: as many as keep all CTAs resident, from two rounds of scalars to four of vectors
+  const long resident = 8l * xl_host::sm_count();
   p.per_cta = 2048;
-  // parts of a table, and of a sequence's rows
-  const int parts = (max(max_blocks, parents ? 0 : min(max_q, n_rows)) + p.per_cta - 1) / p.per_cta;
-  step_rows_kernel<<<dim3(max(parts, 1), B + 1), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  while (p.per_cta < 16384 && long(max_blocks + p.per_cta - 1) / p.per_cta * B > resident) p.per_cta *= 2;
+  p.table_parts = (max_blocks + p.per_cta - 1) / p.per_cta;
+  const int row_parts = parents ? 1 : (min(max_q, n_rows) + p.per_cta - 1) / p.per_cta;
+  step_rows_kernel<<<dim3(p.table_parts + max(row_parts, 1), B + 1), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
   return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }
 
