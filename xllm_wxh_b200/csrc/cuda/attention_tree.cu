@@ -1,17 +1,15 @@
 // Attention of a tree of drafted tokens over a paged cache: o_i = sum_j softmax_j(scale q_i . k_j) v_j over the cached keys ahead of the
 // tree and over those of the sequence's own rows whose bit is set in row i's words (its ancestors and itself).
 //
-// The fp32-pipe kernel serves every type and size: one warp per (row, query head), 32 keys at a time, one key per lane for the scores, then
-// one slice of the value columns per lane for the weighted sum, with a running maximum and sum.
+// Both kernels make one pass over the keys with a running maximum and sum.
 #include <atomic>
+#include <type_traits>
 
 #include "attention_tc.cuh"
 #include "vec8.cuh"
 
 namespace xl_at {
 using namespace xl;
-
-constexpr int kMaxCols = 16;      // value columns per lane: up to 512 columns
 
 struct Params {
   const void* q;                  // [T, n_q, D], pitches in elements
@@ -26,76 +24,287 @@ struct Params {
   int window;                     // > 0: keys at positions above (row's position - window)
 };
 
-template <typename T>
-__global__ void __launch_bounds__(128) attention_tree_simt_kernel(const Params p) {
-  extern __shared__ float s_q[];                 // one query vector per warp
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long item = blockIdx.x * 4l + warp;
-  if (item >= long(p.T) * p.n_q) return;
-  const int t = int(item / p.n_q), h = int(item % p.n_q);
-  T* out = static_cast<T*>(p.out) + (size_t(t) * p.n_q + h) * p.D;
-  const int seq = p.token_seq[t];
-  const int start = seq >= 0 && seq < p.B ? p.q_cu[seq] : 0, n = seq >= 0 && seq < p.B ? p.q_cu[seq + 1] - start : 0;
-  if (t < start || t >= start + n) {             // a row of no sequence
-    for (int c = lane; c < p.D; c += 32) from_f32(out + c, 0.f);
-    return;
+constexpr int BKV = 64;          // keys of a tile of the tensor-core kernel; the first tile starts at a multiple
+struct Seq {
+  int q_start, n, kv_len, base, kv_begin, row_tiles, key_tiles;
+};
+__device__ __forceinline__ Seq load_seq(const Params& p, int s, int per_item) {
+  Seq q;
+  q.q_start = p.q_cu[s];
+  q.n = min(p.q_cu[s + 1], p.T) - q.q_start;
+  q.kv_len = int(min(long(p.kv_lens[s]), long(p.max_blocks) * p.block_size));
+  q.base = max(q.kv_len - q.n, 0);
+  q.kv_begin = p.window > 0 ? max(0, q.base - p.window + 1) / BKV * BKV : 0;
+  q.row_tiles = q.n > 0 && q.kv_len > 0 ? (q.n + per_item - 1) / per_item : 0;
+  q.key_tiles = (q.kv_len - q.kv_begin + BKV - 1) / BKV;
+  return q;
+}
+
+// keys of the tile at kv0 that row t (at position pos) sees
+__device__ __forceinline__ uint64_t seen_keys(const Params& p, const Seq& q, int t, int pos, int kv0) {
+  const int c = q.base - kv0;
+  uint64_t see = c >= 64 ? ~0ull : c > 0 ? (1ull << c) - 1 : 0;
+  if (p.window > 0) {
+    const int lo = pos - p.window + 1 - kv0;
+    see = lo >= 64 ? 0 : lo > 0 ? see >> lo << lo : see;
   }
-  const int kv_len = p.kv_lens[seq], base = max(kv_len - n, 0), pos = p.positions[t];
-  const int kvh = h / (p.n_q / p.n_kv);
+  if (c < 64) {
+    const unsigned long long* words = p.tree + size_t(t) * p.words;
+    uint64_t bits;
+    if (c >= 0) {
+      bits = words[0] << c;
+    } else {
+      const int i = (-c) >> 6, sh = (-c) & 63;
+      bits = i < p.words ? words[i] >> sh : 0;
+      if (sh && i + 1 < p.words) bits |= words[i + 1] << (64 - sh);
+    }
+    const int end = q.base + q.n - kv0;
+    if (end < 64) bits = end > 0 ? bits & ((1ull << end) - 1) : 0;
+    if (p.window > 0 && pos - p.window >= q.base)
+      for (uint64_t todo = bits; todo; todo &= todo - 1) {
+        const int k = __ffsll(todo) - 1;
+        if (p.positions[q.q_start + kv0 + k - q.base] <= pos - p.window) bits &= ~(1ull << k);
+      }
+    see |= bits;
+  }
+  return see;
+}
+
+// ---------------------------------------------------------------- fp32-pipe kernel
+// fp32, and bf16 of the sizes that the tensor-core kernel does not take.  One CTA = (sequence, 32 rows of a key head's query heads times
+// nodes, key head, part of the keys): 32 keys at a time go through shared memory as fp32, a thread computes 4 rows x 2 keys of the
+// scores and 4 rows x 4 NC columns of the sums, so that the multiply-adds bound it rather than shared memory; parts of the keys
+// keep the SMs busy when there are few rows, and are joined by a second kernel.
+constexpr int SR = 32, SK = 32, kSimtThreads = 128;
+template <int NC> struct SimtSmem {
+  static constexpr int DP = 64 * NC, PITCH = DP + 4;         // 16 rows apart lie in 16 banks
+  float q[SR][PITCH], k[SK][PITCH], v[SK][DP], p[SR][SK + 4];
+  long slot[SK];                                             // -1: behind the last key
+};
+
+template <typename T, int NC>
+__global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const Params p, int row_tiles, int splits, int part_keys, float* ws_o,
+                                                                           float2* ws_ml) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  using S = SimtSmem<NC>;
+  S& sm = *reinterpret_cast<S*>(smem);
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15, D = p.D;
+  const int seq = blockIdx.x / row_tiles, row0 = (blockIdx.x - seq * row_tiles) * SR, kvh = blockIdx.y, G = p.n_q / p.n_kv;
+  const Seq q = load_seq(p, seq, 1);
+  if (splits == 1 && kvh == 0) {                             // rows of no sequence
+    for (long i = max(p.q_cu[p.B], 0) + long(blockIdx.x); i < p.T; i += gridDim.x)
+      for (int c = tid; c < p.n_q * D; c += kSimtThreads) from_f32(static_cast<T*>(p.out) + i * p.n_q * D + c, 0.f);
+  }
+  if (row0 >= q.n * G || q.kv_len <= 0) return;
+  const int first = q.kv_begin + int(blockIdx.z) * part_keys, last = int(blockIdx.z) == splits - 1 ? q.kv_len : min(q.kv_len, first + part_keys);
+  if (first >= last) return;
+  // rows of this thread: 4 ty + i
+  int t[4], pos[4];
+  bool valid[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int node = (row0 + 4 * ty + i) / G;
+    valid[i] = node < q.n;
+    t[i] = q.q_start + (valid[i] ? node : 0);
+    pos[i] = p.window > 0 ? p.positions[t[i]] : 0;
+  }
+  const bool vectors = D % 8 == 0 && (reinterpret_cast<uintptr_t>(p.k_cache) | reinterpret_cast<uintptr_t>(p.v_cache)) % 16 == 0;
+  const float scale = p.scale * 1.4426950408889634f;         // scores in the log2 domain
+  for (int i = tid; i < SR * S::DP; i += kSimtThreads) {
+    const int r = i / S::DP, c = i - r * S::DP, node = (row0 + r) / G, h = kvh * G + (row0 + r) % G;
+    sm.q[r][c] = node < q.n && c < D ? to_f32(static_cast<const T*>(p.q)[(q.q_start + node) * p.q_row + h * p.q_head + c]) * scale : 0.f;
+  }
+  for (int i = tid; i < SK * S::DP; i += kSimtThreads) {     // columns past D stay zero
+    sm.k[i / S::DP][i % S::DP] = 0.f;
+    sm.v[i / S::DP][i % S::DP] = 0.f;
+  }
   const int* bt = p.block_tables + size_t(seq) * p.max_blocks;
-  const unsigned long long* words = p.tree + size_t(t) * p.words;
-  const T* qrow = static_cast<const T*>(p.q) + t * p.q_row + h * p.q_head;
-  float* q = s_q + warp * p.D;
-  for (int i = lane; i < p.D; i += 32) q[i] = to_f32(qrow[i]) * p.scale;
-  __syncwarp();
-  float m = -INFINITY, l = 0.f;
-  float acc[kMaxCols];
+  float m[4], l[4], o[4][4 * NC];
 #pragma unroll
-  for (int c = 0; c < kMaxCols; ++c) acc[c] = 0.f;
-  const int lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-  for (int first = min(lo, base) / 32 * 32; first < kv_len; first += 32) {
-    const int key = first + lane;
-    bool see = key >= lo && key < base;
-    if (key >= base && key < kv_len) {
-      const int node = key - base;
-      see = node < n && (node >> 6) < p.words && (words[node >> 6] >> (node & 63) & 1ull);
-      if (see && p.window > 0) see = p.positions[start + node] > pos - p.window;
+  for (int i = 0; i < 4; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4 * NC; ++c) o[i][c] = 0.f;
+  }
+  for (int kv0 = first; kv0 < last; kv0 += SK) {
+    __syncthreads();
+    if (tid < SK) {
+      const int key = kv0 + tid, blk = key / p.block_size;
+      long slot = key < last && blk < p.max_blocks ? long(bt[blk]) * p.block_size + key % p.block_size : -1;
+      sm.slot[tid] = slot < p.num_slots ? slot : -1;
     }
-    float s = -INFINITY;
-    long slot = 0;
-    if (see) {
-      const int blk = key / p.block_size;
-      slot = blk < p.max_blocks ? long(bt[blk]) * p.block_size + key % p.block_size : 0;
-      if (slot < 0 || slot >= p.num_slots) slot = 0;
-      const T* k = static_cast<const T*>(p.k_cache) + (size_t(slot) * p.n_kv + kvh) * p.D;
-      float d = 0.f;
-      for (int i = 0; i < p.D; ++i) d = fmaf(q[i], to_f32(k[i]), d);
-      s = d;
+    __syncthreads();
+    if (vectors) {
+      const int per = D / 8;
+      for (int i = tid; i < SK * per; i += kSimtThreads) {
+        const int j = i / per, c = (i - j * per) * 8;
+        float a[8] = {}, b[8] = {};
+        if (sm.slot[j] >= 0) {
+          const size_t at = (size_t(sm.slot[j]) * p.n_kv + kvh) * D + c;
+          load8(static_cast<const T*>(p.k_cache) + at, a);
+          load8(static_cast<const T*>(p.v_cache) + at, b);
+        }
+        store8(&sm.k[j][c], a);
+        store8(&sm.v[j][c], b);
+      }
+    } else {
+      for (int i = tid; i < SK * D; i += kSimtThreads) {
+        const int j = i / D, c = i - j * D;
+        const size_t at = (size_t(max(sm.slot[j], 0l)) * p.n_kv + kvh) * D + c;
+        sm.k[j][c] = sm.slot[j] >= 0 ? to_f32(static_cast<const T*>(p.k_cache)[at]) : 0.f;
+        sm.v[j][c] = sm.slot[j] >= 0 ? to_f32(static_cast<const T*>(p.v_cache)[at]) : 0.f;
+      }
     }
-    unsigned todo = __ballot_sync(0xffffffffu, see);
-    if (!todo) continue;
-    const float m_new = fmaxf(m, warp_max(s));
-    const float ref = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = m == -INFINITY ? 0.f : expf(m - ref);
-    const float w = see ? expf(s - ref) : 0.f;
-    l = l * alpha + warp_sum(w);
-    m = m_new;
+    __syncthreads();
+    // scores of rows 4 ty + i and keys tx, tx + 16
+    float s[4][2] = {};
+#pragma unroll 4
+    for (int c = 0; c < S::DP; c += 4) {
+      const float4 k0 = *reinterpret_cast<const float4*>(&sm.k[tx][c]), k1 = *reinterpret_cast<const float4*>(&sm.k[tx + 16][c]);
 #pragma unroll
-    for (int c = 0; c < kMaxCols; ++c) acc[c] *= alpha;
-    for (; todo; todo &= todo - 1) {
-      const int j = __ffs(todo) - 1;
-      const float wj = __shfl_sync(0xffffffffu, w, j);
-      const long sj = __shfl_sync(0xffffffffu, slot, j);
-      const T* v = static_cast<const T*>(p.v_cache) + (size_t(sj) * p.n_kv + kvh) * p.D;
+      for (int i = 0; i < 4; ++i) {
+        const float4 w = *reinterpret_cast<const float4*>(&sm.q[4 * ty + i][c]);
+        s[i][0] = fmaf(w.x, k0.x, fmaf(w.y, k0.y, fmaf(w.z, k0.z, fmaf(w.w, k0.w, s[i][0]))));
+        s[i][1] = fmaf(w.x, k1.x, fmaf(w.y, k1.y, fmaf(w.z, k1.z, fmaf(w.w, k1.w, s[i][1]))));
+      }
+    }
+    const bool partly = kv0 + SK > min(q.base, last) || (p.window > 0 && kv0 < q.base + q.n - p.window);
+    uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
+    if (partly) {
+      const uint32_t there = last - kv0 >= SK ? ~0u : (1u << (last - kv0)) - 1;
 #pragma unroll
-      for (int c = 0; c < kMaxCols; ++c)
-        if (c * 32 + lane < p.D) acc[c] = fmaf(wj, to_f32(v[c * 32 + lane]), acc[c]);
+      for (int i = 0; i < 4; ++i) {
+        see[i] = valid[i] ? uint32_t(seen_keys(p, q, t[i], pos[i], kv0)) & there : 0u;
+        if (!(see[i] >> tx & 1u)) s[i][0] = -INFINITY;
+        if (!(see[i] >> (tx + 16) & 1u)) s[i][1] = -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float mx = fmaxf(s[i][0], s[i][1]);
+#pragma unroll
+      for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+      const float m_new = fmaxf(m[i], mx), ref = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = m[i] == -INFINITY ? 1.f : fast_exp2(m[i] - ref);
+      const float e0 = see[i] >> tx & 1u ? fast_exp2(s[i][0] - ref) : 0.f, e1 = see[i] >> (tx + 16) & 1u ? fast_exp2(s[i][1] - ref) : 0.f;
+      float sum = e0 + e1;
+#pragma unroll
+      for (int off = 8; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      m[i] = m_new;
+      l[i] = l[i] * alpha + sum;
+#pragma unroll
+      for (int c = 0; c < 4 * NC; ++c) o[i][c] *= alpha;
+      sm.p[4 * ty + i][tx] = e0;
+      sm.p[4 * ty + i][tx + 16] = e1;
+    }
+    __syncwarp();                                            // a half-warp's weights are its own
+    auto sums = [&](auto masked) {
+#pragma unroll 2
+      for (int j = 0; j < SK; j += 4) {
+        float w[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(w[i]) = *reinterpret_cast<const float4*>(&sm.p[4 * ty + i][j]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            const float4 v = *reinterpret_cast<const float4*>(&sm.v[j + k][64 * c + 4 * tx]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (decltype(masked)::value && !(see[i] >> (j + k) & 1u)) continue;       // whatever stands there
+              o[i][4 * c] = fmaf(w[i][k], v.x, o[i][4 * c]);
+              o[i][4 * c + 1] = fmaf(w[i][k], v.y, o[i][4 * c + 1]);
+              o[i][4 * c + 2] = fmaf(w[i][k], v.z, o[i][4 * c + 2]);
+              o[i][4 * c + 3] = fmaf(w[i][k], v.w, o[i][4 * c + 3]);
+            }
+          }
+      }
+    };
+    if (partly) sums(std::true_type{});
+    else sums(std::false_type{});
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (!valid[i]) continue;
+    const size_t row = size_t(t[i]) * p.n_q + kvh * G + (row0 + 4 * ty + i) % G;
+    if (splits > 1) {
+      const size_t at = size_t(blockIdx.z) * p.T * p.n_q + row;
+      if (tx == 0) ws_ml[at] = make_float2(m[i], l[i]);
+#pragma unroll
+      for (int c = 0; c < 4 * NC; ++c) {
+        const int col = 64 * (c >> 2) + 4 * tx + (c & 3);
+        if (col < D) ws_o[at * D + col] = o[i][c];
+      }
+    } else {
+      const float inv = l[i] != 0.f ? 1.f / l[i] : 0.f;      // a row that sees nothing: zeros
+#pragma unroll
+      for (int c = 0; c < 4 * NC; ++c) {
+        const int col = 64 * (c >> 2) + 4 * tx + (c & 3);
+        if (col < D) from_f32(static_cast<T*>(p.out) + row * D + col, o[i][c] * inv);
+      }
     }
   }
-  const float inv = l != 0.f ? 1.f / l : 0.f;   // a row that sees nothing: zeros
-#pragma unroll
-  for (int c = 0; c < kMaxCols; ++c)
-    if (c * 32 + lane < p.D) from_f32(out + c * 32 + lane, acc[c] * inv);
+}
+
+// One warp per (row, query head): joins the parts of its keys, and clears rows of no sequence.
+template <typename T>
+__global__ void __launch_bounds__(128) attention_tree_join_kernel(const Params p, int splits, int part_keys, const float* ws_o, const float2* ws_ml) {
+  const long row = blockIdx.x * 4l + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= long(p.T) * p.n_q) return;
+  const int t = int(row / p.n_q), seq = p.token_seq[t];
+  T* out = static_cast<T*>(p.out) + size_t(row) * p.D;
+  int parts = 0;
+  if (seq >= 0 && seq < p.B) {
+    const Seq q = load_seq(p, seq, 1);
+    if (t >= q.q_start && t < q.q_start + q.n) parts = min(splits, (q.kv_len - q.kv_begin + part_keys - 1) / part_keys);
+  }
+  float m = -INFINITY, l = 0.f;
+  for (int k = 0; k < parts; ++k) m = fmaxf(m, ws_ml[size_t(k) * p.T * p.n_q + row].x);
+  const float ref = m == -INFINITY ? 0.f : m;
+  for (int k = 0; k < parts; ++k) {
+    const float2 ml = ws_ml[size_t(k) * p.T * p.n_q + row];
+    if (ml.x != -INFINITY || ml.y != 0.f) l += fast_exp2(ml.x == -INFINITY ? 0.f : ml.x - ref) * ml.y;
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  for (int c = lane; c < p.D; c += 32) {
+    float o = 0.f;
+    for (int k = 0; k < parts; ++k) {
+      const size_t at = size_t(k) * p.T * p.n_q + row;
+      const float2 ml = ws_ml[at];
+      if (ml.x != -INFINITY || ml.y != 0.f) o = fmaf(fast_exp2(ml.x == -INFINITY ? 0.f : ml.x - ref), ws_o[at * p.D + c], o);
+    }
+    from_f32(out + c, parts > 0 ? o * inv : 0.f);
+  }
+}
+
+template <typename T, int NC>
+int launch_simt(const Params& p, int row_tiles, int splits, int part_keys, float* ws, cudaStream_t s) {
+  auto* kernel = attention_tree_simt_kernel<T, NC>;
+  static std::atomic<bool> ready[64];                        // per device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SimtSmem<NC>))) != cudaSuccess) return -1;
+    ready[dev].store(true, std::memory_order_release);
+  }
+  float2* ml = reinterpret_cast<float2*>(ws);
+  float* o = ws + 2l * splits * p.T * p.n_q;
+  if (p.B > 0) {
+    kernel<<<dim3(p.B * row_tiles, p.n_kv, splits), kSimtThreads, sizeof(SimtSmem<NC>), s>>>(p, row_tiles, splits, part_keys, o, ml);
+    if (cudaGetLastError() != cudaSuccess) return -1;
+  }
+  if (p.B > 0 && splits == 1) return 0;
+  attention_tree_join_kernel<T><<<unsigned((long(p.T) * p.n_q + 3) / 4), 128, 0, s>>>(p, splits, part_keys, o, ml);
+  return cudaGetLastError() == cudaSuccess ? 0 : -1;
+}
+template <typename T>
+int launch_simt(const Params& p, int row_tiles, int splits, int part_keys, float* ws, cudaStream_t s) {
+  if (p.D <= 64) return launch_simt<T, 1>(p, row_tiles, splits, part_keys, ws, s);
+  if (p.D <= 128) return launch_simt<T, 2>(p, row_tiles, splits, part_keys, ws, s);
+  if (p.D <= 256) return launch_simt<T, 4>(p, row_tiles, splits, part_keys, ws, s);
+  return launch_simt<T, 8>(p, row_tiles, splits, part_keys, ws, s);
 }
 
 // ---------------------------------------------------------------- tensor-core kernel
@@ -120,16 +329,13 @@ __global__ void __launch_bounds__(128) attention_tree_simt_kernel(const Params p
 // border look at them.  There, values behind the last row are cleared, and values that are not finite are taken out of the tile and
 // added to the rows that do see them, so that whatever stands in a masked place reaches no other row.
 // Every wait is bounded; on expiry the kernel records a status code and leaves.
-constexpr int BQ = 128, BKV = 64;
+constexpr int BQ = 128;
 constexpr int kTcThreads = 320;
 constexpr int Q_SLAB = BQ * 128, KV_SLAB = BKV * 128;
 constexpr int kMaxUnits = 20, kPieces = 8, kItemCost = 3;
 
-struct Seq {
-  int q_start, n, kv_len, base, kv_begin, row_tiles, key_tiles;
-  __device__ __forceinline__ int item() const { return key_tiles + kItemCost; }
-  __device__ __forceinline__ long work(int n_kv) const { return long(row_tiles) * n_kv * item(); }
-};
+__device__ __forceinline__ int item_work(const Seq& q) { return q.key_tiles + kItemCost; }
+__device__ __forceinline__ long seq_work(const Seq& q, int n_kv) { return long(q.row_tiles) * n_kv * item_work(q); }
 struct Piece {
   Seq q;
   int seq, head, node0, j0, nt;            // node0: first node of the piece's rows; its key tiles j0 .. j0 + nt - 1 (0: no more pieces)
@@ -179,51 +385,9 @@ struct TcParams {
 };
 enum { DESC_MERGE, DESC_FIRST, DESC_SLOT, DESC_START, DESC_NODES, DESC_HEAD };   // of the item that ends in a CTA's first piece
 
-__device__ __forceinline__ Seq load_seq(const Params& p, int s, int per_item) {
-  Seq q;
-  q.q_start = p.q_cu[s];
-  q.n = min(p.q_cu[s + 1], p.T) - q.q_start;
-  q.kv_len = int(min(long(p.kv_lens[s]), long(p.max_blocks) * p.block_size));
-  q.base = max(q.kv_len - q.n, 0);
-  q.kv_begin = p.window > 0 ? max(0, q.base - p.window + 1) / BKV * BKV : 0;
-  q.row_tiles = q.n > 0 && q.kv_len > 0 ? (q.n + per_item - 1) / per_item : 0;
-  q.key_tiles = (q.kv_len - q.kv_begin + BKV - 1) / BKV;
-  return q;
-}
-
 // S of a tile is issued `lag` tiles ahead of P V: by one tile of the same group.  Unit (within its piece) of the keys and values of tile j.
 __device__ __forceinline__ int k_unit(int j, int lag) { return j < lag ? j : 2 * j - lag; }
 __device__ __forceinline__ int v_unit(int j, int lag, int nt) { return j + lag < nt ? 2 * j + lag + 1 : nt + j; }
-
-// keys of the tile at kv0 that row t (at position pos) sees
-__device__ __forceinline__ uint64_t seen_keys(const Params& p, const Seq& q, int t, int pos, int kv0) {
-  const int c = q.base - kv0;
-  uint64_t see = c >= 64 ? ~0ull : c > 0 ? (1ull << c) - 1 : 0;
-  if (p.window > 0) {
-    const int lo = pos - p.window + 1 - kv0;
-    see = lo >= 64 ? 0 : lo > 0 ? see >> lo << lo : see;
-  }
-  if (c < 64) {
-    const unsigned long long* words = p.tree + size_t(t) * p.words;
-    uint64_t bits;
-    if (c >= 0) {
-      bits = words[0] << c;
-    } else {
-      const int i = (-c) >> 6, sh = (-c) & 63;
-      bits = i < p.words ? words[i] >> sh : 0;
-      if (sh && i + 1 < p.words) bits |= words[i + 1] << (64 - sh);
-    }
-    const int end = q.base + q.n - kv0;
-    if (end < 64) bits = end > 0 ? bits & ((1ull << end) - 1) : 0;
-    if (p.window > 0 && pos - p.window >= q.base)
-      for (uint64_t todo = bits; todo; todo &= todo - 1) {
-        const int k = __ffsll(todo) - 1;
-        if (p.positions[q.q_start + kv0 + k - q.base] <= pos - p.window) bits &= ~(1ull << k);
-      }
-    see |= bits;
-  }
-  return see;
-}
 
 __device__ __forceinline__ bool not_finite(uint32_t pair) {
   return (pair & 0x7F800000u) == 0x7F800000u || (pair & 0x7F80u) == 0x7F80u;
@@ -276,7 +440,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
   const int share = (a.B + kTcThreads - 1) / kTcThreads;
   const int s0 = min(tid * share, a.B), s1 = min(s0 + share, a.B);
   long mine = 0;
-  for (int s = s0; s < s1; ++s) mine += load_seq(a, s, per_item).work(a.n_kv);
+  for (int s = s0; s < s1; ++s) mine += seq_work(load_seq(a, s, per_item), a.n_kv);
   if (warp == 0 && lane < 3) prefetch_tmap(lane == 0 ? &tmQ : lane == 1 ? &tmK : &tmV);
   if (tid == 64) {
     for (int u = 0; u < U; ++u) {
@@ -324,7 +488,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
   if (busy && incl - mine <= w0 && w0 < incl) {
     long at = incl - mine;
     for (int s = s0; s < s1; ++s) {
-      const long n = load_seq(a, s, per_item).work(a.n_kv);
+      const long n = seq_work(load_seq(a, s, per_item), a.n_kv);
       if (w0 < at + n) {
         bars->seq = s;
         bars->seq_work = at;
@@ -348,8 +512,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
     if (busy) {
       x.seq = bars->seq;
       x.q = load_seq(a, x.seq, per_item);
-      const int item = int((w0 - bars->seq_work) / x.q.item());
-      w = bars->seq_work + long(item) * x.q.item();
+      const int item = int((w0 - bars->seq_work) / item_work(x.q));
+      w = bars->seq_work + long(item) * item_work(x.q);
       x.head = item / x.q.row_tiles;
       row = item - x.head * x.q.row_tiles;
     }
@@ -426,7 +590,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
           held0 = slot;
         }
       }
-      w += x.q.item();
+      w += item_work(x.q);
       if (++row == x.q.row_tiles) {
         row = 0;
         if (++x.head == a.n_kv) {
@@ -830,20 +994,44 @@ static bool tc_serves(const void* q, const void* k, const void* v, int block_siz
          q_row % q_head == 0 && (reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 == 0;
 }
 
-// Bytes of the workspace for `ctas` CTAs (0: the tensor-core kernel does not serve these sizes).  max_q: rows of a sequence at most.
-XL_API long xl_attention_tree_workspace(int block_size, int n_q, int n_kv, int D, int max_q, int ctas) {
-  if (!tc_serves(nullptr, nullptr, nullptr, block_size, n_q, n_kv, D, 8, 8, 1.f, 0)) return 0;
-  const long rows = long(max_q) * (n_q / n_kv) > xl_at::BQ ? 256 : 128, DV = (D + 63) / 64 * 64;
-  return 2l * ctas * rows * (DV * 4 + 8) + 32l * ctas;
+// How the fp32-pipe kernel is launched: row tiles of a sequence, parts of the keys, keys of a part.  max_q, max_kv: bounds of a sequence's rows
+// and keys.
+struct SimtPlan { int row_tiles, splits, part_keys; };
+static SimtPlan simt_plan(int B, int n_q, int n_kv, int max_q, int max_kv, int sms) {
+  SimtPlan s{};
+  s.row_tiles = max(1, int((long(max_q) * (n_q / n_kv) + xl_at::SR - 1) / xl_at::SR));
+  const long units = long(s.row_tiles) * n_kv * max(B, 1);
+  // parts of 64 keys at least, as many as give an SM four CTAs
+  s.splits = int(max(1l, min(min(long(max_kv + 63) / 64, 64l), 4l * sms / units)));
+  s.part_keys = (max(max_kv, 1) + s.splits - 1) / s.splits;
+  s.part_keys = (s.part_keys + 63) / 64 * 64;
+  s.splits = (max(max_kv, 1) + s.part_keys - 1) / s.part_keys;
+  return s;
+}
+
+// Bytes of the workspace.  ctas: SMs that the tensor-core kernel may take; max_q, max_kv: bounds of a sequence's rows and keys.  *tc: whether
+// that kernel serves these sizes (rows on 16-byte boundaries and a positive scale given).
+XL_API long xl_attention_tree_workspace(int T, int B, int block_size, int n_q, int n_kv, int D, int f32, int max_q, int max_kv, int ctas, int sms,
+                                        int* tc) {
+  *tc = tc_serves(nullptr, nullptr, nullptr, block_size, n_q, n_kv, D, 8, 8, 1.f, f32);
+  if (*tc) {
+    const long rows = long(max_q) * (n_q / n_kv) > xl_at::BQ ? 256 : 128, DV = (D + 63) / 64 * 64;
+    return 2l * ctas * rows * (DV * 4 + 8) + 32l * ctas;
+  }
+  const SimtPlan s = simt_plan(B, n_q, n_kv, max_q, max_kv, sms);
+  return s.splits > 1 ? long(s.splits) * T * n_q * (D + 2) * 4 : 0;
 }
 
 XL_API int xl_attention_tree(const void* q, const void* k_cache, const void* v_cache, void* out, const void* q_cu, const void* kv_lens,
                              const void* block_tables, const void* token_seq, const void* positions, const void* tree, int T, int B,
                              int max_blocks, int block_size, int num_blocks, int n_q, int n_kv, int D, int words, long q_row, long q_head,
-                             float scale, int window, int f32, int max_q, int ctas, void* workspace, long workspace_bytes, void* stream) {
+                             float scale, int window, int f32, int max_q, int max_kv, int ctas, int sms, int tc, void* workspace, long workspace_bytes,
+                             void* stream) {
   using namespace xl_at;
-  if (T < 0 || B < 0 || n_kv < 1 || n_q % n_kv || D < 1 || D > 32 * kMaxCols || words < 1 || block_size < 1 || max_blocks < 1) return -2;
+  if (T < 0 || B < 0 || n_kv < 1 || n_q % n_kv || D < 1 || D > 512 || words < 1 || block_size < 1 || max_blocks < 1) return -2;
   if (T == 0) return 0;
+  int served = 0;
+  if (workspace_bytes < xl_attention_tree_workspace(T, B, block_size, n_q, n_kv, D, f32 || !tc, max_q, max_kv, ctas, sms, &served)) return -2;
   Params p{};
   p.q = q; p.k_cache = k_cache; p.v_cache = v_cache; p.out = out;
   p.q_cu = static_cast<const int*>(q_cu);
@@ -857,9 +1045,10 @@ XL_API int xl_attention_tree(const void* q, const void* k_cache, const void* v_c
   p.num_slots = long(num_blocks) * block_size;
   p.scale = scale; p.window = window;
   auto s = static_cast<cudaStream_t>(stream);
-  if (workspace && B > 0 && tc_serves(q, k_cache, v_cache, block_size, n_q, n_kv, D, q_row, q_head, scale, f32)) {
+  if (tc) {
+    if (B < 1 || !workspace || !tc_serves(q, k_cache, v_cache, block_size, n_q, n_kv, D, q_row, q_head, scale, f32)) return -2;
     const bool pair = long(max_q) * (n_q / n_kv) > BQ;
-    if (ctas < 1 || workspace_bytes < xl_attention_tree_workspace(block_size, n_q, n_kv, D, max_q, ctas)) return -2;
+    if (ctas < 1) return -2;
     TcParams t{};
     t.a = p;
     t.group = n_q / n_kv;
@@ -887,9 +1076,9 @@ XL_API int xl_attention_tree(const void* q, const void* k_cache, const void* v_c
     if (D <= 64) return pair ? launch_tc<1, 2>(t, mq, mk, mv, ctas, s) : launch_tc<1, 1>(t, mq, mk, mv, ctas, s);
     return pair ? launch_tc<2, 2>(t, mq, mk, mv, ctas, s) : launch_tc<2, 1>(t, mq, mk, mv, ctas, s);
   }
-  const long items = long(T) * n_q, grid = (items + 3) / 4;
-  if (grid > 0x7fffffffl) return -2;
-  if (f32) attention_tree_simt_kernel<float><<<unsigned(grid), 128, 4 * D * sizeof(float), s>>>(p);
-  else attention_tree_simt_kernel<__nv_bfloat16><<<unsigned(grid), 128, 4 * D * sizeof(float), s>>>(p);
-  return cudaGetLastError() == cudaSuccess ? 0 : -1;
+  const SimtPlan plan = simt_plan(B, n_q, n_kv, max_q, max_kv, sms);
+  if (long(B) * plan.row_tiles > 0x7fffffffl || n_kv > 65535 || long(T) * n_q > 0x7fffffffl) return -2;
+  auto* ws = static_cast<float*>(workspace);
+  return f32 ? launch_simt<float>(p, plan.row_tiles, plan.splits, plan.part_keys, ws, s)
+             : launch_simt<__nv_bfloat16>(p, plan.row_tiles, plan.splits, plan.part_keys, ws, s);
 }

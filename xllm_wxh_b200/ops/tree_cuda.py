@@ -13,7 +13,7 @@ _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
 _SIGNATURES = {
     "xl_step_rows": [_P] * 12 + [_I] * 8 + [_P],
     "xl_accept_tree": [_P] * 9 + [_I] * 5 + [_P] * 3 + [_I] * 2 + [_P],
-    "xl_attention_tree": [_P] * 10 + [_I] * 9 + [_L] * 2 + [_F] + [_I] * 4 + [_P, _L, _P],
+    "xl_attention_tree": [_P] * 10 + [_I] * 9 + [_L] * 2 + [_F] + [_I] * 7 + [_P, _L, _P],
     "xl_adjust_logits": [_P] + [_I] * 3 + [_L] + [_P] * 2 + [_I] * 3 + [_P, _L, _I] + [_P] * 10 + [_I, _P, _I, _I, _P, _P],
 }
 _entry = {}
@@ -47,10 +47,11 @@ def _sms(device: int) -> int:
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace(*sizes) -> int:
-    f = cuda_ops.lib().xl_attention_tree_workspace
+def _workspace(*sizes):
+    """(bytes, whether the tensor-core kernel serves these sizes)."""
+    f, tc = cuda_ops.lib().xl_attention_tree_workspace, _I(0)
     f.restype = _L
-    return f(*sizes)
+    return f(*sizes, ctypes.byref(tc)), bool(tc.value)
 
 
 def _ptr(t):
@@ -76,24 +77,21 @@ def tree_attention(q, k_cache, v_cache, inp, tree, scale, window) -> torch.Tenso
     dev = q.get_device()
     out = q.new_empty((T, Hq * D))
     block, Hkv = k_cache.shape[1], k_cache.shape[2]
-    f32, work, ctas, size = q.dtype == torch.float32, None, 0, 0
-    if not f32 and scale > 0:
-        # one CTA per SM, fewer where there are fewer key tiles (of 64 keys for up to 128 rows) than it takes to be worth one
-        tiles = (inp.max_kv // 64 + 1) * Hkv * (inp.n_seqs + T * (Hq // Hkv) // 128)
-        ctas = max(1, min(_sms(dev), tiles))
-        size = _workspace(block, Hq, Hkv, D, inp.max_q, ctas)
-    if size:
-        if q.stride(2) != 1 or q.stride(1) % 8 or q.stride(0) % max(8, q.stride(1)) or q.data_ptr() % 16:
-            q = q.contiguous()
-        work = q.new_empty(size, dtype=torch.uint8)
-    elif q.stride(2) != 1:
+    f32, B, max_q, max_kv, sms = q.dtype is torch.float32, inp.n_seqs, inp.max_q, inp.max_kv, _sms(dev)
+    # one CTA per SM, fewer where there are fewer key tiles (of 64 keys for up to 128 rows)
+    ctas = max(1, min(sms, (max_kv // 64 + 1) * Hkv * (B + T * (Hq // Hkv) // 128)))
+    # no tensor-core kernel: for scores that do not grow with the product, nor where the caches lie off 16-byte boundaries
+    plain = f32 or scale <= 0 or B == 0 or (k_cache.data_ptr() | v_cache.data_ptr()) % 16 != 0
+    size, tc = _workspace(T, B, block, Hq, Hkv, D, int(plain), max_q, max_kv, ctas, sms)
+    if q.stride(2) != 1 or (tc and (q.stride(1) < 1 or q.stride(0) < 1 or q.stride(1) % 8 or q.stride(0) % max(8, q.stride(1)) or q.data_ptr() % 16)):
         q = q.contiguous()
+    work = q.new_empty(size, dtype=torch.uint8) if size else None
     bt = inp.block_tables
     _launch(dev, "xl_attention_tree", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), inp.q_cu.data_ptr(),
-            inp.kv_lens.data_ptr(), bt.data_ptr(), inp.token_seq.data_ptr(), inp.positions.data_ptr(), tree.data_ptr(), T, inp.n_seqs, bt.shape[1],
-            block, k_cache.shape[0], Hq, Hkv, D, tree.shape[1], q.stride(0), q.stride(1), scale, window, int(f32), inp.max_q, ctas, _ptr(work), size)
-    if size:
-        cuda_ops.launch_count += 1                               # the join of pieces
+            inp.kv_lens.data_ptr(), bt.data_ptr(), inp.token_seq.data_ptr(), inp.positions.data_ptr(), tree.data_ptr(), T, B, bt.shape[1], block,
+            k_cache.shape[0], Hq, Hkv, D, tree.shape[1], q.stride(0), q.stride(1), scale, window, int(f32), max_q, max_kv, ctas, sms, int(tc),
+            _ptr(work), size)
+    cuda_ops.launch_count += T > 0 and (ctas > 1 or not tc)      # the join of pieces
     return out
 
 
