@@ -75,11 +75,11 @@ __device__ __forceinline__ uint64_t seen_keys(const Params& p, const Seq& q, int
 // nodes, key head, part of the keys): 32 keys at a time go through shared memory as fp32, a thread computes 4 rows x 2 keys of the
 // scores and 4 rows x 4 NC columns of the sums, so that the multiply-adds bound it rather than shared memory; parts of the keys
 // keep the SMs busy when there are few rows, and are joined by a second kernel.
-constexpr int SR = 32, SK = 32, kSimtThreads = 128;
+constexpr int SR = 32, SK = 32, kSimtThreads = 128, kMaxParts = 64;
 template <int NC> struct SimtSmem {
   static constexpr int DP = 64 * NC, PITCH = DP + 4;         // 16 rows apart lie in 16 banks
   float q[SR][PITCH], k[SK][PITCH], v[SK][DP], p[SR][SK + 4];
-  long slot[SK];                                             // -1: behind the last key
+  long slot[2][SK];                                          // of this tile and the next; -1: behind the last key
 };
 
 template <typename T, int NC>
@@ -110,13 +110,27 @@ __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const
   }
   const bool vectors = D % 8 == 0 && (reinterpret_cast<uintptr_t>(p.k_cache) | reinterpret_cast<uintptr_t>(p.v_cache)) % 16 == 0;
   const float scale = p.scale * 1.4426950408889634f;         // scores in the log2 domain
-  for (int i = tid; i < SR * S::DP; i += kSimtThreads) {
-    const int r = i / S::DP, c = i - r * S::DP, node = (row0 + r) / G, h = kvh * G + (row0 + r) % G;
-    sm.q[r][c] = node < q.n && c < D ? to_f32(static_cast<const T*>(p.q)[(q.q_start + node) * p.q_row + h * p.q_head + c]) * scale : 0.f;
+  if (D < S::DP) {                                           // columns past D stay zero
+    for (int i = tid; i < 32 * S::DP; i += kSimtThreads) {
+      const int r = i / S::DP, c = i % S::DP;
+      if (c >= D) sm.q[r][c] = sm.k[r][c] = sm.v[r][c] = 0.f;
+    }
   }
-  for (int i = tid; i < SK * S::DP; i += kSimtThreads) {     // columns past D stay zero
-    sm.k[i / S::DP][i % S::DP] = 0.f;
-    sm.v[i / S::DP][i % S::DP] = 0.f;
+  const bool q_vectors = D % 8 == 0 && reinterpret_cast<uintptr_t>(p.q) % 16 == 0 && (p.q_row | p.q_head) % 8 == 0;
+  const int q_step = q_vectors ? 8 : 1, q_per = D / q_step;
+#pragma unroll 2
+  for (int i = tid; i < SR * q_per; i += kSimtThreads) {
+    const int r = i / q_per, c = (i - r * q_per) * q_step, node = (row0 + r) / G, h = kvh * G + row0 + r - node * G;
+    const T* from = static_cast<const T*>(p.q) + (q.q_start + (node < q.n ? node : 0)) * p.q_row + h * p.q_head + c;
+    if (q_vectors) {
+      float f[8];
+      load8(from, f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = node < q.n ? f[e] * scale : 0.f;
+      store8(&sm.q[r][c], f);
+    } else {
+      sm.q[r][c] = node < q.n ? to_f32(*from) * scale : 0.f;
+    }
   }
   const int* bt = p.block_tables + size_t(seq) * p.max_blocks;
   float m[4], l[4], o[4][4 * NC];
@@ -127,39 +141,68 @@ __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const
 #pragma unroll
     for (int c = 0; c < 4 * NC; ++c) o[i][c] = 0.f;
   }
-  for (int kv0 = first; kv0 < last; kv0 += SK) {
-    __syncthreads();
-    if (tid < SK) {
-      const int key = kv0 + tid, blk = key / p.block_size;
-      long slot = key < last && blk < p.max_blocks ? long(bt[blk]) * p.block_size + key % p.block_size : -1;
-      sm.slot[tid] = slot < p.num_slots ? slot : -1;
+  auto find_slots = [&](int tile) {
+    const int key = first + tile * SK + tid;
+    if (tid >= SK) return;
+    const int blk = key / p.block_size;
+    const long slot = key < last && blk < p.max_blocks ? long(bt[blk]) * p.block_size + key % p.block_size : -1;
+    sm.slot[tile & 1][tid] = slot < p.num_slots ? slot : -1;
+  };
+  // Eight columns of a key and its values at a time.  Small heads: the next tile's wait in registers while this one is computed.
+  constexpr bool kAhead = NC <= 2;
+  constexpr int kItems = kAhead ? SK * S::DP / 8 / kSimtThreads : 1;
+  const int per = D / 8;
+  float ka[kItems][8], va[kItems][8];
+  auto fetch = [&](int tile, int i, float (&a)[8], float (&b)[8]) {
+    const int j = i / per, c = (i - j * per) * 8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a[e] = b[e] = 0.f;
+    if (j < SK && sm.slot[tile & 1][j] >= 0) {
+      const size_t at = (size_t(sm.slot[tile & 1][j]) * p.n_kv + kvh) * D + c;
+      load8(static_cast<const T*>(p.k_cache) + at, a);
+      load8(static_cast<const T*>(p.v_cache) + at, b);
     }
+  };
+  auto keep = [&](int i, const float (&a)[8], const float (&b)[8]) {
+    const int j = i / per, c = (i - j * per) * 8;
+    if (j >= SK) return;
+    store8(&sm.k[j][c], a);
+    store8(&sm.v[j][c], b);
+  };
+  find_slots(0);
+  find_slots(1);
+  __syncthreads();
+  if (kAhead && vectors)
+#pragma unroll
+    for (int n = 0; n < kItems; ++n) fetch(0, tid + n * kSimtThreads, ka[n], va[n]);
+  int tile = 0;
+  for (int kv0 = first; kv0 < last; kv0 += SK, ++tile) {
     __syncthreads();
-    if (vectors) {
-      const int per = D / 8;
+    if (kAhead && vectors) {
+#pragma unroll
+      for (int n = 0; n < kItems; ++n) keep(tid + n * kSimtThreads, ka[n], va[n]);
+    } else if (vectors) {
       for (int i = tid; i < SK * per; i += kSimtThreads) {
-        const int j = i / per, c = (i - j * per) * 8;
-        float a[8] = {}, b[8] = {};
-        if (sm.slot[j] >= 0) {
-          const size_t at = (size_t(sm.slot[j]) * p.n_kv + kvh) * D + c;
-          load8(static_cast<const T*>(p.k_cache) + at, a);
-          load8(static_cast<const T*>(p.v_cache) + at, b);
-        }
-        store8(&sm.k[j][c], a);
-        store8(&sm.v[j][c], b);
+        fetch(tile, i, ka[0], va[0]);
+        keep(i, ka[0], va[0]);
       }
     } else {
       for (int i = tid; i < SK * D; i += kSimtThreads) {
         const int j = i / D, c = i - j * D;
-        const size_t at = (size_t(max(sm.slot[j], 0l)) * p.n_kv + kvh) * D + c;
-        sm.k[j][c] = sm.slot[j] >= 0 ? to_f32(static_cast<const T*>(p.k_cache)[at]) : 0.f;
-        sm.v[j][c] = sm.slot[j] >= 0 ? to_f32(static_cast<const T*>(p.v_cache)[at]) : 0.f;
+        const long slot = sm.slot[tile & 1][j];
+        const size_t at = (size_t(max(slot, 0l)) * p.n_kv + kvh) * D + c;
+        sm.k[j][c] = slot >= 0 ? to_f32(static_cast<const T*>(p.k_cache)[at]) : 0.f;
+        sm.v[j][c] = slot >= 0 ? to_f32(static_cast<const T*>(p.v_cache)[at]) : 0.f;
       }
     }
     __syncthreads();
+    find_slots(tile + 2);                                    // (in the place of this tile's, which is loaded)
+    if (kAhead && vectors && kv0 + SK < last)
+#pragma unroll
+      for (int n = 0; n < kItems; ++n) fetch(tile + 1, tid + n * kSimtThreads, ka[n], va[n]);
     // scores of rows 4 ty + i and keys tx, tx + 16
     float s[4][2] = {};
-#pragma unroll 4
+#pragma unroll 8
     for (int c = 0; c < S::DP; c += 4) {
       const float4 k0 = *reinterpret_cast<const float4*>(&sm.k[tx][c]), k1 = *reinterpret_cast<const float4*>(&sm.k[tx + 16][c]);
 #pragma unroll
@@ -260,22 +303,39 @@ __global__ void __launch_bounds__(128) attention_tree_join_kernel(const Params p
     const Seq q = load_seq(p, seq, 1);
     if (t >= q.q_start && t < q.q_start + q.n) parts = min(splits, (q.kv_len - q.kv_begin + part_keys - 1) / part_keys);
   }
+  // a lane's share of the (at most kMaxParts) parts
+  const size_t pitch = size_t(p.T) * p.n_q;
+  float2 ml[kMaxParts / 32];
   float m = -INFINITY, l = 0.f;
-  for (int k = 0; k < parts; ++k) m = fmaxf(m, ws_ml[size_t(k) * p.T * p.n_q + row].x);
-  const float ref = m == -INFINITY ? 0.f : m;
-  for (int k = 0; k < parts; ++k) {
-    const float2 ml = ws_ml[size_t(k) * p.T * p.n_q + row];
-    if (ml.x != -INFINITY || ml.y != 0.f) l += fast_exp2(ml.x == -INFINITY ? 0.f : ml.x - ref) * ml.y;
+#pragma unroll
+  for (int i = 0; i < kMaxParts / 32; ++i) {
+    ml[i] = lane + 32 * i < parts ? ws_ml[(lane + 32 * i) * pitch + row] : make_float2(-INFINITY, 0.f);
+    m = fmaxf(m, ml[i].x);
   }
+  m = warp_max(m);
+#pragma unroll
+  for (int i = 0; i < kMaxParts / 32; ++i) {
+    // a part whose row saw nothing has no weight, unless its scores were not numbers
+    const float w = ml[i].x == -INFINITY ? (ml[i].y != 0.f ? 1.f : 0.f) : fast_exp2(ml[i].x - m);
+    l += w != 0.f ? w * ml[i].y : 0.f;
+    ml[i].x = w;
+  }
+  l = warp_sum(l);
   const float inv = l != 0.f ? 1.f / l : 0.f;
-  for (int c = lane; c < p.D; c += 32) {
+  for (int c = lane; c - lane < p.D; c += 32) {
     float o = 0.f;
+#pragma unroll 8
     for (int k = 0; k < parts; ++k) {
-      const size_t at = size_t(k) * p.T * p.n_q + row;
-      const float2 ml = ws_ml[at];
-      if (ml.x != -INFINITY || ml.y != 0.f) o = fmaf(fast_exp2(ml.x == -INFINITY ? 0.f : ml.x - ref), ws_o[at * p.D + c], o);
+      float w = __shfl_sync(0xffffffffu, ml[0].x, k & 31);
+#pragma unroll
+      for (int i = 1; i < kMaxParts / 32; ++i) {
+        const float v = __shfl_sync(0xffffffffu, ml[i].x, k & 31);
+        if (k >> 5 == i) w = v;
+      }
+      const float x = c < p.D ? ws_o[(k * pitch + row) * p.D + c] : 0.f;
+      if (w != 0.f) o = fmaf(w, x, o);
     }
-    from_f32(out + c, parts > 0 ? o * inv : 0.f);
+    if (c < p.D) from_f32(out + c, o * inv);
   }
 }
 
@@ -1001,8 +1061,8 @@ static SimtPlan simt_plan(int B, int n_q, int n_kv, int max_q, int max_kv, int s
   SimtPlan s{};
   s.row_tiles = max(1, int((long(max_q) * (n_q / n_kv) + xl_at::SR - 1) / xl_at::SR));
   const long units = long(s.row_tiles) * n_kv * max(B, 1);
-  // parts of 64 keys at least, as many as give an SM four CTAs
-  s.splits = int(max(1l, min(min(long(max_kv + 63) / 64, 64l), 4l * sms / units)));
+  // parts of 64 keys at least, as many as give an SM eight CTAs if all sequences were as long as the longest
+  s.splits = int(max(1l, min(min(long(max_kv + 63) / 64, long(xl_at::kMaxParts)), 8l * sms / units)));
   s.part_keys = (max(max_kv, 1) + s.splits - 1) / s.splits;
   s.part_keys = (s.part_keys + 63) / 64 * 64;
   s.splits = (max(max_kv, 1) + s.part_keys - 1) / s.part_keys;
