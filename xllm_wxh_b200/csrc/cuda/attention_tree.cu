@@ -372,30 +372,33 @@ int launch_simt(const Params& p, int row_tiles, int splits, int part_keys, float
 // 128 / G nodes of G heads each, so that a key is read once for all of them (two row tiles: for 256 rows).  Reading K and V bounds the
 // kernel up to about 256 rows; above, exponentials and products do.
 //
-//   work      : the key tiles (64 keys) of every item (sequence, key head, rows) one behind the other, each item with kItemCost tiles'
+//   work      : the key tiles (64 keys) of every item (rows, key head, sequence) one behind the other, each item with kItemCost tiles'
 //               worth of work ahead of it, cut into equal stretches, one per CTA (one CTA per SM): ragged lengths leave no SM idle.
-//               A stretch begins and ends anywhere; the at most two pieces of it that are not whole items leave fp32 partials (sums,
+//               Sequences run fastest, so that the CTAs of a sequence's further rows go through the same keys at the same time and
+//               find them in L2.  A stretch begins and ends anywhere; the at most two pieces of it that are not whole items leave fp32 partials (sums,
 //               maximum, denominator) that the merge kernel joins.
 //   warp 0    : TMA producer - says what the next piece is, fetches its query rows (box: 64 columns x G heads x nodes), then a ring of units
 //               in the order of use, each 64 tokens of K or of V through the block table;
-//   warp 1    : MMA issuer   - S = Q K^T (128 x 64 x D, fp32 in TMEM, two buffers a group), O += P V with P from TMEM;
-//   warps 2-5 and 6-9: two softmax groups, one row per thread: running maximum and sum in the log2 domain, P as bf16 over the
+//   warps 1, 2: MMA issuers  - each for one softmax group: S = Q K^T (128 x 64 x D, fp32 in TMEM, two buffers a group), O += P V with P
+//               from TMEM (one issuer's waits would leave the tensor pipe idle);
+//   warps 3-6 and 7-10: two softmax groups, one row per thread: running maximum and sum in the log2 domain, P as bf16 over the
 //               scores it comes from, O rescaled only when the maximum grew by more than 2^8.
 //               An item of two row tiles gives each group one; otherwise the groups take the key tiles in turn for the same rows, each
 //               with its own O, and join at the end of a piece: a single group could not keep up with memory.
-// Products run in the order of their issue, so S of a tile may overwrite P of the tile two before as soon as that one's P V is issued.
+// A warp's products run in the order of their issue, so S of a tile may overwrite P of the tile two before as soon as that one's P V is issued.
 //
 // Masks: keys ahead of the tree are seen by all rows (within the window), the tree's by the row's words; only tiles that hold either
 // border look at them.  There, values behind the last row are cleared, and values that are not finite are taken out of the tile and
 // added to the rows that do see them, so that whatever stands in a masked place reaches no other row.
 // Every wait is bounded; on expiry the kernel records a status code and leaves.
 constexpr int BQ = 128;
-constexpr int kTcThreads = 320;
+constexpr int kTcThreads = 352;
 constexpr int Q_SLAB = BQ * 128, KV_SLAB = BKV * 128;
 constexpr int kMaxUnits = 20, kPieces = 8, kItemCost = 3;
 
 __device__ __forceinline__ int item_work(const Seq& q) { return q.key_tiles + kItemCost; }
-__device__ __forceinline__ long seq_work(const Seq& q, int n_kv) { return long(q.row_tiles) * n_kv * item_work(q); }
+// of a key head's items of row tile `plane`
+__device__ __forceinline__ int plane_work(const Seq& q, int plane) { return q.row_tiles > plane ? item_work(q) : 0; }
 struct Piece {
   Seq q;
   int seq, head, node0, j0, nt;            // node0: first node of the piece's rows; its key tiles j0 .. j0 + nt - 1 (0: no more pieces)
@@ -416,9 +419,9 @@ struct TcBarriers {
   // would be a phase off
   uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];
   uint32_t tmem_base;
-  int seq;
+  int seq, plane, head, planes;                              // of the first item; row tiles of any sequence at most
   int any_bad[4][2];                                         // [piece & 3][group]
-  long seq_work, part[kTcThreads / 32];                      // work ahead of `seq`
+  long ahead, part[kTcThreads / 32];                         // work ahead of the first item
   uint32_t bad[4][2][16][2];                                 // [piece & 3][group][tile][key]: keys whose values are not all finite
   float2 ml[2][BQ];
   Piece piece[kPieces];
@@ -499,16 +502,22 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
   const int per_item = NQ * p.nodes;
   const int share = (a.B + kTcThreads - 1) / kTcThreads;
   const int s0 = min(tid * share, a.B), s1 = min(s0 + share, a.B);
-  long mine = 0;
-  for (int s = s0; s < s1; ++s) mine += seq_work(load_seq(a, s, per_item), a.n_kv);
+  long mine = 0;                                             // of the first row tiles
+  if (tid == 0) bars->planes = 0;
+  int most = 0;
+  for (int s = s0; s < s1; ++s) {
+    const Seq q = load_seq(a, s, per_item);
+    mine += plane_work(q, 0);
+    most = max(most, q.row_tiles);
+  }
   if (warp == 0 && lane < 3) prefetch_tmap(lane == 0 ? &tmQ : lane == 1 ? &tmK : &tmV);
   if (tid == 64) {
     for (int u = 0; u < U; ++u) {
       mbar_init(&bars->full[u], 1);
-      mbar_init(&bars->empty[u], 1);
+      mbar_init(&bars->empty[u], 2);
     }
     mbar_init(&bars->q_full, 1);
-    mbar_init(&bars->q_empty, 1);
+    mbar_init(&bars->q_empty, 2);
     for (int i = 0; i < kPieces; ++i) mbar_init(&bars->info[i], 1);
     for (int g = 0; g < 2; ++g) {
       for (int b = 0; b < 2; ++b) {
@@ -525,36 +534,75 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
     tmem_alloc(&bars->tmem_base, 512);
     tmem_relinquish();
   }
-  long incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) bars->part[warp] = incl;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  long total = 0;
+  // sums over the sequences up to and with this thread's, and over all
+  auto scan = [&](long v, long& all) {
+    long incl = v;
 #pragma unroll
-  for (int i = 0; i < kTcThreads / 32; ++i) {
-    if (i < warp) incl += bars->part[i];
-    total += bars->part[i];
+    for (int o = 1; o < 32; o <<= 1) {
+      const long w = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += w;
+    }
+    if (lane == 31) bars->part[warp] = incl;
+    __syncthreads();
+    all = 0;
+#pragma unroll
+    for (int i = 0; i < kTcThreads / 32; ++i) {
+      if (i < warp) incl += bars->part[i];
+      all += bars->part[i];
+    }
+    return incl;
+  };
+  if (most > 1) atomicMax(&bars->planes, most);
+  long per_head, total;
+  long incl = scan(mine, per_head);
+  total = per_head * a.n_kv;
+  const int planes = max(bars->planes, 1);
+  if (planes > 1) {                                          // (the sum over row tiles is a scan of its own: few batches need it)
+    long w = 0, all;
+    for (int s = s0; s < s1; ++s) {
+      const Seq q = load_seq(a, s, per_item);
+      w += long(q.row_tiles) * item_work(q);
+    }
+    __syncthreads();
+    scan(w, all);
+    total = all * a.n_kv;
   }
-  const long ctas = max(1l, min(long(gridDim.x), total / p.min_work));
+  long ctas = max(1l, min(long(gridDim.x), total / p.min_work));
+  // row tiles side by side, if that leaves no more than a thirtieth of the SMs idle
+  const long lanes = long(a.n_kv) * planes;
+  if (planes > 1 && ctas % lanes * 30 <= ctas && ctas >= lanes) ctas -= ctas % lanes;
   const long w0 = blockIdx.x * total / ctas, w1 = min(total, (blockIdx.x + 1) * total / ctas);
   const bool busy = long(blockIdx.x) < ctas && w0 < w1;
   if (!busy && tid == 0) p.ws_desc[blockIdx.x * 8 + DESC_MERGE] = 0;
-  if (busy && incl - mine <= w0 && w0 < incl) {
-    long at = incl - mine;
-    for (int s = s0; s < s1; ++s) {
-      const long n = seq_work(load_seq(a, s, per_item), a.n_kv);
-      if (w0 < at + n) {
-        bars->seq = s;
-        bars->seq_work = at;
-        break;
+  if (busy) {
+    long base = 0;
+    int plane = 0;
+    while (w0 >= base + per_head * a.n_kv) {                 // the row tile that the stretch begins in
+      base += per_head * a.n_kv;
+      ++plane;
+      mine = 0;
+      for (int s = s0; s < s1; ++s) mine += plane_work(load_seq(a, s, per_item), plane);
+      __syncthreads();
+      incl = scan(mine, per_head);
+    }
+    const int head = int((w0 - base) / per_head);
+    const long in_head = w0 - base - head * per_head;
+    if (incl - mine <= in_head && in_head < incl) {
+      long at = incl - mine;
+      for (int s = s0; s < s1; ++s) {
+        const int n = plane_work(load_seq(a, s, per_item), plane);
+        if (in_head < at + n) {
+          bars->seq = s;
+          bars->plane = plane;
+          bars->head = head;
+          bars->ahead = base + head * per_head + at;
+          break;
+        }
+        at += n;
       }
-      at += n;
     }
   }
   __syncthreads();
@@ -567,15 +615,12 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
     bool ok = true;
     int st = 0, phase = 0, count = 0;
     Piece x;
-    long w = w0;                                                       // work ahead of the current item
-    int row = 0;
+    long w = bars->ahead;                                              // work ahead of the current item
+    int plane = bars->plane;
     if (busy) {
       x.seq = bars->seq;
+      x.head = bars->head;
       x.q = load_seq(a, x.seq, per_item);
-      const int item = int((w0 - bars->seq_work) / item_work(x.q));
-      w = bars->seq_work + long(item) * item_work(x.q);
-      x.head = item / x.q.row_tiles;
-      row = item - x.head * x.q.row_tiles;
     }
     while (ok && busy && w < w1) {
       // the part of the item that lies in the stretch
@@ -583,7 +628,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
       x.j0 = int(max(ahead, 0l));
       x.nt = int(min(behind, long(x.q.key_tiles))) - x.j0;
       if (x.nt > 0) {
-        x.node0 = row * per_item;
+        x.node0 = plane * per_item;
         x.pair = NQ == 2 && x.q.n - x.node0 > p.nodes;
         x.whole = x.nt == x.q.key_tiles;
         x.slot = 2 * blockIdx.x + (count > 0);
@@ -651,14 +696,17 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
         }
       }
       w += item_work(x.q);
-      if (++row == x.q.row_tiles) {
-        row = 0;
-        if (++x.head == a.n_kv) {
-          x.head = 0;
-          if (w < w1)
-            do x.q = load_seq(a, ++x.seq, per_item);
-            while (x.q.row_tiles == 0);
-        }
+      if (w < w1) {
+        do {
+          if (++x.seq == a.B) {
+            x.seq = 0;
+            if (++x.head == a.n_kv) {
+              x.head = 0;
+              ++plane;
+            }
+          }
+          x.q = load_seq(a, x.seq, per_item);
+        } while (x.q.row_tiles <= plane);
       }
     }
     if (lane == 0) {
@@ -667,80 +715,78 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
       if (busy && count == 0) p.ws_desc[blockIdx.x * 8 + DESC_MERGE] = 0;
       if (!ok) atomicExch(p.status, XL_ERR_WAIT_EMPTY);
     }
-  } else if (warp == 1) {
-    // ---------------------------------------------------------- MMA issuer
+  } else if (warp <= 2) {
+    // ---------------------------------------------------------- MMA issuer of group g
     if (elect_one_sync()) {
+      const int g = warp - 1;
       const uint32_t idesc_s = umma_idesc_f16(BQ, BKV, 1), idesc_o = umma_idesc_f16(BQ, DV, 1) | (1u << 16);   // V is MN-major
       // descriptors count in units of 16 bytes: a step along a tile is an addition
       const uint64_t q_desc = umma_desc_sw128(smem_u32(sQ), 0), k_desc = umma_desc_sw128(smem_u32(ring), 0);
       const uint64_t v_desc = umma_desc_sw128_mn(smem_u32(ring), KV_SLAB, 1024);
+      const uint32_t t_s = tmem + g * 256, t_o = t_s + 128;
       bool ok = true;
-      int st = 0, phase = 0, s_count[2] = {0, 0}, p_count[2] = {0, 0};
-      auto take = [&] {                                                // the next unit
-        ok = mbar_wait(&bars->full[st], phase);
-        return ok;
-      };
-      auto leave = [&] {
-        tc_commit(&bars->empty[st]);
+      int st = 0, phase = 0, s_count = 0, p_count = 0;
+      // both issuers go through all units; one that has no use for a unit lets go of it as soon as it is there
+      auto next = [&] {
         if (++st == U) {
           st = 0;
           phase ^= 1;
         }
       };
-      for (int count = 0;; ++count) {
+      for (int count = 0; ok; ++count) {
         const int info = count % kPieces;
         if (!(ok = mbar_wait(&bars->info[info], (count / kPieces) & 1))) break;
         const int nt = bars->piece[info].nt;
         if (nt == 0) break;
         const bool pair = NQ == 2 && bars->piece[info].pair;
         const int lag = pair ? 1 : 2;
-        ok = mbar_wait(&bars->q_full, count & 1);
-        for (int j = 0; ok && j < nt + lag; ++j) {
+        const uint64_t q0 = q_desc + (pair ? g * C::Q_BYTES / 16 : 0);
+        if (!(ok = mbar_wait(&bars->q_full, count & 1))) break;
+        for (int j = 0; j < nt + lag; ++j) {
           if (j < nt) {
-            if (!take()) break;
-            tc_fence_after();
-            const uint64_t k0 = k_desc + st * (UNIT / 16);
-#pragma unroll
-            for (int h = 0; h < NQ; ++h) {
-              if (h == 1 && !pair) break;
-              const int g = pair ? h : j & 1, b = s_count[g]++ & 1;
+            if (!(ok = mbar_wait(&bars->full[st], phase))) break;
+            if (pair || (j & 1) == g) {
+              tc_fence_after();
+              const uint64_t k0 = k_desc + st * (UNIT / 16);
+              const int b = s_count++ & 1;
 #pragma unroll
               for (int k = 0; k < DV / 16; ++k)
-                tc_mma_f16(tmem + g * 256 + b * 64, q_desc + (h * C::Q_BYTES + (k >> 2) * Q_SLAB) / 16 + (k & 3) * 2,
-                           k0 + (k >> 2) * (KV_SLAB / 16) + (k & 3) * 2, idesc_s, k != 0);
+                tc_mma_f16(t_s + b * 64, q0 + (k >> 2) * (Q_SLAB / 16) + (k & 3) * 2, k0 + (k >> 2) * (KV_SLAB / 16) + (k & 3) * 2, idesc_s, k != 0);
               tc_commit(&bars->s_full[g][b]);
+              tc_commit(&bars->empty[st]);
+            } else {
+              mbar_arrive(&bars->empty[st]);
             }
-            leave();
             if (j == nt - 1) tc_commit(&bars->q_empty);
+            next();
           }
           if (j >= lag && j - lag < nt) {
             const int i = j - lag;
-            if (!take()) break;
-            const uint64_t v0 = v_desc + st * (UNIT / 16);
-#pragma unroll
-            for (int h = 0; h < NQ; ++h) {
-              if (h == 1 && !pair) break;
-              const int g = pair ? h : i & 1, b = p_count[g] & 1;
-              if (!(ok = mbar_wait(&bars->p_full[g][b], (p_count[g] >> 1) & 1))) break;
-              ++p_count[g];
+            if (!(ok = mbar_wait(&bars->full[st], phase))) break;
+            if (pair || (i & 1) == g) {
+              const uint64_t v0 = v_desc + st * (UNIT / 16);
+              const int b = p_count & 1;
+              if (!(ok = mbar_wait(&bars->p_full[g][b], (p_count >> 1) & 1))) break;
+              ++p_count;
               tc_fence_after();
 #pragma unroll
               for (int k = 0; k < BKV / 16; ++k)
-                tc_mma_f16_ts(tmem + g * 256 + 128, tmem + g * 256 + b * 64 + k * 8, v0 + k * (2048 / 16), idesc_o, ((pair ? i : i >> 1) | k) != 0);
+                tc_mma_f16_ts(t_o, t_s + b * 64 + k * 8, v0 + k * (2048 / 16), idesc_o, ((pair ? i : i >> 1) | k) != 0);
               tc_commit(&bars->pv_done[g][b]);
+              tc_commit(&bars->empty[st]);
+            } else {
+              mbar_arrive(&bars->empty[st]);
             }
-            if (!ok) break;
-            leave();
+            next();
           }
         }
-        if (!ok) break;
       }
       if (!ok) atomicExch(p.status, XL_ERR_WAIT_FULL);
     }
   } else {
     // ---------------------------------------------------------- softmax, one row per thread
-    const int g = (warp - 2) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
-    const int gt = (warp - 2 - 4 * g) * 32 + lane;                     // thread of the group
+    const int g = (warp - 3) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    const int gt = (warp - 3 - 4 * g) * 32 + lane;                     // thread of the group
     const uint32_t t_lane = tmem + (uint32_t(quarter * 32) << 16), t_s = t_lane + g * 256, t_o = t_s + 128;
     const int node = r / p.group, head_in = r - node * p.group;
     const float sc = p.scale_log2;
@@ -750,7 +796,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
     {
       const int behind = max(a.q_cu[a.B], 0), width = a.n_q * a.D;
       for (long t = long(behind) + blockIdx.x; t < a.T; t += gridDim.x)
-        for (int c = tid - 64; c < width / 8; c += 256) reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + t * width)[c] = make_uint4(0, 0, 0, 0);
+        for (int c = tid - 96; c < width / 8; c += 256) reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + t * width)[c] = make_uint4(0, 0, 0, 0);
     }
     bool ok = true;
     int u0 = 0, count = 0;                                             // units ahead of the piece; tiles of this group so far
@@ -866,8 +912,9 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
             bars->any_bad[piece & 3][g] = 1;
           }
           fence_proxy_async_smem();
-          group_sync();
+          if (!pair) group_sync();
         }
+        if (partly && pair) both_sync();                               // the other group's products wait for the values too
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->p_full[g][b]);
