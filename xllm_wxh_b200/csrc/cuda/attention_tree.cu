@@ -1116,13 +1116,18 @@ static SimtPlan simt_plan(int B, int n_q, int n_kv, int max_q, int max_kv, int s
   return s;
 }
 
-// Bytes of the workspace.  ctas: SMs that the tensor-core kernel may take; max_q, max_kv: bounds of a sequence's rows and keys.  *tc: whether
-// that kernel serves these sizes (rows on 16-byte boundaries and a positive scale given).
-XL_API long xl_attention_tree_workspace(int T, int B, int block_size, int n_q, int n_kv, int D, int f32, int max_q, int max_kv, int ctas, int sms,
-                                        int* tc) {
-  *tc = tc_serves(nullptr, nullptr, nullptr, block_size, n_q, n_kv, D, 8, 8, 1.f, f32);
+// CTAs of the tensor-core kernel: one per SM, fewer where there are fewer key tiles (of 64 keys for up to 128 rows).
+static int tc_ctas(int T, int B, int n_q, int n_kv, int max_kv, int sms) {
+  return int(max(1l, min(long(sms), (long(max_kv) / 64 + 1) * n_kv * (B + long(T) * (n_q / n_kv) / xl_at::BQ))));
+}
+
+// Bytes of the workspace.  max_q, max_kv: bounds of a sequence's rows and keys; plain: fp32, or scores or caches that the tensor-core kernel does not
+// take.  *tc: whether that kernel serves these sizes (for query rows on 16-byte boundaries).
+XL_API long xl_attention_tree_workspace(int T, int B, int block_size, int n_q, int n_kv, int D, int plain, int max_q, int max_kv, int* tc) {
+  *tc = tc_serves(nullptr, nullptr, nullptr, block_size, n_q, n_kv, D, 8, 8, 1.f, plain);
+  const int sms = xl_host::sm_count();
   if (*tc) {
-    const long rows = long(max_q) * (n_q / n_kv) > xl_at::BQ ? 256 : 128, DV = (D + 63) / 64 * 64;
+    const long rows = long(max_q) * (n_q / n_kv) > xl_at::BQ ? 256 : 128, DV = (D + 63) / 64 * 64, ctas = tc_ctas(T, B, n_q, n_kv, max_kv, sms);
     return 2l * ctas * rows * (DV * 4 + 8) + 32l * ctas;
   }
   const SimtPlan s = simt_plan(B, n_q, n_kv, max_q, max_kv, sms);
@@ -1132,13 +1137,13 @@ XL_API long xl_attention_tree_workspace(int T, int B, int block_size, int n_q, i
 XL_API int xl_attention_tree(const void* q, const void* k_cache, const void* v_cache, void* out, const void* q_cu, const void* kv_lens,
                              const void* block_tables, const void* token_seq, const void* positions, const void* tree, int T, int B,
                              int max_blocks, int block_size, int num_blocks, int n_q, int n_kv, int D, int words, long q_row, long q_head,
-                             float scale, int window, int f32, int max_q, int max_kv, int ctas, int sms, int tc, void* workspace, long workspace_bytes,
-                             void* stream) {
+                             float scale, int window, int f32, int max_q, int max_kv, int tc, void* workspace, long workspace_bytes, void* stream) {
   using namespace xl_at;
   if (T < 0 || B < 0 || n_kv < 1 || n_q % n_kv || D < 1 || D > 512 || words < 1 || block_size < 1 || max_blocks < 1) return -2;
   if (T == 0) return 0;
   int served = 0;
-  if (workspace_bytes < xl_attention_tree_workspace(T, B, block_size, n_q, n_kv, D, f32 || !tc, max_q, max_kv, ctas, sms, &served)) return -2;
+  if (workspace_bytes < xl_attention_tree_workspace(T, B, block_size, n_q, n_kv, D, f32 || !tc, max_q, max_kv, &served)) return -2;
+  const int sms = xl_host::sm_count();
   Params p{};
   p.q = q; p.k_cache = k_cache; p.v_cache = v_cache; p.out = out;
   p.q_cu = static_cast<const int*>(q_cu);
@@ -1155,7 +1160,7 @@ XL_API int xl_attention_tree(const void* q, const void* k_cache, const void* v_c
   if (tc) {
     if (B < 1 || !workspace || !tc_serves(q, k_cache, v_cache, block_size, n_q, n_kv, D, q_row, q_head, scale, f32)) return -2;
     const bool pair = long(max_q) * (n_q / n_kv) > BQ;
-    if (ctas < 1) return -2;
+    const int ctas = tc_ctas(T, B, n_q, n_kv, max_kv, sms);
     TcParams t{};
     t.a = p;
     t.group = n_q / n_kv;

@@ -335,6 +335,11 @@ def _tree():
     return tree_cuda
 
 
+def _amiss(name):
+    """The kernels' host side has turned a call down that none of the checks finds fault with."""
+    raise RuntimeError(f"{name}: sizes beyond what the kernels take")
+
+
 def _like(t, dtype, shape, dev, name):
     """Checks one argument: element type, sizes, dense, on the device of that number."""
     assert t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous(), \
@@ -351,6 +356,12 @@ def step_rows(tables, lens, seqs, counts, n_rows, block_size, parents=None, max_
     the reserved block 0.  max_q bounds counts (trees: at most 256); max_blocks: columns of the new tables (all), unused ones 0.
     Sequences outside the pool (padding: -1) add nothing.  Returns StepRows (positions, slots, token_seq, q_cu, kv_lens,
     block_tables, tree)."""
+    max_q = max(1, n_rows) if max_q is None else max_q
+    max_blocks = tables.shape[1] if max_blocks is None else max_blocks
+    if tables.is_cuda:
+        out = _tree().step_rows(tables, lens, seqs, counts, n_rows, block_size, parents, max_q, max_blocks)
+        if out is not None:
+            return out
     dev, i32 = tables.get_device(), torch.int32
     assert tables.dtype is i32 and tables.dim() == 2 and (tables.stride(1) == 1 or tables.shape[1] <= 1), "tables: int32 [pool, blocks]"
     pool, blocks = tables.shape
@@ -358,14 +369,13 @@ def step_rows(tables, lens, seqs, counts, n_rows, block_size, parents=None, max_
     _like(lens, i32, (pool,), dev, "lens")
     _like(seqs, i32, B, dev, "seqs")
     _like(counts, i32, B, dev, "counts")
-    max_q = max(1, n_rows) if max_q is None else max_q
-    max_blocks = blocks if max_blocks is None else max_blocks
     assert n_rows >= 0 and block_size >= 1 and max_q >= 1 and 0 <= max_blocks <= blocks and B[0] < 65535
     if parents is not None:
         _like(parents, i32, (n_rows,), dev, "parents")
         assert max_q <= TREE_MAX_ROWS, f"trees have at most {TREE_MAX_ROWS} rows a sequence: give max_q"
-    f = _tree().step_rows if tables.is_cuda else ref.step_rows
-    return f(tables, lens, seqs, counts, n_rows, block_size, parents, max_q, max_blocks)
+    if tables.is_cuda:
+        _amiss("step_rows")
+    return ref.step_rows(tables, lens, seqs, counts, n_rows, block_size, parents, max_q, max_blocks)
 
 
 def tree_attention(q, k_cache, v_cache, inp, tree, scale, sliding_window=-1):
@@ -374,6 +384,10 @@ def tree_attention(q, k_cache, v_cache, inp, tree, scale, sliding_window=-1):
     block, Hkv, D] that hold the step's rows already; `inp` has q_cu, kv_lens, block_tables, token_seq, positions, n_seqs, and max_q and
     max_kv as bounds.  `sliding_window`: only keys at positions above the row's own - window.  Rows that see nothing and rows of no
     sequence are zero.  Returns [T, Hq * D].  bf16 or fp32, up to 512 columns a head."""
+    if q.is_cuda:
+        out = _tree().tree_attention(q, k_cache, v_cache, inp, tree, scale, sliding_window)
+        if out is not None:
+            return out
     T, Hq, D = q.shape
     dev, i32, B = q.get_device(), torch.int32, inp.n_seqs
     assert q.dtype is k_cache.dtype is v_cache.dtype and q.dtype in (torch.bfloat16, torch.float32), "q and caches: one type, bf16 or fp32"
@@ -390,8 +404,9 @@ def tree_attention(q, k_cache, v_cache, inp, tree, scale, sliding_window=-1):
     _like(tables, i32, (B, tables.shape[1]), dev, "block_tables")
     _like(inp.token_seq, i32, (T,), dev, "token_seq")
     _like(inp.positions, i32, (T,), dev, "positions")
-    f = _tree().tree_attention if q.is_cuda else ref.tree_attention
-    return f(q, k_cache, v_cache, inp, tree, float(scale), int(sliding_window))
+    if q.is_cuda:
+        _amiss("tree_attention")
+    return ref.tree_attention(q, k_cache, v_cache, inp, tree, scale, sliding_window)
 
 
 def adjust_logits(logits, q_cu, seqs=None, history=None, penalties=None, tokens=None, parents=None, bias=None, mask=None, max_q=None):
@@ -406,6 +421,9 @@ def adjust_logits(logits, q_cu, seqs=None, history=None, penalties=None, tokens=
     mask = (words int32 [masks, >= V / 32], rows int32 [S]): ids whose bit is 0 in the row's mask become -inf (rows: -1 for none).
     Ids outside the vocabulary are passed over.  Returns logits."""
     S, V = logits.shape
+    max_q = max(1, S) if max_q is None else max_q
+    if logits.is_cuda and _tree().adjust_logits(logits, q_cu, seqs, history, penalties, tokens, parents, bias, mask, max_q):
+        return logits
     dev, i32, f32 = logits.get_device(), torch.int32, torch.float32
     assert logits.dtype in (f32, torch.bfloat16) and (logits.stride(1) == 1 or V == 1) and (logits.stride(0) >= V or S <= 1), "logits: fp32 or bf16 rows"
     assert q_cu.dim() == 1 and q_cu.numel() >= 1, "q_cu: [B + 1]"
@@ -442,10 +460,10 @@ def adjust_logits(logits, q_cu, seqs=None, history=None, penalties=None, tokens=
         assert words.dtype is i32 and words.dim() == 2 and words.stride(1) == 1 and words.shape[1] * 32 >= V and words.get_device() == dev, \
             "mask: int32 [masks, V / 32]"
         _like(rows, i32, (S,), dev, "mask rows")
-    max_q = max(1, S) if max_q is None else max_q
     assert max_q >= 1 and (tokens is None or max_q <= TREE_MAX_ROWS), f"at most {TREE_MAX_ROWS} rows a sequence with tokens: give max_q"
-    f = _tree().adjust_logits if logits.is_cuda else ref.adjust_logits
-    return f(logits, q_cu, seqs, history, penalties, tokens, parents, bias, mask, max_q)
+    if logits.is_cuda:
+        _amiss("adjust_logits")
+    return ref.adjust_logits(logits, q_cu, seqs, history, penalties, tokens, parents, bias, mask, max_q)
 
 
 def accept_tree(target, inp, parents, caches=(), max_depth=None):
@@ -455,6 +473,11 @@ def accept_tree(target, inp, parents, caches=(), max_depth=None):
     target's tokens along the path, then -1; accepted [B]: drafted rows on the path; path [B, max_depth + 1]: their numbers, then -1).
     In every tensor of `caches` ([blocks, block, ...], contiguous, no tensor twice) the path's rows move to the positions behind the
     sequence's earlier tokens, which then has 1 + accepted more; the other drafted rows' places hold what they held."""
+    depth = max(0, inp.max_q - 1) if max_depth is None else max_depth
+    if target.is_cuda:
+        out = _tree().accept_tree(target, inp, parents, caches, depth)
+        if out is not None:
+            return out
     dev, i32, B, tables, block = target.get_device(), torch.int32, inp.n_seqs, inp.block_tables, inp.block_size
     T = (target.numel(),)
     _like(target, i32, T, dev, "target")
@@ -465,18 +488,12 @@ def accept_tree(target, inp, parents, caches=(), max_depth=None):
     assert tables.dim() == 2, "block_tables: [B, blocks]"
     _like(tables, i32, (B, tables.shape[1]), dev, "block_tables")
     assert inp.max_q <= TREE_MAX_ROWS, f"trees have at most {TREE_MAX_ROWS} rows a sequence"
-    depth = max(0, inp.max_q - 1) if max_depth is None else max_depth
     assert 0 <= depth < TREE_MAX_ROWS and B < 65536
-    at, shape = [], None
     for c in caches:
-        if c.shape != shape:
-            shape = c.shape
-            assert len(shape) >= 2 and shape[1] == block, "caches: [blocks, block, ...]"
-        assert c.is_contiguous() and c.get_device() == dev, "caches: contiguous, beside the others"
-        at.append(c.data_ptr())
-    assert len(set(at)) == len(at) or len({c.data_ptr() for c in caches if c.numel()}) == sum(c.numel() > 0 for c in caches), "a cache may be named once"
+        assert c.is_contiguous() and c.dim() >= 2 and c.shape[1] == block and c.get_device() == dev, "caches: [blocks, block, ...], contiguous"
+    assert len({c.data_ptr() for c in caches if c.numel()}) == sum(c.numel() > 0 for c in caches), "a cache may be named once"
     if target.is_cuda:
-        return _tree().accept_tree(target, inp, parents, caches, at, depth)
+        _amiss("accept_tree")
     return ref.accept_tree(target, inp, parents, caches, depth)
 
 
