@@ -397,6 +397,8 @@ constexpr int Q_SLAB = BQ * 128, KV_SLAB = BKV * 128;
 constexpr int kMaxUnits = 20, kPieces = 8, kItemCost = 3;
 
 __device__ __forceinline__ int item_work(const Seq& q) { return q.key_tiles + kItemCost; }
+// a quotient of two numbers that are hardly ever above 32 bits
+__device__ __forceinline__ long quotient(long a, long b) { return uint64_t(a | b) >> 32 ? a / b : long(uint32_t(a) / uint32_t(b)); }
 // of a key head's items of row tile `plane`
 __device__ __forceinline__ int plane_work(const Seq& q, int plane) { return q.row_tiles > plane ? item_work(q) : 0; }
 struct Piece {
@@ -570,11 +572,14 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
     scan(w, all);
     total = all * a.n_kv;
   }
-  long ctas = max(1l, min(long(gridDim.x), total / p.min_work));
+  long ctas = max(1l, min(long(gridDim.x), quotient(total, p.min_work)));
   // row tiles side by side, if that leaves no more than a thirtieth of the SMs idle
   const long lanes = long(a.n_kv) * planes;
   if (planes > 1 && ctas % lanes * 30 <= ctas && ctas >= lanes) ctas -= ctas % lanes;
-  const long w0 = blockIdx.x * total / ctas, w1 = min(total, (blockIdx.x + 1) * total / ctas);
+  // the first `longer` stretches have one more
+  const long per_cta = quotient(total, ctas), longer = total - per_cta * ctas;
+  auto begin = [&](long c) { return c * per_cta + min(c, longer); };
+  const long w0 = begin(blockIdx.x), w1 = long(blockIdx.x) < ctas ? begin(blockIdx.x + 1l) : w0;
   const bool busy = long(blockIdx.x) < ctas && w0 < w1;
   if (!busy && tid == 0) p.ws_desc[blockIdx.x * 8 + DESC_MERGE] = 0;
   if (busy) {
@@ -588,7 +593,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
       __syncthreads();
       incl = scan(mine, per_head);
     }
-    const int head = int((w0 - base) / per_head);
+    const int head = int(quotient(w0 - base, per_head));
     const long in_head = w0 - base - head * per_head;
     if (incl - mine <= in_head && in_head < incl) {
       long at = incl - mine;
@@ -632,21 +637,17 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
         x.pair = NQ == 2 && x.q.n - x.node0 > p.nodes;
         x.whole = x.nt == x.q.key_tiles;
         x.slot = 2 * blockIdx.x + (count > 0);
+        // a lane's place in tile j; the values of a tile are fetched `lag` tiles after its keys, from the same places
+        const int* bt = a.block_tables + size_t(x.seq) * a.max_blocks;
+        auto place = [&](int j) {
+          const int tok = x.key0(j) + bx * p.box_tokens;
+          const int blk = p.block_shift >= 0 ? tok >> p.block_shift : tok / a.block_size;
+          const long slot = long(bt[min(blk, a.max_blocks - 1)]) * a.block_size + (tok - blk * a.block_size);
+          return slot < 0 || slot + p.box_tokens > a.num_slots ? 0 : int(slot);  // places behind the last row
+        };
+        int next = lane < per_unit ? place(0) : 0, held0 = 0, held1 = 0;
         const int info = count % kPieces;
         if (lane == 0) {
-          if (count == 0) {
-            int* d = p.ws_desc + blockIdx.x * 8;
-            const bool merge = x.j0 > 0 && x.j0 + x.nt == x.q.key_tiles;
-            d[DESC_MERGE] = merge;
-            if (merge) {
-              const long first = ((w + kItemCost + 1) * ctas - 1) / total;      // CTA of the item's first tile
-              d[DESC_FIRST] = int(first);
-              d[DESC_SLOT] = int(2 * first + (first * total / ctas < w ? 1 : 0));
-              d[DESC_START] = x.q.q_start + x.node0;
-              d[DESC_NODES] = min(per_item, x.q.n - x.node0);
-              d[DESC_HEAD] = x.head;
-            }
-          }
           ok = mbar_wait(&bars->q_empty, (count & 1) ^ 1);
           if (ok) {
             bars->piece[info] = x;
@@ -660,15 +661,6 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
           }
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
-        ++count;
-        // a lane's place in tile j; the values of a tile are fetched `lag` tiles after its keys, from the same places
-        const int* bt = a.block_tables + size_t(x.seq) * a.max_blocks;
-        auto place = [&](int j) {
-          const int tok = x.key0(j) + bx * p.box_tokens;
-          const int blk = p.block_shift >= 0 ? tok >> p.block_shift : tok / a.block_size;
-          const long slot = long(bt[min(blk, a.max_blocks - 1)]) * a.block_size + (tok - blk * a.block_size);
-          return slot < 0 || slot + p.box_tokens > a.num_slots ? 0 : int(slot);  // places behind the last row
-        };
         auto unit = [&](const CUtensorMap* map, int slot) {
           if (lane == 0) {
             ok = mbar_wait(&bars->empty[st], phase ^ 1);
@@ -683,7 +675,6 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
           }
         };
         const int lag = x.pair ? 1 : 2;
-        int next = lane < per_unit ? place(0) : 0, held0 = 0, held1 = 0;
         for (int j = 0; ok && j < x.nt + lag; ++j) {
           const int slot = next;
           if (j < x.nt) {
@@ -694,6 +685,21 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
           held1 = held0;
           held0 = slot;
         }
+        if (count == 0 && lane == 0) {
+          int* d = p.ws_desc + blockIdx.x * 8;
+          const bool merge = x.j0 > 0 && x.j0 + x.nt == x.q.key_tiles;
+          d[DESC_MERGE] = merge;
+          if (merge) {
+            const long tile0 = w + kItemCost, even = (per_cta + 1) * longer;    // the item's first tile; work of the longer stretches
+            const long first = tile0 < even ? quotient(tile0, per_cta + 1) : longer + quotient(tile0 - even, per_cta);
+            d[DESC_FIRST] = int(first);
+            d[DESC_SLOT] = int(2 * first + (begin(first) < w ? 1 : 0));
+            d[DESC_START] = x.q.q_start + x.node0;
+            d[DESC_NODES] = min(per_item, x.q.n - x.node0);
+            d[DESC_HEAD] = x.head;
+          }
+        }
+        ++count;
       }
       w += item_work(x.q);
       if (w < w1) {
