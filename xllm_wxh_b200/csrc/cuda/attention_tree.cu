@@ -397,8 +397,6 @@ constexpr int Q_SLAB = BQ * 128, KV_SLAB = BKV * 128;
 constexpr int kMaxUnits = 20, kPieces = 8, kItemCost = 3;
 
 __device__ __forceinline__ int item_work(const Seq& q) { return q.key_tiles + kItemCost; }
-// a quotient of two numbers that are hardly ever above 32 bits
-__device__ __forceinline__ long quotient(long a, long b) { return uint64_t(a | b) >> 32 ? a / b : long(uint32_t(a) / uint32_t(b)); }
 // of a key head's items of row tile `plane`
 __device__ __forceinline__ int plane_work(const Seq& q, int plane) { return q.row_tiles > plane ? item_work(q) : 0; }
 struct Piece {
@@ -421,9 +419,8 @@ struct TcBarriers {
   // would be a phase off
   uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];
   uint32_t tmem_base;
-  int seq, plane, head, planes;                              // of the first item; row tiles of any sequence at most
+  int work[kTcThreads], most[kTcThreads];                    // of a thread's sequences: work of the first row tiles, row tiles at most
   int any_bad[4][2];                                         // [piece & 3][group]
-  long ahead, part[kTcThreads / 32];                         // work ahead of the first item
   uint32_t bad[4][2][16][2];                                 // [piece & 3][group][tile][key]: keys whose values are not all finite
   float2 ml[2][BQ];
   Piece piece[kPieces];
@@ -504,14 +501,14 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
   const int per_item = NQ * p.nodes;
   const int share = (a.B + kTcThreads - 1) / kTcThreads;
   const int s0 = min(tid * share, a.B), s1 = min(s0 + share, a.B);
-  long mine = 0;                                             // of the first row tiles
-  if (tid == 0) bars->planes = 0;
-  int most = 0;
+  int mine = 0, most = 1;
   for (int s = s0; s < s1; ++s) {
     const Seq q = load_seq(a, s, per_item);
     mine += plane_work(q, 0);
     most = max(most, q.row_tiles);
   }
+  bars->work[tid] = mine;
+  bars->most[tid] = most;
   if (warp == 0 && lane < 3) prefetch_tmap(lane == 0 ? &tmQ : lane == 1 ? &tmK : &tmV);
   if (tid == 64) {
     for (int u = 0; u < U; ++u) {
@@ -539,99 +536,78 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // sums over the sequences up to and with this thread's, and over all
-  auto scan = [&](long v, long& all) {
-    long incl = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long w = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += w;
-    }
-    if (lane == 31) bars->part[warp] = incl;
-    __syncthreads();
-    all = 0;
-#pragma unroll
-    for (int i = 0; i < kTcThreads / 32; ++i) {
-      if (i < warp) incl += bars->part[i];
-      all += bars->part[i];
-    }
-    return incl;
-  };
-  if (most > 1) atomicMax(&bars->planes, most);
-  long per_head, total;
-  long incl = scan(mine, per_head);
-  total = per_head * a.n_kv;
-  const int planes = max(bars->planes, 1);
-  if (planes > 1) {                                          // (the sum over row tiles is a scan of its own: few batches need it)
-    long w = 0, all;
-    for (int s = s0; s < s1; ++s) {
-      const Seq q = load_seq(a, s, per_item);
-      w += long(q.row_tiles) * item_work(q);
-    }
-    __syncthreads();
-    scan(w, all);
-    total = all * a.n_kv;
-  }
-  long ctas = max(1l, min(long(gridDim.x), quotient(total, p.min_work)));
-  // row tiles side by side, if that leaves no more than a thirtieth of the SMs idle
-  const long lanes = long(a.n_kv) * planes;
-  if (planes > 1 && ctas % lanes * 30 <= ctas && ctas >= lanes) ctas -= ctas % lanes;
-  // the first `longer` stretches have one more
-  const long per_cta = quotient(total, ctas), longer = total - per_cta * ctas;
-  auto begin = [&](long c) { return c * per_cta + min(c, longer); };
-  const long w0 = begin(blockIdx.x), w1 = long(blockIdx.x) < ctas ? begin(blockIdx.x + 1l) : w0;
-  const bool busy = long(blockIdx.x) < ctas && w0 < w1;
-  if (!busy && tid == 0) p.ws_desc[blockIdx.x * 8 + DESC_MERGE] = 0;
-  if (busy) {
-    long base = 0;
-    int plane = 0;
-    while (w0 >= base + per_head * a.n_kv) {                 // the row tile that the stretch begins in
-      base += per_head * a.n_kv;
-      ++plane;
-      mine = 0;
-      for (int s = s0; s < s1; ++s) mine += plane_work(load_seq(a, s, per_item), plane);
-      __syncthreads();
-      incl = scan(mine, per_head);
-    }
-    const int head = int(quotient(w0 - base, per_head));
-    const long in_head = w0 - base - head * per_head;
-    if (incl - mine <= in_head && in_head < incl) {
-      long at = incl - mine;
-      for (int s = s0; s < s1; ++s) {
-        const int n = plane_work(load_seq(a, s, per_item), plane);
-        if (in_head < at + n) {
-          bars->seq = s;
-          bars->plane = plane;
-          bars->head = head;
-          bars->ahead = base + head * per_head + at;
-          break;
-        }
-        at += n;
-      }
-    }
-  }
-  __syncthreads();
   const uint32_t tmem = bars->tmem_base;                     // group g: S / P buffers at g * 256 + {0, 64}, O at g * 256 + 128
 
   if (warp == 0) {
     // ---------------------------------------------------------- TMA producer (whole warp: lanes share the boxes)
     const int boxes = BKV / p.box_tokens, per_unit = boxes * QS;       // boxes of a 64-column slab; at most 8 x 2
     const int slab = lane / boxes, bx = lane % boxes;
+    // the sum of the work; this CTA's stretch [w0, w1) of it; the item that it begins in.  (Only this warp needs them.)
+    auto inclusive = [&](int v) {
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int w = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += w;
+      }
+      return v;
+    };
+    constexpr int kEach = kTcThreads / 32;
+    int sum = 0, planes = 1;
+#pragma unroll 1
+    for (int i = 0; i < kEach; ++i) {
+      sum += bars->work[lane * kEach + i];
+      planes = max(planes, bars->most[lane * kEach + i]);
+    }
+    planes = __reduce_max_sync(0xffffffffu, planes);
+    int upto = inclusive(sum), per_head = __shfl_sync(0xffffffffu, upto, 31), total = per_head * a.n_kv;
+    auto plane_sum = [&](int plane) {
+      int v = 0;
+      for (int s = lane; s < a.B; s += 32) v += plane_work(load_seq(a, s, per_item), plane);
+      return __reduce_add_sync(0xffffffffu, v);
+    };
+    for (int i = 1; i < planes; ++i) total += plane_sum(i) * a.n_kv;
+    int ctas = max(1, min(int(gridDim.x), total / p.min_work));
+    // row tiles side by side, if that leaves no more than a thirtieth of the SMs idle
+    const int lanes = a.n_kv * planes;
+    if (planes > 1 && ctas % lanes * 30 <= ctas && ctas >= lanes) ctas -= ctas % lanes;
+    const int per_cta = total / ctas, longer = total - per_cta * ctas;   // the first `longer` stretches have one more
+    auto begin = [&](int c) { return c * per_cta + min(c, longer); };
+    const int w0 = begin(min(int(blockIdx.x), ctas)), w1 = begin(min(int(blockIdx.x) + 1, ctas));
+    const bool busy = w0 < w1;
+    Piece x;
+    int w = 0, plane = 0;                                              // w: work ahead of the current item
+    if (busy) {
+      while (w0 >= w + per_head * a.n_kv) {                            // the row tile
+        w += per_head * a.n_kv;
+        per_head = plane_sum(++plane);
+      }
+      x.head = (w0 - w) / per_head;
+      w += x.head * per_head;
+      int s = 0, at = 0;                                               // a sequence at or ahead of the one, the work ahead of it
+      if (plane == 0) {                                                // by the threads' sums
+        const uint32_t here = __ballot_sync(0xffffffffu, upto - sum <= w0 - w && w0 - w < upto);
+        const int l = __ffs(here) - 1;
+        at = __shfl_sync(0xffffffffu, upto - sum, l);
+        int t = l * kEach;
+        while (at + bars->work[t] <= w0 - w) at += bars->work[t++];
+        s = t * share;
+      }
+      while (true) {
+        x.seq = s;
+        x.q = load_seq(a, s, per_item);
+        const int n = plane_work(x.q, plane);
+        if (w0 - w < at + n) break;
+        at += n;
+        ++s;
+      }
+      w += at;
+    }
     bool ok = true;
     int st = 0, phase = 0, count = 0;
-    Piece x;
-    long w = bars->ahead;                                              // work ahead of the current item
-    int plane = bars->plane;
-    if (busy) {
-      x.seq = bars->seq;
-      x.head = bars->head;
-      x.q = load_seq(a, x.seq, per_item);
-    }
     while (ok && busy && w < w1) {
       // the part of the item that lies in the stretch
-      const long ahead = w0 - w - kItemCost, behind = w1 - w - kItemCost;
-      x.j0 = int(max(ahead, 0l));
-      x.nt = int(min(behind, long(x.q.key_tiles))) - x.j0;
+      x.j0 = max(w0 - w - kItemCost, 0);
+      x.nt = min(w1 - w - kItemCost, x.q.key_tiles) - x.j0;
       if (x.nt > 0) {
         x.node0 = plane * per_item;
         x.pair = NQ == 2 && x.q.n - x.node0 > p.nodes;
@@ -639,13 +615,16 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
         x.slot = 2 * blockIdx.x + (count > 0);
         // a lane's place in tile j; the values of a tile are fetched `lag` tiles after its keys, from the same places
         const int* bt = a.block_tables + size_t(x.seq) * a.max_blocks;
-        auto place = [&](int j) {
+        auto block_of = [&](int j) {
           const int tok = x.key0(j) + bx * p.box_tokens;
-          const int blk = p.block_shift >= 0 ? tok >> p.block_shift : tok / a.block_size;
-          const long slot = long(bt[min(blk, a.max_blocks - 1)]) * a.block_size + (tok - blk * a.block_size);
+          return min(p.block_shift >= 0 ? tok >> p.block_shift : tok / a.block_size, a.max_blocks - 1);
+        };
+        auto place = [&](int j, int entry) {
+          const int tok = x.key0(j) + bx * p.box_tokens;
+          const long slot = long(entry) * a.block_size + (p.block_shift >= 0 ? tok & (a.block_size - 1) : tok % a.block_size);
           return slot < 0 || slot + p.box_tokens > a.num_slots ? 0 : int(slot);  // places behind the last row
         };
-        int next = lane < per_unit ? place(0) : 0, held0 = 0, held1 = 0;
+        int next = lane < per_unit ? bt[block_of(0)] : 0, held0 = 0, held1 = 0;  // (looked up one tile ahead)
         const int info = count % kPieces;
         if (lane == 0) {
           ok = mbar_wait(&bars->q_empty, (count & 1) ^ 1);
@@ -676,9 +655,9 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
         };
         const int lag = x.pair ? 1 : 2;
         for (int j = 0; ok && j < x.nt + lag; ++j) {
-          const int slot = next;
+          const int slot = place(j, next);
           if (j < x.nt) {
-            if (lane < per_unit && j + 1 < x.nt) next = place(j + 1);
+            if (lane < per_unit && j + 1 < x.nt) next = bt[block_of(j + 1)];
             unit(&tmK, slot);
           }
           if (ok && j >= lag && j - lag < x.nt) unit(&tmV, lag == 1 ? held0 : held1);
@@ -690,10 +669,10 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
           const bool merge = x.j0 > 0 && x.j0 + x.nt == x.q.key_tiles;
           d[DESC_MERGE] = merge;
           if (merge) {
-            const long tile0 = w + kItemCost, even = (per_cta + 1) * longer;    // the item's first tile; work of the longer stretches
-            const long first = tile0 < even ? quotient(tile0, per_cta + 1) : longer + quotient(tile0 - even, per_cta);
-            d[DESC_FIRST] = int(first);
-            d[DESC_SLOT] = int(2 * first + (begin(first) < w ? 1 : 0));
+            const int tile0 = w + kItemCost, even = (per_cta + 1) * longer;     // the item's first tile; work of the longer stretches
+            const int first = tile0 < even ? tile0 / (per_cta + 1) : longer + (tile0 - even) / per_cta;
+            d[DESC_FIRST] = first;
+            d[DESC_SLOT] = 2 * first + (begin(first) < w ? 1 : 0);
             d[DESC_START] = x.q.q_start + x.node0;
             d[DESC_NODES] = min(per_item, x.q.n - x.node0);
             d[DESC_HEAD] = x.head;
@@ -718,7 +697,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
     if (lane == 0) {
       bars->piece[count % kPieces].nt = 0;
       mbar_arrive(&bars->info[count % kPieces]);
-      if (busy && count == 0) p.ws_desc[blockIdx.x * 8 + DESC_MERGE] = 0;
+      if (count == 0) p.ws_desc[blockIdx.x * 8 + DESC_MERGE] = 0;
       if (!ok) atomicExch(p.status, XL_ERR_WAIT_EMPTY);
     }
   } else if (warp <= 2) {
@@ -1167,6 +1146,8 @@ XL_API int xl_attention_tree(const void* q, const void* k_cache, const void* v_c
     if (B < 1 || !workspace || !tc_serves(q, k_cache, v_cache, block_size, n_q, n_kv, D, q_row, q_head, scale, f32)) return -2;
     const bool pair = long(max_q) * (n_q / n_kv) > BQ;
     const int ctas = tc_ctas(T, B, n_q, n_kv, max_kv, sms);
+    // the kernel counts its work in 32 bits
+    if ((long(B) + long(T) * (n_q / n_kv) / BQ) * n_kv * (long(max_blocks) * block_size / BKV + 2 + kItemCost) > 0x7fffffffl) return -2;
     TcParams t{};
     t.a = p;
     t.group = n_q / n_kv;
