@@ -122,6 +122,8 @@ SIZES = [                     # before, counts, Hq, Hkv, D, block, words
     ([90, 40], [12, 7], 4, 2, 512, 16, 1),
     ([90, 40], [12, 7], 6, 2, 7, 5, 1),
     ([90, 40], [12, 7], 6, 2, 64, 1, 1),
+    ([300], [1], 1, 1, 64, 16, 1),                               # an odd number of partial rows
+    ([700], [3], 3, 1, 68, 16, 1),
     (list(range(0, 400, 10)), [1 + i % 6 for i in range(40)], 8, 2, 64, 16, 1),
 ]
 

@@ -86,6 +86,7 @@ template <typename T, int NC>
 __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const Params p, int row_tiles, int splits, int part_keys, float* ws_o,
                                                                            float2* ws_ml) {
   extern __shared__ __align__(16) uint8_t smem[];
+  grid_dep_launch();
   using S = SimtSmem<NC>;
   S& sm = *reinterpret_cast<S*>(smem);
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15, D = p.D;
@@ -293,6 +294,7 @@ __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const
 // One warp per (row, query head): joins the parts of its keys, and clears rows of no sequence.
 template <typename T>
 __global__ void __launch_bounds__(128) attention_tree_join_kernel(const Params p, int splits, int part_keys, const float* ws_o, const float2* ws_ml) {
+  grid_dep_wait();
   const long row = blockIdx.x * 4l + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (row >= long(p.T) * p.n_q) return;
@@ -322,22 +324,41 @@ __global__ void __launch_bounds__(128) attention_tree_join_kernel(const Params p
   }
   l = warp_sum(l);
   const float inv = l != 0.f ? 1.f / l : 0.f;
-  for (int c = lane; c - lane < p.D; c += 32) {
-    float o = 0.f;
+  // four columns a lane; the two halves of the warp take the parts in turn, eight loads at a time
+  for (int c0 = 0; c0 < p.D; c0 += 64) {
+    const int c = c0 + 4 * (lane & 15);
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-    for (int k = 0; k < parts; ++k) {
-      float w = __shfl_sync(0xffffffffu, ml[0].x, k & 31);
+    for (int k = 0; k < parts; k += 2) {
+      const int mine = k + (lane >> 4);
+      float w = __shfl_sync(0xffffffffu, ml[0].x, mine & 31);
 #pragma unroll
       for (int i = 1; i < kMaxParts / 32; ++i) {
-        const float v = __shfl_sync(0xffffffffu, ml[i].x, k & 31);
-        if (k >> 5 == i) w = v;
+        const float v = __shfl_sync(0xffffffffu, ml[i].x, mine & 31);
+        if (mine >> 5 == i) w = v;
       }
-      const float x = c < p.D ? ws_o[(k * pitch + row) * p.D + c] : 0.f;
-      if (w != 0.f) o = fmaf(w, x, o);
+      const float* from = ws_o + (mine * pitch + row) * p.D + c;
+      float x[4] = {0.f, 0.f, 0.f, 0.f};
+      if (mine < parts && p.D % 4 == 0 && c < p.D) {
+        *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(from);
+      } else if (mine < parts) {
+        for (int e = 0; e < 4; ++e)
+          if (c + e < p.D) x[e] = from[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (mine < parts && w != 0.f) o[e] = fmaf(w, x[e], o[e]);
     }
-    if (c < p.D) from_f32(out + c, o * inv);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o[e] += __shfl_xor_sync(0xffffffffu, o[e], 16);
+      if (lane < 16 && c + e < p.D) from_f32(out + c + e, o[e] * inv);
+    }
   }
 }
+
+// floats of the parts' maxima and sums, so that what follows lies on 16 bytes
+inline long ml_floats(int splits, int T, int n_q) { return (2l * splits * T * n_q + 3) / 4 * 4; }
 
 template <typename T, int NC>
 int launch_simt(const Params& p, int row_tiles, int splits, int part_keys, float* ws, cudaStream_t s) {
@@ -350,14 +371,24 @@ int launch_simt(const Params& p, int row_tiles, int splits, int part_keys, float
     ready[dev].store(true, std::memory_order_release);
   }
   float2* ml = reinterpret_cast<float2*>(ws);
-  float* o = ws + 2l * splits * p.T * p.n_q;
+  float* o = ws + ml_floats(splits, p.T, p.n_q);
   if (p.B > 0) {
     kernel<<<dim3(p.B * row_tiles, p.n_kv, splits), kSimtThreads, sizeof(SimtSmem<NC>), s>>>(p, row_tiles, splits, part_keys, o, ml);
     if (cudaGetLastError() != cudaSuccess) return -1;
   }
   if (p.B > 0 && splits == 1) return 0;
-  attention_tree_join_kernel<T><<<unsigned((long(p.T) * p.n_q + 3) / 4), 128, 0, s>>>(p, splits, part_keys, o, ml);
-  return cudaGetLastError() == cudaSuccess ? 0 : -1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned((long(p.T) * p.n_q + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.B > 0 ? 1 : 0;
+  const float* from = o;
+  const float2* from_ml = ml;
+  return cudaLaunchKernelEx(&cfg, attention_tree_join_kernel<T>, p, splits, part_keys, from, from_ml) == cudaSuccess ? 0 : -1;
 }
 template <typename T>
 int launch_simt(const Params& p, int row_tiles, int splits, int part_keys, float* ws, cudaStream_t s) {
@@ -1116,7 +1147,7 @@ XL_API long xl_attention_tree_workspace(int T, int B, int block_size, int n_q, i
     return 2l * ctas * rows * (DV * 4 + 8) + 32l * ctas;
   }
   const SimtPlan s = simt_plan(B, n_q, n_kv, max_q, max_kv, sms);
-  return s.splits > 1 ? long(s.splits) * T * n_q * (D + 2) * 4 : 0;
+  return s.splits > 1 ? 4 * (xl_at::ml_floats(s.splits, T, n_q) + long(s.splits) * T * n_q * D) : 0;
 }
 
 XL_API int xl_attention_tree(const void* q, const void* k_cache, const void* v_cache, void* out, const void* q_cu, const void* kv_lens,
