@@ -112,6 +112,8 @@ def test_other_attention_refuses_trees():
         ops.paged_attention_ext(None, None, None, inp, 1.0)
     with pytest.raises(NotImplementedError):
         ops.mla_attention(None, None, None, inp, 1.0, 512)
+    with pytest.raises(NotImplementedError):
+        ops.latent_attention(torch.zeros(1, 2, 24), torch.zeros(2, 8, 16), torch.zeros(2, 16, 8), torch.zeros(1, 4, 16), inp, None, 1.0, 16)
 
 
 # ----------------------------------------------------------------------------- logits

@@ -230,6 +230,22 @@ def test_tree_attention_empty_steps():
     assert ops.tree_attention(q.cuda(), k.cuda(), v.cuda(), step.to("cuda"), step.tree.cuda(), 1.0).shape == (0, 256)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_tree_attention_rows_ahead_of_the_first_sequence_and_without_keys(dtype):
+    """Rows that no sequence owns lie ahead of the first one too; a sequence without keys gets zeros."""
+    step = oracle.Step([20, 5], [6, 4], 16, seed=3)
+    q, k, v = attention_inputs(step, 4, 2, 64, dtype)
+    inp = step.to("cuda")
+    inp.q_cu = inp.q_cu + 3
+    pad = lambda t: torch.cat([t[:1].expand(3, *t.shape[1:]), t])
+    inp.token_seq, inp.positions = pad(inp.token_seq), pad(inp.positions)
+    inp.kv_lens = inp.kv_lens * torch.tensor([1, 0], dtype=I32).cuda()
+    got = ops.tree_attention(pad(q).cuda(), k.cuda(), v.cuda(), inp, pad(step.tree).cuda(), 0.3).view(13, 4, 64).cpu().double()
+    want, size = oracle.attention(q, k, v, step, step.tree, 0.3)
+    assert not got[:3].any() and not got[9:].any()
+    assert ((got[3:9] - want[:6]).abs() <= oracle.attention_bound(q, k, want, size, 0.3, 26, dtype)[:6]).all()
+
+
 def test_tree_attention_places_past_32_bits():
     """A cache of more than 2^32 elements: keys and values at its far end."""
     block, Hkv, D = 128, 16, 128

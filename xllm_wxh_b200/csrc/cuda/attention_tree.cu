@@ -40,6 +40,12 @@ __device__ __forceinline__ Seq load_seq(const Params& p, int s, int per_item) {
   return q;
 }
 
+// whether row t belongs to no sequence, or to one without keys: its output is zero
+__device__ __forceinline__ bool row_is_idle(const Params& p, int t) {
+  const int s = p.token_seq[t];
+  return s < 0 || s >= p.B || t < p.q_cu[s] || t >= p.q_cu[s + 1] || p.kv_lens[s] <= 0;
+}
+
 // keys of the tile at kv0 that row t (at position pos) sees
 __device__ __forceinline__ uint64_t seen_keys(const Params& p, const Seq& q, int t, int pos, int kv0) {
   const int c = q.base - kv0;
@@ -92,9 +98,10 @@ __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15, D = p.D;
   const int seq = blockIdx.x / row_tiles, row0 = (blockIdx.x - seq * row_tiles) * SR, kvh = blockIdx.y, G = p.n_q / p.n_kv;
   const Seq q = load_seq(p, seq, 1);
-  if (splits == 1 && kvh == 0) {                             // rows of no sequence
-    for (long i = max(p.q_cu[p.B], 0) + long(blockIdx.x); i < p.T; i += gridDim.x)
-      for (int c = tid; c < p.n_q * D; c += kSimtThreads) from_f32(static_cast<T*>(p.out) + i * p.n_q * D + c, 0.f);
+  if (splits == 1 && kvh == 0) {                             // a row at a time: a vote of the warp costs the rest registers and 3 us
+    for (long i = blockIdx.x; i < p.T; i += gridDim.x)
+      if (row_is_idle(p, int(i)))
+        for (int c = tid; c < p.n_q * D; c += kSimtThreads) from_f32(static_cast<T*>(p.out) + i * p.n_q * D + c, 0.f);
   }
   if (row0 >= q.n * G || q.kv_len <= 0) return;
   const int first = q.kv_begin + int(blockIdx.z) * part_keys, last = int(blockIdx.z) == splits - 1 ? q.kv_len : min(q.kv_len, first + part_keys);
@@ -303,7 +310,7 @@ __global__ void __launch_bounds__(128) attention_tree_join_kernel(const Params p
   int parts = 0;
   if (seq >= 0 && seq < p.B) {
     const Seq q = load_seq(p, seq, 1);
-    if (t >= q.q_start && t < q.q_start + q.n) parts = min(splits, (q.kv_len - q.kv_begin + part_keys - 1) / part_keys);
+    if (t >= q.q_start && t < q.q_start + q.n && q.kv_len > 0) parts = min(splits, (q.kv_len - q.kv_begin + part_keys - 1) / part_keys);
   }
   // a lane's share of the (at most kMaxParts) parts
   const size_t pitch = size_t(p.T) * p.n_q;
@@ -808,11 +815,14 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
     const float sc = p.scale_log2;
     auto group_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory"); };
     auto both_sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
-    // rows of no sequence
-    {
-      const int behind = max(a.q_cu[a.B], 0), width = a.n_q * a.D;
-      for (long t = long(behind) + blockIdx.x; t < a.T; t += gridDim.x)
-        for (int c = tid - 96; c < width / 8; c += 256) reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + t * width)[c] = make_uint4(0, 0, 0, 0);
+    // idle rows: every thread looks at one of this CTA's share, a warp clears what its lanes found
+    for (long t0 = blockIdx.x; t0 < a.T; t0 += 256l * gridDim.x) {
+      const long t = t0 + (tid - 96l) * gridDim.x;
+      for (uint32_t todo = __ballot_sync(0xffffffffu, t < a.T && row_is_idle(a, int(t))); todo; todo &= todo - 1) {
+        const long idle = __shfl_sync(0xffffffffu, t, __ffs(todo) - 1);
+        for (int c = tid & 31; c < a.n_q * a.D / 8; c += 32)
+          reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + idle * a.n_q * a.D)[c] = make_uint4(0, 0, 0, 0);
+      }
     }
     bool ok = true;
     int u0 = 0, count = 0;                                             // units ahead of the piece; tiles of this group so far

@@ -299,7 +299,7 @@ def latent_down(low, q_rank, kv_rank, q_w, kv_w, eps, rot, slots, cache):
 def latent_attention(q, w_uk, w_uv, cache, inp, rot, scale, dim):
     """Attention over cached latents in absorbed form.  q [T, H, dim + rot_dim] (unrotated part first), w_uk [H, kv_rank, dim],
     w_uv [H, vdim, kv_rank], cache of `latent_down`.  Returns [T, H * vdim]."""
-    import torch
+    _no_tree(inp)
     T, H, _ = q.shape
     C, row = w_uk.shape[1], cache.shape[-1]
     if q.is_cuda and _cuda().mla_serves(H, C, row - C, q.dtype):
