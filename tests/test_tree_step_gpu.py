@@ -65,6 +65,17 @@ def test_step_rows_past_the_table():
     assert got.slots.tolist() == [7, 1, 2, 3] and got.block_tables.tolist() == [[1, 1]]                     # places past the table: the reserved block
 
 
+@pytest.mark.parametrize("cut", [lambda t: t[:, 3:7], lambda t: t[:1, 3:7].expand(3, 4)])
+def test_step_rows_columns_of_a_wider_table(cut):
+    """Places past the columns that were given are past the table, whatever lies behind them in memory."""
+    base = torch.arange(1, 25, dtype=I32).view(3, 8)
+    rest = torch.tensor([14, 3, 9], dtype=I32), torch.tensor([2, 0, 1], dtype=I32), torch.tensor([9, 4, 8], dtype=I32)
+    want = ops.step_rows(cut(base), *rest, 24, 4)
+    got = ops.step_rows(cut(base.cuda()), *cuda(rest), 24, 4)
+    for a, b in zip(got[:6], want[:6]):
+        assert torch.equal(a.cpu(), b)
+
+
 # ----------------------------------------------------------------------------- attention
 def check_attention(step, Hq, Hkv, D, dtype, window=-1, tree=None, seed=0, scale=None, change=None, layout="dense"):
     scale = D ** -0.5 if scale is None else scale

@@ -24,14 +24,15 @@ __device__ __forceinline__ long block_sum(long v, long* s) {
 
 // ---------------------------------------------------------------- step_rows
 struct RowsParams {
-  const int* tables;            // [pool, table_ld]
+  const int* tables;            // [pool, columns], rows table_ld apart
   const int* lens;              // [pool]
   const int* seqs;              // [B] rows of the pool (outside: no sequence)
   const int* counts;            // [B]
   const int* parents;           // [n_rows] or null
   int *positions, *slots, *token_seq, *q_cu, *kv_lens, *block_tables;
   unsigned long long* tree;     // [n_rows, words] or null
-  int pool, table_ld, B, n_rows, max_q, max_blocks, block_size, words, per_cta, table_parts, vectors;
+  int pool, columns, B, n_rows, max_q, max_blocks, block_size, words, per_cta, table_parts, vectors;
+  long table_ld;
 };
 
 // blockIdx.y = sequence (B: the rows behind the last one); blockIdx.x = a part of `per_cta` entries of its table, or behind those a part of
@@ -99,7 +100,7 @@ __global__ void __launch_bounds__(kThreads) step_rows_kernel(const RowsParams p)
   if (part == 0 && tid == 0) p.kv_lens[b] = len + n;
   auto slot_of = [&](long at, int t) {
     const long blk = at / p.block_size;
-    return blk < p.table_ld ? from[blk] * p.block_size + int(at % p.block_size) : t % p.block_size;   // past the table: the reserved block
+    return blk < p.columns ? from[blk] * p.block_size + int(at % p.block_size) : t % p.block_size;   // past the table: the reserved block
   };
   if (!p.parents) {
     const int hi = min(lo + p.per_cta, n);
@@ -233,10 +234,10 @@ __global__ void __launch_bounds__(kThreads) accept_tree_kernel(const __grid_cons
 }  // namespace xl_ts
 
 XL_API int xl_step_rows(const void* tables, const void* lens, const void* seqs, const void* counts, const void* parents, void* positions,
-                        void* slots, void* token_seq, void* q_cu, void* kv_lens, void* block_tables, void* tree, int pool, int table_ld, int B,
+                        void* slots, void* token_seq, void* q_cu, void* kv_lens, void* block_tables, void* tree, int pool, int columns, long table_ld, int B,
                         int n_rows, int max_q, int max_blocks, int block_size, int words, void* stream) {
   using namespace xl_ts;
-  if (B < 0 || B > 65534 || n_rows < 0 || max_q < 1 || max_blocks < 0 || max_blocks > table_ld || block_size < 1 || pool < 0) return -2;
+  if (B < 0 || B > 65534 || n_rows < 0 || max_q < 1 || max_blocks < 0 || max_blocks > columns || table_ld < 0 || block_size < 1 || pool < 0) return -2;
   if (parents && (max_q > kTreeRows || words != (max_q + 63) / 64)) return -2;
   RowsParams p{};
   p.tables = static_cast<const int*>(tables);
@@ -251,7 +252,7 @@ XL_API int xl_step_rows(const void* tables, const void* lens, const void* seqs, 
   p.kv_lens = static_cast<int*>(kv_lens);
   p.block_tables = static_cast<int*>(block_tables);
   p.tree = static_cast<unsigned long long*>(tree);
-  p.pool = pool; p.table_ld = table_ld; p.B = B; p.n_rows = n_rows; p.max_q = max_q; p.max_blocks = max_blocks;
+  p.pool = pool; p.columns = columns; p.table_ld = table_ld; p.B = B; p.n_rows = n_rows; p.max_q = max_q; p.max_blocks = max_blocks;
   p.block_size = block_size; p.words = parents ? words : 0;
   p.vectors = max_blocks % 4 == 0 && table_ld % 4 == 0 && (reinterpret_cast<uintptr_t>(tables) | reinterpret_cast<uintptr_t>(block_tables)) % 16 == 0;
   // table entries of a CTA: as many as keep all CTAs resident, from two rounds of scalars to four of vectors

@@ -20,7 +20,7 @@ namespace {
 constexpr int64_t kTreeRows = 256;
 
 using StepRowsFn = int (*)(const void*, const void*, const void*, const void*, const void*, void*, void*, void*, void*, void*, void*, void*, int,
-                           int, int, int, int, int, int, int, void*);
+                           int, long, int, int, int, int, int, int, void*);
 using AcceptFn = int (*)(const void*, const void*, const void*, const void*, const void*, const void*, void*, void*, void*, int, int, int, int, int,
                          void**, const int*, const int*, int, int, void*);
 using WorkspaceFn = long (*)(int, int, int, int, int, int, int, int, int, int*);
@@ -69,7 +69,7 @@ py::object step_rows(const Tensor& tables, const Tensor& lens, const Tensor& seq
   const int64_t pool = tables.size(0), B = seqs.numel();
   if (!like(lens, i32, {pool}) || !like(seqs, i32, {B}) || !like(counts, i32, {B}) || (parents && !like(*parents, i32, {n_rows})) || n_rows < 0 ||
       n_rows > INT32_MAX || block < 1 || block > INT32_MAX || max_q < 1 || max_q > INT32_MAX || max_blocks < 0 || max_blocks > tables.size(1) ||
-      B >= 65535 || (parents && max_q > kTreeRows) || tables.stride(0) > INT32_MAX)
+      B >= 65535 || (parents && max_q > kTreeRows) || tables.size(1) > INT32_MAX)
     return py::none();
   const c10::cuda::CUDAGuard guard(tables.device());
   const int64_t words = parents ? (max_q + 63) / 64 : 0;
@@ -80,7 +80,7 @@ py::object step_rows(const Tensor& tables, const Tensor& lens, const Tensor& seq
   int* at = small.data_ptr<int>();
   check(f_step_rows(tables.const_data_ptr(), lens.const_data_ptr(), seqs.const_data_ptr(), counts.const_data_ptr(), ptr(parents), at, at + n_rows,
                     at + 2 * n_rows, at + 3 * n_rows, at + 3 * n_rows + B + 1, out.data_ptr(), tree ? tree->data_ptr() : nullptr, int(pool),
-                    int(tables.stride(0)), int(B), int(n_rows), int(max_q), int(max_blocks), int(block), int(words),
+                    int(tables.size(1)), tables.stride(0), int(B), int(n_rows), int(max_q), int(max_blocks), int(block), int(words),
                     c10::cuda::getCurrentCUDAStream().stream()),
         "xl_step_rows");
   auto part = [&](int64_t from, int64_t n) { return small.as_strided({n}, {1}, from); };
