@@ -243,6 +243,15 @@ def test_accept_tree_refusals():
             ops.accept_tree(**{**ok, **bad})
 
 
+def test_accept_tree_refuses_caches_that_overlap():
+    step = oracle.Step([4], [3], 4)
+    n = step.blocks
+    both = torch.zeros(2 * n, 4, 2)
+    with pytest.raises(AssertionError):
+        ops.accept_tree(acceptance(step, 1), step.inp, step.parents, [both[:n], both[n - 1:]])
+    ops.accept_tree(acceptance(step, 1), step.inp, step.parents, [both[:n], both[n:]])
+
+
 # ----------------------------------------------------------------------------- together
 def test_tree_step_needs_trees():
     r = ops.step_rows(torch.ones(1, 4, dtype=I32), ints(0), ints(0), ints(2), 2, 4)

@@ -533,3 +533,70 @@ def test_a_whole_step_replayed():
             else:
                 assert torch.equal(a.cpu(), b), i
         assert torch.equal(dev[1].cpu(), lens) and torch.equal(dev[12].cpu(), kc) and torch.equal(dev[13].cpu(), vc)
+
+
+# ----------------------------------------------------------------------------- refusals
+def refused(op, ok, bads):
+    op(**ok)
+    for bad in bads:
+        with pytest.raises(AssertionError):
+            op(**{**ok, **bad})
+
+
+def test_refusals():
+    i = lambda *v: torch.tensor(v, dtype=I32).cuda()
+    tables = torch.ones(2, 4, dtype=I32).cuda()
+    refused(ops.step_rows, dict(tables=tables, lens=i(1, 2), seqs=i(0, 1), counts=i(1, 1), n_rows=2, block_size=4, parents=i(-1, -1)),
+            [dict(tables=tables.long()), dict(tables=tables.t()), dict(lens=i(1)), dict(lens=i(1, 2).cpu()), dict(seqs=i(0)), dict(counts=i(1, 1).long()),
+             dict(n_rows=-1), dict(block_size=0), dict(max_q=0), dict(max_blocks=5), dict(parents=i(0)), dict(max_q=257)])
+    step = oracle.Step([4], [3], 16)
+    target = acceptance(step, 1).cuda()
+    q, k, v = (t.cuda() for t in attention_inputs(step, 4, 2, 64, torch.bfloat16))
+    inp, tree = step.to("cuda"), step.tree.cuda()
+    other = lambda **kw: types.SimpleNamespace(**{**vars(inp), **kw})
+    refused(ops.tree_attention, dict(q=q, k_cache=k, v_cache=v, inp=inp, tree=tree, scale=1.0),
+            [dict(q=q.half(), k_cache=k.half(), v_cache=v.half()), dict(q=q.float()), dict(v_cache=v[..., :32].contiguous()), dict(q=q[:, :3]),
+             dict(k_cache=k.transpose(1, 2)), dict(k_cache=k.cpu()), dict(tree=tree.int()), dict(tree=tree[:2]),
+             dict(tree=torch.zeros(3, 5, dtype=torch.int64).cuda()), dict(inp=other(q_cu=inp.q_cu.long())), dict(inp=other(kv_lens=i(1, 2))),
+             dict(inp=other(positions=i(1))), dict(inp=other(max_q=300))])
+    x, cu, f = torch.zeros(3, 40).cuda(), i(0, 3), torch.ones(1).cuda()
+    history, words = (i(1, 2).view(1, 2), i(2), i(1)), torch.ones(1, 2, dtype=I32).cuda()
+    refused(ops.adjust_logits, dict(logits=x, q_cu=cu, history=history, penalties=(f, f, f), tokens=i(1, 2, 3), mask=(words, i(0, 0, 0)),
+                                    bias=(i(0, 1), i(4), f)),
+            [dict(logits=x.half()), dict(logits=x.t()), dict(q_cu=cu.long()), dict(history=None), dict(penalties=None), dict(penalties=(f, f, f.cpu())),
+             dict(tokens=i(1)), dict(tokens=None, parents=i(0, 0, 0)), dict(mask=(words[:, :1], i(0, 0, 0))), dict(mask=(words, i(0))),
+             dict(bias=(i(0, 1, 1), i(4), f)), dict(bias=(i(0, 1), i(4), f.double())), dict(seqs=i(0, 0)), dict(max_q=257), dict(max_q=0)])
+    n = step.blocks
+    caches = torch.zeros(2 * n, 16, 2).cuda()
+    parents = step.parents.cuda()
+    refused(ops.accept_tree, dict(target=target, inp=inp, parents=parents, caches=[caches[:n], caches[n:]]),
+            [dict(target=target.long()), dict(parents=parents[:2]), dict(caches=[caches[:n], caches[n - 1:]]), dict(caches=[caches, caches]),
+             dict(caches=[caches.transpose(0, 1)]), dict(caches=[caches.cpu()]), dict(caches=[torch.zeros(2, 8, 2).cuda()]), dict(max_depth=-1),
+             dict(max_depth=256), dict(inp=other(max_q=300))])
+    torch.cuda.synchronize()
+
+
+def test_allowed_views():
+    """One mask that stands for several by expansion."""
+    V = 100
+    x = torch.randn(4, V)
+    words = torch.randint(-2 ** 31, 2 ** 31 - 1, (1, 4), dtype=I32)
+    of = torch.tensor([0, 2, -1, 1], dtype=I32)
+    want = ops.adjust_logits(x.clone(), torch.tensor([0, 4], dtype=I32), mask=(words.expand(3, 4), of))
+    got = ops.adjust_logits(x.cuda(), torch.tensor([0, 4], dtype=I32).cuda(), mask=(words.cuda().expand(3, 4), of.cuda()))
+    assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_more_rows_than_keys(dtype):
+    """A step whose lengths name fewer keys than rows: the rows' first keys are the tree's, as on the CPU."""
+    step = oracle.Step([0], [5], 16, seed=1)
+    q, k, v = attention_inputs(step, 2, 2, 64, dtype)
+    inp = types.SimpleNamespace(**{**vars(step.inp), "kv_lens": torch.tensor([3], dtype=I32)})
+    want = ops.tree_attention(q, k, v, inp, step.tree, 0.2)
+    there = types.SimpleNamespace(**{**vars(step.to("cuda")), "kv_lens": torch.tensor([3], dtype=I32).cuda()})
+    got = ops.tree_attention(q.cuda(), k.cuda(), v.cuda(), there, step.tree.cuda(), 0.2)
+    # fp32: scores of 64 products below 20 in sum of sizes 2^9 are off by 2^-24 x 2^9 x 8 at most, which the weights take over: 2^-12 of
+    # values below 8.  bf16: the weights' and the result's roundings besides, 2^-8 each and once more for the CPU's
+    bound = 2 ** -9 if dtype is torch.float32 else 2 ** -9 + 3 * 2 ** -8 * 8
+    assert ((got.cpu() - want).abs().float() <= bound).all()

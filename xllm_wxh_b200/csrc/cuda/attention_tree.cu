@@ -30,7 +30,7 @@ struct Seq {
 };
 __device__ __forceinline__ Seq load_seq(const Params& p, int s, int per_item) {
   Seq q;
-  q.q_start = p.q_cu[s];
+  q.q_start = max(p.q_cu[s], 0);
   q.n = min(p.q_cu[s + 1], p.T) - q.q_start;
   q.kv_len = int(min(long(p.kv_lens[s]), long(p.max_blocks) * p.block_size));
   q.base = max(q.kv_len - q.n, 0);
@@ -64,7 +64,7 @@ __device__ __forceinline__ uint64_t seen_keys(const Params& p, const Seq& q, int
       bits = i < p.words ? words[i] >> sh : 0;
       if (sh && i + 1 < p.words) bits |= words[i + 1] << (64 - sh);
     }
-    const int end = q.base + q.n - kv0;
+    const int end = q.kv_len - kv0;
     if (end < 64) bits = end > 0 ? bits & ((1ull << end) - 1) : 0;
     if (p.window > 0 && pos - p.window >= q.base)
       for (uint64_t todo = bits; todo; todo &= todo - 1) {
@@ -1136,9 +1136,10 @@ static SimtPlan simt_plan(int B, int n_q, int n_kv, int max_q, int max_kv, int s
   const long units = long(s.row_tiles) * n_kv * max(B, 1);
   // parts of 64 keys at least, as many as give an SM eight CTAs if all sequences were as long as the longest
   s.splits = int(max(1l, min(min(long(max_kv + 63) / 64, long(xl_at::kMaxParts)), 8l * sms / units)));
-  s.part_keys = (max(max_kv, 1) + s.splits - 1) / s.splits;
+  max_kv = min(max(max_kv, 1), 0x7fffffff - 4096);
+  s.part_keys = (max_kv + s.splits - 1) / s.splits;
   s.part_keys = (s.part_keys + 63) / 64 * 64;
-  s.splits = (max(max_kv, 1) + s.part_keys - 1) / s.part_keys;
+  s.splits = (max_kv + s.part_keys - 1) / s.part_keys;
   return s;
 }
 
@@ -1187,6 +1188,7 @@ XL_API int xl_attention_tree(const void* q, const void* k_cache, const void* v_c
     if (B < 1 || !workspace || !tc_serves(q, k_cache, v_cache, block_size, n_q, n_kv, D, q_row, q_head, scale, f32)) return -2;
     const bool pair = long(max_q) * (n_q / n_kv) > BQ;
     const int ctas = tc_ctas(T, B, n_q, n_kv, max_kv, sms);
+    if (p.num_slots > 0x7fffffffl) return -2;
     // the kernel counts its work in 32 bits
     if ((long(B) + long(T) * (n_q / n_kv) / BQ) * n_kv * (long(max_blocks) * block_size / BKV + 2 + kItemCost) > 0x7fffffffl) return -2;
     TcParams t{};

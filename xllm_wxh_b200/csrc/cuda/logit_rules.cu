@@ -399,7 +399,7 @@ XL_API int xl_adjust_logits(void* logits, int f32, int S, int V, long ld, const 
                             const void* bias_ids, const void* bias_values, int n_bias, const void* words, int words_ld, int n_masks,
                             const void* mask_of, void* stream) {
   using namespace xl_lr;
-  if (S < 0 || V < 1 || B < 0 || max_q < 1 || (tokens && max_q > kPathRows) || (words && words_ld < (V + 31) / 32)) return -2;
+  if (S < 0 || V < 1 || B < 0 || max_q < 1 || (tokens && max_q > kPathRows) || V > (1 << 30) || words_ld < 0) return -2;
   if (S == 0) return 0;
   Params p{};
   p.logits = logits;
@@ -430,6 +430,7 @@ XL_API int xl_adjust_logits(void* logits, int f32, int S, int V, long ld, const 
   // rows of a sequence over several CTAs (each counts the history again), as long as there are SMs without one; windows, where
   // histories are long enough to need several
   p.row_parts = B > 0 ? max(1, min(min(max_q, S), 2 * sms / B)) : 1;
+  p.row_parts = max(p.row_parts, (min(max_q, S) >> 18) + 1);                       // rows of a CTA times its table's entries count in 32 bits
   p.parts = B > 0 && text && text_cap > 4l * p.slots ? max(1, min(text_cap / p.slots + 1, 2 * sms / (B * p.row_parts))) : 1;
   // a row's mask over CTAs of eight warps, two times 32 words a warp: in more CTAs their start costs open rows more, in fewer what is
   // written at a time lies further apart (1024 rows of 152064 fp32: 99 us with one, 102 with two, 107 with four, 122 with nineteen)

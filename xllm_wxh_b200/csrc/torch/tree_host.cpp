@@ -8,8 +8,11 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
+#include <optional>
 #include <string>
 #include <unordered_map>
+#include <utility>
 #include <vector>
 
 namespace py = pybind11;
@@ -101,9 +104,10 @@ py::object tree_attention(Tensor q, const Tensor& k, const Tensor& v, const Tens
     return py::none();
   const c10::cuda::CUDAGuard guard(q.device());
   const Tensor out = at::empty({T, Hq * D}, q.options());
-  // no tensor-core kernel: for scores that do not grow with the product, nor where the caches lie off 16-byte boundaries
+  // no tensor-core kernel: for scores that do not grow with the product, nor where the caches lie off 16-byte boundaries or have more
+  // places than a copy's coordinate counts
   const auto address = [](const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()); };
-  const bool f32 = type == at::kFloat, plain = f32 || !(scale > 0) || B == 0 || (address(k) | address(v)) % 16 != 0;
+  const bool f32 = type == at::kFloat, plain = f32 || !(scale > 0) || B == 0 || (address(k) | address(v)) % 16 != 0 || blocks * block > INT32_MAX;
   int tc = 0;
   const long size = f_workspace(int(T), int(B), int(block), int(Hq), int(Hkv), int(D), plain, int(max_q), int(max_kv), &tc);
   if (q.stride(2) != 1 || (tc && (q.stride(1) < 1 || q.stride(0) < 1 || q.stride(1) % 8 || q.stride(0) % std::max<int64_t>(8, q.stride(1)) ||
@@ -126,7 +130,7 @@ py::object adjust_logits(const Tensor& logits, const Tensor& q_cu, const Opt& se
   const auto i32 = at::kInt, f32 = at::kFloat, type = logits.scalar_type();
   if (logits.dim() != 2 || (type != f32 && type != at::kBFloat16) || q_cu.dim() != 1 || q_cu.numel() < 1) return py::none();
   const int64_t S = logits.size(0), V = logits.size(1), B = q_cu.numel() - 1;
-  if (V < 1 || (logits.stride(1) != 1 && V > 1) || (logits.stride(0) < V && S > 1) || S > INT32_MAX || V > INT32_MAX - 4096 || !like(q_cu, i32, {B + 1}))
+  if (V < 1 || (logits.stride(1) != 1 && V > 1) || (logits.stride(0) < V && S > 1) || S > INT32_MAX || V > (1 << 30) || !like(q_cu, i32, {B + 1}))
     return py::none();
   int64_t pool = B;
   if (text) {
@@ -171,7 +175,9 @@ py::object accept_tree(const Tensor& target, const Tensor& tokens, const Tensor&
     return py::none();
   std::vector<void*> at;
   std::vector<int> rows, blocks;
+  std::vector<std::pair<uintptr_t, uintptr_t>> held;                   // first byte of a cache, the one behind its last
   uintptr_t all = 0;
+  held.reserve(caches.size());
   at.reserve(caches.size());
   rows.reserve(caches.size());
   blocks.reserve(caches.size());
@@ -183,12 +189,14 @@ py::object accept_tree(const Tensor& target, const Tensor& tokens, const Tensor&
     at.push_back(c.data_ptr());
     rows.push_back(int(row));
     blocks.push_back(int(c.size(0)));
-    all |= reinterpret_cast<uintptr_t>(c.data_ptr()) | uintptr_t(row);
+    const auto first = reinterpret_cast<uintptr_t>(c.data_ptr());
+    held.emplace_back(first, first + c.nbytes());
+    all |= first | uintptr_t(row);
   }
-  // a cache may be named once
-  std::vector<void*> sorted = at;
-  std::sort(sorted.begin(), sorted.end());
-  if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end()) return py::none();
+  // no memory twice: it would move twice
+  std::sort(held.begin(), held.end());
+  for (size_t i = 1; i < held.size(); ++i)
+    if (held[i].first < held[i - 1].second) return py::none();
   // the widest unit that divides every cache's rows and address
   const int unit = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
   for (int& r : rows) r /= unit;

@@ -471,7 +471,7 @@ def accept_tree(target, inp, parents, caches=(), max_depth=None):
     tokens, parents as in `step_rows`; row 0 of a sequence is its last token, which counts as agreed.  From there the path goes to the
     first row that follows with the target's token, up to max_depth rows (default: inp.max_q - 1).  Returns (out [B, max_depth + 1]: the
     target's tokens along the path, then -1; accepted [B]: drafted rows on the path; path [B, max_depth + 1]: their numbers, then -1).
-    In every tensor of `caches` ([blocks, block, ...], contiguous, no tensor twice) the path's rows move to the positions behind the
+    In every tensor of `caches` ([blocks, block, ...], contiguous, no memory twice) the path's rows move to the positions behind the
     sequence's earlier tokens, which then has 1 + accepted more; the other drafted rows' places hold what they held."""
     depth = max(0, inp.max_q - 1) if max_depth is None else max_depth
     if target.is_cuda:
@@ -491,7 +491,8 @@ def accept_tree(target, inp, parents, caches=(), max_depth=None):
     assert 0 <= depth < TREE_MAX_ROWS and B < 65536
     for c in caches:
         assert c.is_contiguous() and c.dim() >= 2 and c.shape[1] == block and c.get_device() == dev, "caches: [blocks, block, ...], contiguous"
-    assert len({c.data_ptr() for c in caches if c.numel()}) == sum(c.numel() > 0 for c in caches), "a cache may be named once"
+    held = sorted((c.data_ptr(), c.data_ptr() + c.nbytes) for c in caches if c.numel())
+    assert all(a[1] <= b[0] for a, b in zip(held, held[1:])), "caches: no memory twice"
     if target.is_cuda:
         _amiss("accept_tree")
     return ref.accept_tree(target, inp, parents, caches, depth)

@@ -837,20 +837,20 @@ def tree_attention(q, k_cache, v_cache, inp, tree, scale: float, window: int) ->
     out = torch.zeros(T, Hq, D, dtype=q.dtype)
     cu = inp.q_cu.tolist()
     for i in range(inp.n_seqs):
-        a, n, L = cu[i], cu[i + 1] - cu[i], int(inp.kv_lens[i])
+        a, n, L = cu[i], cu[i + 1] - cu[i], min(int(inp.kv_lens[i]), inp.block_tables.shape[1] * block)
         if n <= 0 or L <= 0:
             continue
         blocks = inp.block_tables[i, :-(-L // block)].long()
         k = k_cache.index_select(0, blocks).reshape(-1, Hkv, D)[:L].float()
         v = v_cache.index_select(0, blocks).reshape(-1, Hkv, D)[:L].float()
         pos = inp.positions[a:a + n].long()
-        base = L - n
+        base = max(L - n, 0)
         see = torch.zeros(n, L, dtype=torch.bool)
         see[:, :base] = True
-        for j in range(min(n, 64 * tree.shape[1])):
+        for j in range(min(n, 64 * tree.shape[1], L)):
             see[:, base + j] = (tree[a:a + n, j // 64] >> (j % 64) & 1).bool()
         if window > 0:
-            see &= torch.cat([torch.arange(base), pos])[None] > pos[:, None] - window
+            see &= torch.cat([torch.arange(base), pos[:L - base]])[None] > pos[:, None] - window
         s = torch.einsum("nhd,lhd->hnl", q[a:a + n].float(), k.repeat_interleave(Hq // Hkv, 1)) * scale
         s = s.masked_fill(~see[None], float("-inf"))
         top = s.amax(-1, keepdim=True)
