@@ -75,6 +75,7 @@ py::object step_rows(const Tensor& tables, const Tensor& lens, const Tensor& seq
       B >= 65535 || (parents && max_q > kTreeRows) || tables.size(1) > INT32_MAX)
     return py::none();
   const c10::cuda::CUDAGuard guard(tables.device());
+  const at::AutoDispatchBelowADInplaceOrView fresh;                    // the parts of an allocation are outputs of their own, no views
   const int64_t words = parents ? (max_q + 63) / 64 : 0;
   // one allocation for the small outputs
   const Tensor small = ints(tables, {3 * n_rows + 2 * B + 1}), out = ints(tables, {B, max_blocks});
@@ -201,12 +202,16 @@ py::object accept_tree(const Tensor& target, const Tensor& tokens, const Tensor&
   const int unit = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
   for (int& r : rows) r /= unit;
   const c10::cuda::CUDAGuard guard(target.device());
-  const Tensor out = ints(target, {B, depth + 1}), path = ints(target, {B, depth + 1}), accepted = ints(target, {B});
+  const at::AutoDispatchBelowADInplaceOrView fresh;
+  // one allocation for the outputs
+  const Tensor all_out = ints(target, {B * (2 * depth + 3)});
+  int* const o = all_out.data_ptr<int>();
   check(f_accept(target.const_data_ptr(), tokens.const_data_ptr(), parents.const_data_ptr(), q_cu.const_data_ptr(), kv_lens.const_data_ptr(),
-                 tables.const_data_ptr(), out.data_ptr(), accepted.data_ptr(), path.data_ptr(), int(T), int(B), int(tables.size(1)), int(block), int(depth),
+                 tables.const_data_ptr(), o, o + 2 * B * (depth + 1), o + B * (depth + 1), int(T), int(B), int(tables.size(1)), int(block), int(depth),
                  at.data(), rows.data(), blocks.data(), int(at.size()), unit, c10::cuda::getCurrentCUDAStream().stream()),
         "xl_accept_tree");
-  return py::make_tuple(out, accepted, path);
+  auto rows_of = [&](int64_t from) { return all_out.as_strided({B, depth + 1}, {depth + 1, 1}, from); };
+  return py::make_tuple(rows_of(0), all_out.as_strided({B}, {1}, 2 * B * (depth + 1)), rows_of(B * (depth + 1)));
 }
 
 }  // namespace

@@ -330,9 +330,15 @@ TREE_MAX_ROWS = ref.TREE_MAX_ROWS
 StepRows = ref.StepRows
 
 
+_tree_cuda = None
+
+
 def _tree():
-    from . import tree_cuda
-    return tree_cuda
+    global _tree_cuda
+    if _tree_cuda is None:
+        from . import tree_cuda
+        _tree_cuda = tree_cuda
+    return _tree_cuda
 
 
 def _amiss(name):

@@ -10,12 +10,12 @@ import torch
 from . import cuda_ops
 from .reference import StepRows
 
-_host = None
+_host = _timed = None
 _ENTRIES = ("xl_step_rows", "xl_accept_tree", "xl_attention_tree_workspace", "xl_attention_tree", "xl_adjust_logits")
 
 
 def host():
-    global _host
+    global _host, _timed
     if _host is None:
         L = cuda_ops.lib()
         real = getattr(L, "_real", L)
@@ -24,19 +24,18 @@ def host():
         except ImportError as e:
             raise RuntimeError("_tree_host is missing: run `python -m xllm_wxh_b200.build_ext` (needs g++)") from e
         h.bind({name: ctypes.cast(getattr(real, name), ctypes.c_void_p).value for name in _ENTRIES})
-        _host = h
+        _host, _timed = h, cuda_ops.kernel_timing()
     return _host
 
 
 def _call(name, launches, *args):
     f = getattr(_host or host(), name)
-    timed = cuda_ops.kernel_timing()
-    if timed is not None and timed.enabled and not torch.cuda.is_current_stream_capturing():
+    if _timed is not None and _timed.enabled and not torch.cuda.is_current_stream_capturing():
         e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         e0.record()
         out = f(*args)
         e1.record()
-        timed.records.append(("xl_" + name, e0, e1))
+        _timed.records.append(("xl_" + name, e0, e1))
     else:
         out = f(*args)
     if out is not None:
