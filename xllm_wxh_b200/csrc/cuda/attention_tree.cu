@@ -80,7 +80,9 @@ __device__ __forceinline__ uint64_t seen_keys(const Params& p, const Seq& q, int
 // fp32, and bf16 of the sizes that the tensor-core kernel does not take.  One CTA = (sequence, 32 rows of a key head's query heads times
 // nodes, key head, part of the keys): 32 keys at a time go through shared memory as fp32, a thread computes 4 rows x 2 keys of the
 // scores and 4 rows x 4 NC columns of the sums, so that the multiply-adds bound it rather than shared memory; parts of the keys
-// keep the SMs busy when there are few rows, and are joined by a second kernel.
+// keep the SMs busy when there are few rows, and are joined by a second kernel.  Scores, weights and sums stay fp32; only the result is
+// rounded.  8 trees of 3 to 12 rows, 14 query heads for 2 key heads of 64 columns, up to 2000 keys in fp32: 28 us (floor of the bytes 1.4),
+// two tiles of keys a CTA, of which loads through the table, latency of 4 x 2 products and the join (4 us) are all of it.
 constexpr int SR = 32, SK = 32, kSimtThreads = 128, kMaxParts = 64;
 template <int NC> struct SimtSmem {
   static constexpr int DP = 64 * NC, PITCH = DP + 4;         // 16 rows apart lie in 16 banks
@@ -424,6 +426,17 @@ int launch_simt(const Params& p, int row_tiles, int splits, int part_keys, float
 //               An item of two row tiles gives each group one; otherwise the groups take the key tiles in turn for the same rows, each
 //               with its own O, and join at the end of a piece: a single group could not keep up with memory.
 // A warp's products run in the order of their issue, so S of a tile may overwrite P of the tile two before as soon as that one's P V is issued.
+//
+// Measured (times of single calls; figures in parentheses under the power cap of calls in a long row):
+//   64 trees of 9 to 32 rows, 32 query heads for 8 of 128 columns, contexts of 300 to 8192: 205 us, 1.14 GB at 5.6 TB/s, 0.85 of a copy's
+//   bandwidth (251 us); 16 trees of 64 rows, 64 heads for 8, contexts of 16000 to 32704: 890 us, 920 TFLOP/s, 0.56 of cuBLAS (1026 us):
+//   per 64 keys of 256 rows the products take 1280 cycles (S is issued at 48 cycles a step of 16, where N = 128 would take 64 for twice
+//   the columns), the exponentials 1024, the chain of score, maximum, weight and product of a tile about 2000;
+//   one tree of 16 rows over 1000 keys: 14.0 us, of which launch, first loads and the join are 9.
+//   Earlier forms at 64 x 32 rows: fp32 pipe 97 ms, P through shared memory 273 us, without pieces published by the producer 215 us.
+//   Tried without gain: two threads a row, every eighth exponential as a polynomial, turns between the groups, 144 CTAs by head.
+//
+// Roundings to bf16: P (2^-8 of each weight at most, with the sum taken of the unrounded ones in fp32) because the products take bf16, and the result.
 //
 // Masks: keys ahead of the tree are seen by all rows (within the window), the tree's by the row's words; only tiles that hold either
 // border look at them.  There, values behind the last row are cleared, and values that are not finite are taken out of the tile and
@@ -1044,7 +1057,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
 }
 
 // Joins the partials of the item that ends in CTA blockIdx.x's first piece: o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i.
-// Four parts at a time are fetched together, so that the chain of loads is short.
+// Bound by the latency of the loads (from L2), so four parts at a time are fetched together and 16 CTAs share an item: behind a step of 16
+// rows and 1000 keys it takes 3.4 us, 1.3 of them the launch (4.3 with 8 CTAs an item; eight parts at a time or 32 CTAs gain nothing more).
 template <int QS, int NQ>
 __global__ void __launch_bounds__(128) attention_tree_merge_kernel(const TcParams p) {
   using C = Cfg<QS, NQ>;
@@ -1107,7 +1121,7 @@ int launch_tc(const TcParams& p, const CUtensorMap& q, const CUtensorMap& k, con
   if (cudaGetLastError() != cudaSuccess) return -1;
   if (ctas == 1) return 0;                                             // nothing was split
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(ctas, 8);
+  cfg.gridDim = dim3(ctas, 16);                                        // an item over 16 CTAs: short chains of loads
   cfg.blockDim = dim3(128);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];

@@ -5,10 +5,15 @@
 // added; ids that the row's mask forbids become -inf.  Everything is computed in fp32 and rounded once.
 //
 // Two kernels that never write the same logit, so that they may run side by side:
-//   masks    : (row, columns) - writes -inf where the mask forbids and reads no logit; bound by the bytes written;
+//   masks    : (row, columns) - writes -inf where the mask forbids and reads no logit; bound by the bytes written.  1024 rows of 152064 fp32
+//              logits, seven of ten forbidden: 100 us alone, about 440 MB (67 us at a copy's rate).  Single open ids among forbidden
+//              ones leave sectors that are written in part, and these keep it from that rate;
 //   penalties: (sequence, part, rows) - counts the history's ids in a table in shared memory, so that nothing of the history has to be
 //              counted and sent by the host, and touches only the logits whose ids are in it (one sector each); forbidden ids are left
-//              to the other kernel.  Bound by the latency of a few dependent loads when there are few rows.
+//              to the other kernel.  Bound by the latency of a few dependent loads and of the shared-memory counts when there are few rows:
+//              256 rows with histories of 50 to 3100 ids take 18.5 us, where the bytes alone would take 2.6.
+// Both together, for 64 sequences of 16 rows with histories of 200 to 8000 ids: 131 us (masks 100; penalties 49 alone, of which 31 do not
+// hide behind the masks), and 7.6 ms written as a row's torch calls.
 // The ids that a CTA has to do with (history, path, biases) are marked in a bitmap of the vocabulary; an id's rank in it is its place in
 // the table of counts, so that the table is as long as there are distinct ids, nothing is probed for, and the logits are visited in
 // the order of their addresses.  More ids than the table holds are taken window by window, larger vocabularies slice by slice.  Counts
