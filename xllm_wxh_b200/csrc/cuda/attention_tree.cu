@@ -428,13 +428,15 @@ int launch_simt(const Params& p, int row_tiles, int splits, int part_keys, float
 // A warp's products run in the order of their issue, so S of a tile may overwrite P of the tile two before as soon as that one's P V is issued.
 //
 // Measured (times of single calls; figures in parentheses under the power cap of calls in a long row):
-//   64 trees of 9 to 32 rows, 32 query heads for 8 of 128 columns, contexts of 300 to 8192: 205 us, 1.14 GB at 5.6 TB/s, 0.85 of a copy's
-//   bandwidth (251 us); 16 trees of 64 rows, 64 heads for 8, contexts of 16000 to 32704: 890 us, 920 TFLOP/s, 0.56 of cuBLAS (1026 us):
+//   64 trees of 9 to 32 rows, 32 query heads for 8 of 128 columns, contexts of 300 to 8192: 196 us, 1.14 GB at 5.8 TB/s, 0.88 of a copy's
+//   bandwidth; 16 trees of 64 rows, 64 heads for 8, contexts of 16000 to 32704: 830 us, 985 TFLOP/s, 0.60 of cuBLAS:
 //   per 64 keys of 256 rows the products take 1280 cycles (S is issued at 48 cycles a step of 16, where N = 128 would take 64 for twice
-//   the columns), the exponentials 1024, the chain of score, maximum, weight and product of a tile about 2000;
-//   one tree of 16 rows over 1000 keys: 14.0 us, of which launch, first loads and the join are 9.
+//   the columns), the exponentials 1024, a softmax thread's own chain for a tile about 2200, in which code that is rarely run (masks,
+//   values that are not finite, rescaling) is kept out of the way and the piece's numbers in registers (935 us otherwise);
+//   one tree of 16 rows over 1000 keys: 13.9 us, of which launch, first loads and the join are 9.
 //   Earlier forms at 64 x 32 rows: fp32 pipe 97 ms, P through shared memory 273 us, without pieces published by the producer 215 us.
-//   Tried without gain: two threads a row, every eighth exponential as a polynomial, turns between the groups, 144 CTAs by head.
+//   Tried without gain: the next tile's scores fetched while a tile's weights are stored (registers spill), two threads a row, every eighth
+//   exponential as a polynomial, turns between the groups, 144 CTAs by head.
 //
 // Roundings to bf16: P (2^-8 of each weight at most, with the sum taken of the unrounded ones in fp32) because the products take bf16, and the result.
 //
@@ -455,10 +457,6 @@ struct Piece {
   int seq, head, node0, j0, nt;            // node0: first node of the piece's rows; its key tiles j0 .. j0 + nt - 1 (0: no more pieces)
   int pair, whole, slot;                   // pair: two row tiles; slot: of its partials
   __device__ __forceinline__ int key0(int j) const { return q.kv_begin + (j0 + j) * BKV; }
-  // tiles in which some row may see only a part: the window's border, the tree, the end
-  __device__ __forceinline__ bool partly(const Params& p, int kv0) const {
-    return kv0 + BKV > q.base || (p.window > 0 && kv0 < q.base + q.n - p.window);
-  }
   __device__ __forceinline__ int tile_number(int kv0) const {        // of such a tile among its item's
     return kv0 + BKV > q.base ? min(8 + (kv0 - q.base / BKV * BKV) / BKV, 15) : min((kv0 - q.kv_begin) / BKV, 7);
   }
@@ -856,12 +854,15 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
       const int pos = valid && a.window > 0 ? a.positions[t] : 0;
       float m_ref = -INFINITY, l_run = 0.f;
       int done = 0;                                                    // tiles of this group in this piece
+      // tiles up to the window's border and from the tree's first on are seen in part (in registers: the piece itself is read again each time)
+      const int first_key = x.key0(0);
+      const int ahead = a.window > 0 ? (x.q.base + x.q.n - a.window - first_key + BKV - 1) / BKV : 0, behind = (x.q.base - first_key) / BKV;
       // (a group whose wait ran out goes on without waiting, so that the others still meet it at the barriers)
       for (int j = pair ? 0 : g; j < nt; j += pair ? 1 : 2, ++done, ++count) {
-        const int b = count & 1, kv0 = x.key0(j);
+        const int b = count & 1, kv0 = first_key + j * BKV;
         if (ok && !__all_sync(0xffffffffu, mbar_wait(&bars->s_full[g][b], (count >> 1) & 1))) ok = false;
         tc_fence_after();
-        const bool partly = x.partly(a, kv0);
+        const bool partly = j < ahead || j >= behind;
         if (warp_valid) {
           uint32_t s0[32], s1[32];
           tmem_ld_32x32(t_s + b * 64, s0);
@@ -873,7 +874,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
             v[c] = __uint_as_float(s0[c]);
             v[32 + c] = __uint_as_float(s1[c]);
           }
-          if (partly) {
+          if (__builtin_expect(partly, 0)) {
             const uint64_t see = valid ? seen_keys(a, x.q, t, pos, kv0) : 0;
             const uint32_t lo = uint32_t(see), hi = uint32_t(see >> 32);
 #pragma unroll
@@ -911,11 +912,11 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
           const float2 sum = unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])));
           l_run = l_run * alpha + (sum.x + sum.y);
           tmem_st_32x32(t_s + b * 64, pk);
-          if (done > 0 && __any_sync(0xffffffffu, rescale)) {
+          if (__builtin_expect(done > 0 && __any_sync(0xffffffffu, rescale), 0)) {
             // O is at rest once P V of this group's tile before has run
             if (ok && !__all_sync(0xffffffffu, mbar_wait(&bars->pv_done[g][(count - 1) & 1], ((count - 1) >> 1) & 1))) ok = false;
             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < DV; c += 32) {
               uint32_t o[32];
               tmem_ld_32x32(t_o + c, o);
@@ -927,7 +928,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
           }
           tc_wait_st();
         }
-        if (partly && owner == g) {
+        if (__builtin_expect(partly && owner == g, 0)) {
           // two threads look at the values of one key
           const int u = u0 + v_unit(j, lag, nt), st = u % U, key = gt >> 1;
           if (ok && !__all_sync(0xffffffffu, mbar_wait(&bars->full[st], (u / U) & 1))) ok = false;
@@ -953,7 +954,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
           fence_proxy_async_smem();
           if (!pair) group_sync();
         }
-        if (partly && pair) both_sync();                               // the other group's products wait for the values too
+        if (__builtin_expect(partly && pair, 0)) both_sync();                               // the other group's products wait for the values too
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->p_full[g][b]);
