@@ -427,7 +427,7 @@ int launch_simt(const Params& p, int row_tiles, int splits, int part_keys, float
 //               with its own O, and join at the end of a piece: a single group could not keep up with memory.
 // A warp's products run in the order of their issue, so S of a tile may overwrite P of the tile two before as soon as that one's P V is issued.
 //
-// Measured (times of single calls; figures in parentheses under the power cap of calls in a long row):
+// Measured (single calls; in a long row of calls the power cap lowers the clocks: 238 and 981 us for the first two):
 //   64 trees of 9 to 32 rows, 32 query heads for 8 of 128 columns, contexts of 300 to 8192: 196 us, 1.14 GB at 5.8 TB/s, 0.88 of a copy's
 //   bandwidth; 16 trees of 64 rows, 64 heads for 8, contexts of 16000 to 32704: 830 us, 985 TFLOP/s, 0.60 of cuBLAS:
 //   per 64 keys of 256 rows the products take 1280 cycles (S is issued at 48 cycles a step of 16, where N = 128 would take 64 for twice
