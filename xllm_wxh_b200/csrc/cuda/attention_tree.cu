@@ -427,16 +427,17 @@ int launch_simt(const Params& p, int row_tiles, int splits, int part_keys, float
 //               with its own O, and join at the end of a piece: a single group could not keep up with memory.
 // A warp's products run in the order of their issue, so S of a tile may overwrite P of the tile two before as soon as that one's P V is issued.
 //
-// Measured (single calls; in a long row of calls the power cap lowers the clocks: 238 and 981 us for the first two):
-//   64 trees of 9 to 32 rows, 32 query heads for 8 of 128 columns, contexts of 300 to 8192: 196 us, 1.14 GB at 5.8 TB/s, 0.88 of a copy's
-//   bandwidth; 16 trees of 64 rows, 64 heads for 8, contexts of 16000 to 32704: 830 us, 985 TFLOP/s, 0.60 of cuBLAS:
+// Measured (single calls on two GPUs; in a long row of calls the power cap lowers the clocks: 238 and 981 us for the first two):
+//   64 trees of 9 to 32 rows, 32 query heads for 8 of 128 columns, contexts of 300 to 8192: 196 and 205 us, 1.14 GB at 5.8 TB/s, 0.88 of a copy's
+//   bandwidth; 16 trees of 64 rows, 64 heads for 8, contexts of 16000 to 32704: 830 and 855 us, 985 TFLOP/s, 0.60 of cuBLAS:
 //   per 64 keys of 256 rows the products take 1280 cycles (S is issued at 48 cycles a step of 16, where N = 128 would take 64 for twice
 //   the columns), the exponentials 1024, a softmax thread's own chain for a tile about 2200, in which code that is rarely run (masks,
-//   values that are not finite, rescaling) is kept out of the way and the piece's numbers in registers (935 us otherwise);
+//   values that are not finite, rescaling) is kept out of the way and the piece's numbers in registers (8 % more otherwise);
 //   one tree of 16 rows over 1000 keys: 13.9 us, of which launch, first loads and the join are 9.
 //   Earlier forms at 64 x 32 rows: fp32 pipe 97 ms, P through shared memory 273 us, without pieces published by the producer 215 us.
-//   Tried without gain: the next tile's scores fetched while a tile's weights are stored (registers spill), two threads a row, every eighth
-//   exponential as a polynomial, turns between the groups, 144 CTAs by head.
+//   Tried without gain: the next tile's scores fetched while a tile's weights are stored (8 to 28 % slower, with registers moved from the
+//   other warps to the softmax warps or without), two threads a row, every eighth exponential as a polynomial, turns between the groups,
+//   144 CTAs by head.
 //
 // Roundings to bf16: P (2^-8 of each weight at most, with the sum taken of the unrounded ones in fp32) because the products take bf16, and the result.
 //
