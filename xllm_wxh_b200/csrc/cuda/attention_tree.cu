@@ -448,7 +448,8 @@ int launch_simt(const Params& p, int row_tiles, int splits, int part_keys, float
 constexpr int BQ = 128;
 constexpr int kTcThreads = 352;
 constexpr int Q_SLAB = BQ * 128, KV_SLAB = BKV * 128;
-constexpr int kMaxUnits = 20, kPieces = 8, kItemCost = 3;
+constexpr int kMaxUnits = 20, kPieces = 8;
+constexpr int kItemCost = 3;     // (16 rows, 1000 keys: 13.8 us; 2: 14.3, 5: 14.0; long contexts alike)
 
 __device__ __forceinline__ int item_work(const Seq& q) { return q.key_tiles + kItemCost; }
 // of a key head's items of row tile `plane`
@@ -1213,7 +1214,7 @@ XL_API int xl_attention_tree(const void* q, const void* k_cache, const void* v_c
     t.nodes = BQ / t.group;
     t.box_tokens = min(block_size & -block_size, BKV);
     t.block_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
-    t.min_work = 3;
+    t.min_work = 3;                                         // (16 rows, 1000 keys: 13.8 us; 2: 13.9, 5: 14.7)
     t.scale_log2 = scale * 1.4426950408889634f;
     const int rows = pair ? 256 : 128, DV = (D + 63) / 64 * 64;
     t.ws_o = static_cast<float4*>(workspace);
