@@ -432,7 +432,8 @@ XL_API int xl_adjust_logits(void* logits, int f32, int S, int V, long ld, const 
   // a table that holds any history of the given length; of long ones their distinct ids, which text has far fewer of, at a time
   p.bitmap_words = (min((V + 31) / 32, kMaxWords) + 1) & ~1;
   p.slots = int(min(long(kMaxSlots), ((text ? text_cap : 0) + long(n_bias) + max_q + 31) / 32 * 32));
-  // rows of a sequence over several CTAs (each counts the history again), as long as there are SMs without one; windows, where
+  // rows of a sequence over several CTAs (each counts the history again), as long as an SM has fewer than two (64 sequences of 16 rows
+  // beside their masks: 131 us, with one CTA an SM 146, with three 137); windows, where
   // histories are long enough to need several
   p.row_parts = B > 0 ? max(1, min(min(max_q, S), 2 * sms / B)) : 1;
   p.row_parts = max(p.row_parts, (min(max_q, S) >> 18) + 1);                       // rows of a CTA times its table's entries count in 32 bits
