@@ -1,0 +1,48 @@
+"""Kernels of a step with trees of drafted tokens at the edges of what their documentation allows: empty histories, tables and caches,
+positions of any kind, values that are not finite, vocabularies of several slices."""
+import types
+
+import pytest
+import torch
+
+import oracle_tree as oracle
+from test_tree_step_cpu import attention_inputs, check_rules, rules
+from test_tree_step_gpu import cuda, status      # noqa: F401 (every test reads the status word)
+from xllm_wxh_b200 import ops
+
+pytestmark = pytest.mark.gpu
+I32 = torch.int32
+
+def check_not_finite(step, q, k, v, dtype, scale=1.0):
+    """Numbers come out where the definition has numbers, and nowhere else."""
+    got = ops.tree_attention(q.cuda(), k.cuda(), v.cuda(), step.to("cuda"), step.tree.cuda(), scale).view(q.shape).cpu().double()
+    want, size = oracle.attention(q, k, v, step, step.tree, scale)
+    fine = want.isfinite()
+    assert torch.equal(fine, got.isfinite())
+    longest = max(b + n for b, n in zip(step.before, step.counts))
+    off = (got - want).abs() - oracle.attention_bound(q, k, want, size, scale, longest, dtype)
+    assert not (off[fine] > 0).any()
+    return fine
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("before,at", [(2000, 5), (2000, 1998), (2000, 2001), (20, 5), (20, 21)])
+def test_tree_attention_visible_values_and_scores_that_are_not_finite(before, at, bad, dtype):
+    """A row whose scores are not all numbers, or that sees a value that is not finite, does not become finite because other keys outweigh
+    that one by more than fp32 holds."""
+    step = oracle.Step([before], [3], 16, seed=5)
+    step.tree[:] = 7                                             # every row sees all three
+    q, k, v = attention_inputs(step, 2, 1, 64, dtype)
+    q.fill_(1)
+    k.mul_(0.125)
+    for p in range(at // 64 * 64, min(at // 64 * 64 + 64, before + 3)):
+        k[step.place(0, p)] = -10                                # scores of -640 among keys whose scores are about 0
+    if before < 64:
+        k[step.place(0, 1)] = 0.5                                # one score of 32 among them
+    v[step.place(0, at)][..., 9] = bad
+    fine = check_not_finite(step, q, k, v, dtype)
+    assert not fine[..., 9].any() and fine[..., :9].all()
+    v[step.place(0, at)][..., 9] = 1
+    k[step.place(0, at)][..., 4] = float("nan")
+    assert not check_not_finite(step, q, k, v, dtype).any()

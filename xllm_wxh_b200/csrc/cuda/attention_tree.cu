@@ -326,9 +326,10 @@ __global__ void __launch_bounds__(128) attention_tree_join_kernel(const Params p
   m = warp_max(m);
 #pragma unroll
   for (int i = 0; i < kMaxParts / 32; ++i) {
-    // a part whose row saw nothing has no weight, unless its scores were not numbers
+    // a part whose row saw nothing has no weight, unless its scores were not numbers; one far below the others still makes the sums
+    // NaN if its own are no numbers, as within a part
     const float w = ml[i].x == -INFINITY ? (ml[i].y != 0.f ? 1.f : 0.f) : fast_exp2(ml[i].x - m);
-    l += w != 0.f ? w * ml[i].y : 0.f;
+    l += w * ml[i].y;
     ml[i].x = w;
   }
   l = warp_sum(l);
@@ -356,7 +357,7 @@ __global__ void __launch_bounds__(128) attention_tree_join_kernel(const Params p
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (mine < parts && w != 0.f) o[e] = fmaf(w, x[e], o[e]);
+        if (mine < parts) o[e] = fmaf(w, x[e], o[e]);
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
