@@ -13,6 +13,20 @@ from xllm_wxh_b200 import ops
 pytestmark = pytest.mark.gpu
 I32 = torch.int32
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_adjust_logits_history_without_columns(dtype):
+    """Histories that hold nothing yet: the rows' own tokens are penalised all the same."""
+    r = rules(200, 5, [4, 1, 7], 11, dtype)
+    r.history = (r.history[0][:, :0], torch.zeros_like(r.history[1]), torch.zeros_like(r.history[2]))
+    got = r.logits.cuda()
+    ops.adjust_logits(got, *cuda((r.cu, r.seqs, r.history, r.penalties, r.tokens, r.parents, r.bias, r.mask)), max_q=7)
+    check_rules(r, got.cpu(), dtype)
+    # a pool without requests: every sequence lies outside
+    none = ((r.history[0][:0], r.history[1][:0], r.history[2][:0]), tuple(p[:0] for p in r.penalties))
+    got = r.logits.cuda()
+    ops.adjust_logits(got, *cuda((r.cu, r.seqs, *none, r.tokens, r.parents)), max_q=7)
+    assert torch.equal(got.cpu(), r.logits)
+
 def check_not_finite(step, q, k, v, dtype, scale=1.0):
     """Numbers come out where the definition has numbers, and nowhere else."""
     got = ops.tree_attention(q.cuda(), k.cuda(), v.cuda(), step.to("cuda"), step.tree.cuda(), scale).view(q.shape).cpu().double()

@@ -35,10 +35,10 @@ struct Params {
   int V, S, B, pool, max_q;
   const int* q_cu;              // [B + 1] rows of each sequence
   const int* seqs;              // [B] pool rows (null: the sequence's own number)
-  const int* text;              // [pool, text_ld] (null: no histories)
+  const int* text;              // [pool, text_ld] (null where text_cap is 0)
   long text_ld;
   int text_cap;
-  const int *lens, *prompts;    // [pool]
+  const int *lens, *prompts;    // [pool] (null: no histories)
   const float *rep, *freq, *pres;
   const int* tokens;            // [S] (null: rows have no tokens of their own)
   const int* parents;           // [S] (null: every row follows the one before)
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, 2) penalise_logits_kernel(const Para
   if (unsigned(src) >= unsigned(p.pool) || r0 >= r1) return;
   float rep = 1.f, freq = 0.f, pres = 0.f;
   int given = 0, prompt = 0, e0 = 0, e1 = 0;
-  if (p.text) {
+  if (p.lens) {
     rep = p.rep[src]; freq = p.freq[src]; pres = p.pres[src];
     given = max(p.lens[src], 0);
     prompt = p.prompts[src];
@@ -405,6 +405,7 @@ XL_API int xl_adjust_logits(void* logits, int f32, int S, int V, long ld, const 
                             const void* mask_of, void* stream) {
   using namespace xl_lr;
   if (S < 0 || V < 1 || B < 0 || max_q < 1 || (tokens && max_q > kPathRows) || V > (1 << 30) || words_ld < 0) return -2;
+  if (text_cap < 0 || (lens && text_cap > 0 && !text)) return -2;
   if (S == 0) return 0;
   Params p{};
   p.logits = logits;
@@ -431,17 +432,17 @@ XL_API int xl_adjust_logits(void* logits, int f32, int S, int V, long ld, const 
   const int sms = xl_host::sm_count();
   // a table that holds any history of the given length; of long ones their distinct ids, which text has far fewer of, at a time
   p.bitmap_words = (min((V + 31) / 32, kMaxWords) + 1) & ~1;
-  p.slots = int(min(long(kMaxSlots), ((text ? text_cap : 0) + long(n_bias) + max_q + 31) / 32 * 32));
+  p.slots = int(min(long(kMaxSlots), (text_cap + long(n_bias) + max_q + 31) / 32 * 32));
   // rows of a sequence over several CTAs (each counts the history again), as long as an SM has fewer than two (64 sequences of 16 rows
   // beside their masks: 131 us, with one CTA an SM 146, with three 137); windows, where
   // histories are long enough to need several
   p.row_parts = B > 0 ? max(1, min(min(max_q, S), 2 * sms / B)) : 1;
   p.row_parts = max(p.row_parts, (min(max_q, S) >> 18) + 1);                       // rows of a CTA times its table's entries count in 32 bits
-  p.parts = B > 0 && text && text_cap > 4l * p.slots ? max(1, min(text_cap / p.slots + 1, 2 * sms / (B * p.row_parts))) : 1;
+  p.parts = B > 0 && text_cap > 4l * p.slots ? max(1, min(text_cap / p.slots + 1, 2 * sms / (B * p.row_parts))) : 1;
   // a row's mask over CTAs of eight warps, two times 32 words a warp: in more CTAs their start costs open rows more, in fewer what is
   // written at a time lies further apart (1024 rows of 152064 fp32: 99 us with one, 102 with two, 107 with four, 122 with nineteen)
   const int mask_parts = ((V + 31) / 32 + 1 + 2 * kMaskThreads - 1) / (2 * kMaskThreads);
   auto s = static_cast<cudaStream_t>(stream);
-  const bool penalties = B > 0 && (text || bias_cu);
+  const bool penalties = B > 0 && (lens || bias_cu);
   return f32 ? launch<float>(p, penalties, mask_parts, s) : launch<__nv_bfloat16>(p, penalties, mask_parts, s);
 }
