@@ -60,3 +60,15 @@ def test_tree_attention_visible_values_and_scores_that_are_not_finite(before, at
     v[step.place(0, at)][..., 9] = 1
     k[step.place(0, at)][..., 4] = float("nan")
     assert not check_not_finite(step, q, k, v, dtype).any()
+
+def test_adjust_logits_refuses_parts_that_are_missing():
+    f, i = torch.ones(1, device="cuda"), lambda *v: torch.tensor(v, dtype=I32).cuda()
+    x, words = torch.zeros(3, 40, device="cuda"), torch.zeros(1, 2, dtype=I32, device="cuda")
+    ok = dict(logits=x, q_cu=i(0, 3), history=(i(1, 2).view(1, 2), i(2), i(1)), penalties=(f, f, f), mask=(words, i(-1, -1, -1)), bias=(i(0, 1), i(4), f))
+    for name in ("history", "penalties", "mask", "bias"):
+        for missing in range(len(ok[name])):
+            part = tuple(None if j == missing else t for j, t in enumerate(ok[name]))
+            with pytest.raises(AssertionError):
+                ops.adjust_logits(**{**ok, name: part})
+    assert not x.any()
+    ops.adjust_logits(**ok)

@@ -133,15 +133,18 @@ py::object adjust_logits(const Tensor& logits, const Tensor& q_cu, const Opt& se
   const int64_t S = logits.size(0), V = logits.size(1), B = q_cu.numel() - 1;
   if (V < 1 || (logits.stride(1) != 1 && V > 1) || (logits.stride(0) < V && S > 1) || S > INT32_MAX || V > (1 << 30) || !like(q_cu, i32, {B + 1}))
     return py::none();
+  // what comes in several parts is there as a whole or not at all
+  const bool history = text || lens || prompts || rep || freq || pres, biased = bias_cu || bias_ids || bias_values;
+  if ((history && !(text && lens && prompts && rep && freq && pres)) || (biased && !(bias_cu && bias_ids && bias_values)) || bool(words) != bool(mask_of))
+    return py::none();
   int64_t pool = B;
   if (text) {
-    if (!lens || !prompts || !rep || !freq || !pres) return py::none();
     pool = lens->numel();
     if (text->scalar_type() != i32 || text->dim() != 2 || text->size(0) != pool || (text->stride(1) != 1 && text->size(1) > 1) ||
         text->device() != like.dev || text->size(1) > INT32_MAX || !like(*lens, i32, {pool}) || !like(*prompts, i32, {pool}) ||
         !like(*rep, f32, {pool}) || !like(*freq, f32, {pool}) || !like(*pres, f32, {pool}))
       return py::none();
-  } else if (rep || tokens) {
+  } else if (tokens) {
     return py::none();
   }
   if ((tokens && !like(*tokens, i32, {S})) || (parents && (!tokens || !like(*parents, i32, {S}))) || (seqs && !like(*seqs, i32, {B}))) return py::none();

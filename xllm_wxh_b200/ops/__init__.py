@@ -348,6 +348,7 @@ def _amiss(name):
 
 def _like(t, dtype, shape, dev, name):
     """Checks one argument: element type, sizes, dense, on the device of that number."""
+    assert isinstance(t, torch.Tensor), f"{name}: a tensor, not {type(t).__name__}"
     assert t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous(), \
         f"{name}: {dtype} {tuple(shape)}, contiguous, beside the others; not {t.dtype} {tuple(t.shape)}"
 
@@ -437,6 +438,8 @@ def adjust_logits(logits, q_cu, seqs=None, history=None, penalties=None, tokens=
     B = q_cu.numel() - 1
     _like(q_cu, i32, (B + 1,), dev, "q_cu")
     pool = None
+    for name, parts in (("history", history), ("bias", bias), ("mask", mask)):
+        assert parts is None or all(isinstance(t, torch.Tensor) for t in parts), f"{name}: tensors only"
     if history is not None:
         ids, lens, prompts = history
         pool = lens.numel()
