@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from test_tree_step_cpu import rules
+import oracle_tree as oracle
+from test_tree_step_cpu import attention_inputs, rules
 from xllm_wxh_b200 import ops
 
 
@@ -16,3 +17,19 @@ def test_adjust_logits_refuses_parts_that_are_missing():
             with pytest.raises(AssertionError):
                 ops.adjust_logits(**{**ok, name: part})
     assert torch.equal(r.logits, kept)
+
+
+@pytest.mark.parametrize("window", [1, 40, 150])
+def test_tree_attention_window_with_positions_of_any_kind(window):
+    """A row's position counts as one of its sequence's rows': the nearest one."""
+    step = oracle.Step([0, 5, 64, 200], [9, 30, 3, 64], 16, seed=4, deep=True, junk_tables=False)
+    q, k, v = attention_inputs(step, 4, 2, 16, torch.float32)
+    given = step.inp.positions + torch.randint(-400, 400, (step.T,), generator=torch.Generator().manual_seed(window), dtype=torch.int32)
+    given[3], given[50] = 2 ** 31 - 1, -2 ** 31
+    counts = torch.tensor(step.counts)
+    first = torch.repeat_interleave(torch.tensor(step.before), counts).int()
+    step.inp.positions = given
+    got = ops.tree_attention(q, k, v, step.inp, step.tree, 0.25, window).view(step.T, 4, 16)
+    step.inp.positions = given.clamp(first, first + torch.repeat_interleave(counts, counts).int() - 1)
+    want, size = oracle.attention(q, k, v, step, step.tree, 0.25, window)
+    assert ((got.double() - want).abs() <= oracle.attention_bound(q, k, want, size, 0.25, 264, torch.float32)).all()

@@ -27,6 +27,23 @@ def test_adjust_logits_history_without_columns(dtype):
     ops.adjust_logits(got, *cuda((r.cu, r.seqs, *none, r.tokens, r.parents)), max_q=7)
     assert torch.equal(got.cpu(), r.logits)
 
+@pytest.mark.parametrize("window", [1, 40, 150])
+@pytest.mark.parametrize("D,dtype", [(128, torch.bfloat16), (64, torch.float32)])
+def test_tree_attention_window_with_positions_of_any_kind(window, D, dtype):
+    """A row's position counts as one of its sequence's rows': the nearest one."""
+    step = oracle.Step([0, 5, 64, 200, 700], [9, 30, 3, 64, 12], 16, seed=4, deep=True)
+    q, k, v = attention_inputs(step, 8, 2, D, dtype)
+    given = step.inp.positions + torch.randint(-400, 400, (step.T,), generator=torch.Generator().manual_seed(window), dtype=I32)
+    given[3], given[50] = 2 ** 31 - 1, -2 ** 31
+    first = torch.repeat_interleave(torch.tensor(step.before), torch.tensor(step.counts)).int()
+    last = first + torch.repeat_interleave(torch.tensor(step.counts), torch.tensor(step.counts)).int() - 1
+    step.inp.positions = given
+    inp = step.to("cuda")
+    step.inp.positions = given.clamp(first, last)
+    got = ops.tree_attention(q.cuda(), k.cuda(), v.cuda(), inp, step.tree.cuda(), D ** -0.5, window).view(step.T, 8, D).cpu().double()
+    want, size = oracle.attention(q, k, v, step, step.tree, D ** -0.5, window)
+    assert ((got - want).abs() <= oracle.attention_bound(q, k, want, size, D ** -0.5, 712, dtype)).all()
+
 def check_not_finite(step, q, k, v, dtype, scale=1.0):
     """Numbers come out where the definition has numbers, and nowhere else."""
     got = ops.tree_attention(q.cuda(), k.cuda(), v.cuda(), step.to("cuda"), step.tree.cuda(), scale).view(q.shape).cpu().double()

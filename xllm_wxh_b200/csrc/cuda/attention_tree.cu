@@ -40,6 +40,12 @@ __device__ __forceinline__ Seq load_seq(const Params& p, int s, int per_item) {
   return q;
 }
 
+// Position of row t of the sequence for the window.  It counts as one of the sequence's rows', the nearest: which tiles the window opens,
+// cuts and leaves out goes by base and n alone, so a position outside would open or lose keys by the tile that they lie in.
+__device__ __forceinline__ int row_position(const Params& p, const Seq& q, int t) {
+  return min(max(p.positions[t], q.base), q.base + q.n - 1);
+}
+
 // whether row t belongs to no sequence, or to one without keys: its output is zero
 __device__ __forceinline__ bool row_is_idle(const Params& p, int t) {
   const int s = p.token_seq[t];
@@ -69,7 +75,7 @@ __device__ __forceinline__ uint64_t seen_keys(const Params& p, const Seq& q, int
     if (p.window > 0 && pos - p.window >= q.base)
       for (uint64_t todo = bits; todo; todo &= todo - 1) {
         const int k = __ffsll(todo) - 1;
-        if (p.positions[q.q_start + kv0 + k - q.base] <= pos - p.window) bits &= ~(1ull << k);
+        if (row_position(p, q, q.q_start + kv0 + k - q.base) <= pos - p.window) bits &= ~(1ull << k);
       }
     see |= bits;
   }
@@ -116,7 +122,7 @@ __global__ void __launch_bounds__(kSimtThreads) attention_tree_simt_kernel(const
     const int node = (row0 + 4 * ty + i) / G;
     valid[i] = node < q.n;
     t[i] = q.q_start + (valid[i] ? node : 0);
-    pos[i] = p.window > 0 ? p.positions[t[i]] : 0;
+    pos[i] = p.window > 0 ? row_position(p, q, t[i]) : 0;
   }
   const bool vectors = D % 8 == 0 && (reinterpret_cast<uintptr_t>(p.k_cache) | reinterpret_cast<uintptr_t>(p.v_cache)) % 16 == 0;
   const float scale = p.scale * 1.4426950408889634f;         // scores in the log2 domain
@@ -854,7 +860,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
       const bool valid = node < p.nodes && my_node < x.q.n;
       const bool warp_valid = __any_sync(0xffffffffu, valid);
       const int t = x.q.q_start + (valid ? my_node : 0);
-      const int pos = valid && a.window > 0 ? a.positions[t] : 0;
+      const int pos = valid && a.window > 0 ? row_position(a, x.q, t) : 0;
       float m_ref = -INFINITY, l_run = 0.f;
       int done = 0;                                                    // tiles of this group in this piece
       // tiles up to the window's border and from the tree's first on are seen in part (in registers: the piece itself is read again each time)

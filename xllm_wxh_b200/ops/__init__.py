@@ -389,9 +389,10 @@ def tree_attention(q, k_cache, v_cache, inp, tree, scale, sliding_window=-1):
     """Attention of rows that see their sequence's cached tokens ahead of the step and those of its own rows whose bit is set in `tree`
     (int64 [T, words], as `step_rows` makes it; any set of a sequence's first 64 x words rows will do).  q [T, Hq, D], caches [blocks,
     block, Hkv, D] that hold the step's rows already; `inp` has q_cu, kv_lens, block_tables, token_seq, positions, n_seqs, and max_q and
-    max_kv as bounds.  `sliding_window`: only keys at positions above the row's own - window.  Rows that see nothing and rows of no
-    sequence are zero.  Values that are not finite reach the rows that see them and no others: there the column is not finite either
-    (infinite or NaN, by how small the weight is).  Returns [T, Hq * D].  bf16 or fp32, up to 512 columns a head."""
+    max_kv as bounds.  `sliding_window`: only keys at positions above the row's own - window, where a cached token's position is its
+    place and a row's is inp.positions, brought between those of its sequence's first and last place in the cache (where `step_rows` puts
+    it).  Rows that see nothing and rows of no sequence are zero.  Values that are not finite reach the rows that see them and no others:
+    there the column is not finite either (infinite or NaN, by how small the weight is).  Returns [T, Hq * D].  bf16 or fp32, up to 512 columns a head."""
     if q.is_cuda:
         out = _tree().tree_attention(q, k_cache, v_cache, inp, tree, scale, sliding_window)
         if out is not None:

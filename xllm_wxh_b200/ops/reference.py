@@ -843,8 +843,8 @@ def tree_attention(q, k_cache, v_cache, inp, tree, scale: float, window: int) ->
         blocks = inp.block_tables[i, :-(-L // block)].long()
         k = k_cache.index_select(0, blocks).reshape(-1, Hkv, D)[:L].float()
         v = v_cache.index_select(0, blocks).reshape(-1, Hkv, D)[:L].float()
-        pos = inp.positions[a:a + n].long()
         base = max(L - n, 0)
+        pos = inp.positions[a:a + n].long().clamp(base, base + n - 1)
         see = torch.zeros(n, L, dtype=torch.bool)
         see[:, :base] = True
         for j in range(min(n, 64 * tree.shape[1], L)):
