@@ -33,3 +33,21 @@ def test_tree_attention_window_with_positions_of_any_kind(window):
     step.inp.positions = given.clamp(first, first + torch.repeat_interleave(counts, counts).int() - 1)
     want, size = oracle.attention(q, k, v, step, step.tree, 0.25, window)
     assert ((got.double() - want).abs() <= oracle.attention_bound(q, k, want, size, 0.25, 264, torch.float32)).all()
+
+
+def test_tree_attention_without_table_columns_or_blocks():
+    step = oracle.Step([20, 5], [6, 4], 16, seed=3, spare_rows=2, junk_tables=False)
+    q, k, v = attention_inputs(step, 4, 2, 8, torch.float32)
+    step.inp.block_tables = step.inp.block_tables[:, :0].contiguous()
+    assert not ops.tree_attention(q, k, v, step.inp, step.tree, 0.3).any()
+    step.inp.kv_lens = torch.zeros_like(step.inp.kv_lens)
+    assert not ops.tree_attention(q, k[:0], v[:0], step.inp, step.tree, 0.3).any()
+
+
+def test_tree_attention_refuses_heads_and_blocks_of_nothing():
+    step = oracle.Step([4], [3], 4, junk_tables=False)
+    q, k, v = attention_inputs(step, 4, 2, 8, torch.float32)
+    for bad in [dict(q=q[:, :0]), dict(q=q[..., :0], k=k[..., :0], v=v[..., :0]), dict(k=k[:, :, :0], v=v[:, :, :0]), dict(k=k[:, :0], v=v[:, :0])]:
+        a = {**dict(q=q, k=k, v=v), **bad}
+        with pytest.raises(AssertionError):
+            ops.tree_attention(a["q"], a["k"], a["v"], step.inp, step.tree, 1.0)

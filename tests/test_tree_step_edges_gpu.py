@@ -44,6 +44,41 @@ def test_tree_attention_window_with_positions_of_any_kind(window, D, dtype):
     want, size = oracle.attention(q, k, v, step, step.tree, D ** -0.5, window)
     assert ((got - want).abs() <= oracle.attention_bound(q, k, want, size, D ** -0.5, 712, dtype)).all()
 
+@pytest.mark.parametrize("D,dtype", [(64, torch.bfloat16), (64, torch.float32), (192, torch.bfloat16)])
+def test_tree_attention_without_table_columns_or_blocks(D, dtype):
+    """No place to read from: every row sees nothing."""
+    step = oracle.Step([20, 5], [6, 4], 16, seed=3, spare_rows=2)
+    q, k, v = attention_inputs(step, 4, 2, D, dtype)
+    inp = step.to("cuda")
+    inp.block_tables = inp.block_tables[:, :0].contiguous()
+    assert not ops.tree_attention(q.cuda(), k.cuda(), v.cuda(), inp, step.tree.cuda(), 0.3).any()
+    inp.block_tables, inp.kv_lens = step.inp.block_tables.cuda(), torch.zeros_like(inp.kv_lens)
+    assert not ops.tree_attention(q.cuda(), k[:0].cuda(), v[:0].cuda(), inp, step.tree.cuda(), 0.3).any()
+    none = types.SimpleNamespace(**{**vars(inp), "positions": inp.positions[:0], "token_seq": inp.token_seq[:0], "q_cu": torch.zeros_like(inp.q_cu),
+                                    "block_tables": inp.block_tables[:, :0].contiguous()})
+    assert ops.tree_attention(q[:0].cuda(), k.cuda(), v.cuda(), none, step.tree[:0].cuda(), 0.3).shape == (0, 4 * D)
+
+
+def test_tree_attention_refuses_heads_and_blocks_of_nothing():
+    step = oracle.Step([4], [3], 16)
+    q, k, v = (t.cuda() for t in attention_inputs(step, 4, 2, 64, torch.bfloat16))
+    inp, tree = step.to("cuda"), step.tree.cuda()
+    for bad in [dict(q=q[:, :0]), dict(q=q[..., :0], k=k[..., :0], v=v[..., :0]), dict(k=k[:, :, :0], v=v[:, :, :0]), dict(k=k[:, :0], v=v[:, :0])]:
+        a = {**dict(q=q, k=k, v=v), **bad}
+        with pytest.raises(AssertionError):
+            ops.tree_attention(a["q"], a["k"], a["v"], inp, tree, 1.0)
+
+def test_tree_attention_tables_of_more_places_than_32_bits_count():
+    """Tables so wide that their key tiles, over all sequences and heads, pass 2^31."""
+    step = oracle.Step([300, 0, 41, 7, 100, 64, 65, 1], [5, 1, 9, 0, 3, 2, 2, 16], 8192, seed=3)
+    q, k, v = attention_inputs(step, 16, 8, 8, torch.bfloat16)
+    inp = step.to("cuda")
+    inp.block_tables = torch.zeros(8, 2 ** 19, dtype=I32, device="cuda")
+    inp.block_tables[:, 0] = step.inp.block_tables[:, 0].cuda() % step.blocks
+    got = ops.tree_attention(q.cuda(), k.cuda(), v.cuda(), inp, step.tree.cuda(), 0.3).view(step.T, 16, 8).cpu().double()
+    want, size = oracle.attention(q, k, v, step, step.tree, 0.3)
+    assert ((got - want).abs() <= oracle.attention_bound(q, k, want, size, 0.3, 305, torch.bfloat16)).all()
+
 def check_not_finite(step, q, k, v, dtype, scale=1.0):
     """Numbers come out where the definition has numbers, and nowhere else."""
     got = ops.tree_attention(q.cuda(), k.cuda(), v.cuda(), step.to("cuda"), step.tree.cuda(), scale).view(q.shape).cpu().double()

@@ -49,7 +49,7 @@ __device__ __forceinline__ int row_position(const Params& p, const Seq& q, int t
 // whether row t belongs to no sequence, or to one without keys: its output is zero
 __device__ __forceinline__ bool row_is_idle(const Params& p, int t) {
   const int s = p.token_seq[t];
-  return s < 0 || s >= p.B || t < p.q_cu[s] || t >= p.q_cu[s + 1] || p.kv_lens[s] <= 0;
+  return s < 0 || s >= p.B || t < p.q_cu[s] || t >= p.q_cu[s + 1] || p.kv_lens[s] <= 0 || p.max_blocks == 0;
 }
 
 // keys of the tile at kv0 that row t (at position pos) sees
@@ -1151,6 +1151,14 @@ static bool tc_serves(const void* q, const void* k, const void* v, int block_siz
          q_row % q_head == 0 && (reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 == 0;
 }
 
+// Whether the places of the caches and the work of a step (key tiles of all its items) count in 32 bits, and there are any.
+static bool tc_counts(int T, int B, int max_blocks, int block_size, int num_blocks, int n_q, int n_kv) {
+  const long places = long(num_blocks) * block_size;
+  const double items = (double(B) + double(T) / (xl_at::BQ / (n_q / n_kv))) * n_kv;       // row tiles at most, of as many nodes as fit 128 rows
+  return B > 0 && max_blocks > 0 && places > 0 && places <= 0x7fffffffl &&
+         items * (double(max_blocks) * block_size / xl_at::BKV + 2 + xl_at::kItemCost) <= double(0x7fffffff);
+}
+
 // How the fp32-pipe kernel is launched: row tiles of a sequence, parts of the keys, keys of a part.  max_q, max_kv: bounds of a sequence's rows
 // and keys.
 struct SimtPlan { int row_tiles, splits, part_keys; };
@@ -1174,8 +1182,10 @@ static int tc_ctas(int T, int B, int n_q, int n_kv, int max_kv, int sms) {
 
 // Bytes of the workspace.  max_q, max_kv: bounds of a sequence's rows and keys; plain: fp32, or scores or caches that the tensor-core kernel does not
 // take.  *tc: whether that kernel serves these sizes (for query rows on 16-byte boundaries).
-XL_API long xl_attention_tree_workspace(int T, int B, int block_size, int n_q, int n_kv, int D, int plain, int max_q, int max_kv, int* tc) {
-  *tc = tc_serves(nullptr, nullptr, nullptr, block_size, n_q, n_kv, D, 8, 8, 1.f, plain);
+XL_API long xl_attention_tree_workspace(int T, int B, int max_blocks, int block_size, int num_blocks, int n_q, int n_kv, int D, int plain, int max_q,
+                                        int max_kv, int* tc) {
+  *tc = tc_serves(nullptr, nullptr, nullptr, block_size, n_q, n_kv, D, 8, 8, 1.f, plain) &&
+        tc_counts(T, B, max_blocks, block_size, num_blocks, n_q, n_kv);
   const int sms = xl_host::sm_count();
   if (*tc) {
     const long rows = long(max_q) * (n_q / n_kv) > xl_at::BQ ? 256 : 128, DV = (D + 63) / 64 * 64, ctas = tc_ctas(T, B, n_q, n_kv, max_kv, sms);
@@ -1190,10 +1200,10 @@ XL_API int xl_attention_tree(const void* q, const void* k_cache, const void* v_c
                              int max_blocks, int block_size, int num_blocks, int n_q, int n_kv, int D, int words, long q_row, long q_head,
                              float scale, int window, int f32, int max_q, int max_kv, int tc, void* workspace, long workspace_bytes, void* stream) {
   using namespace xl_at;
-  if (T < 0 || B < 0 || n_kv < 1 || n_q % n_kv || D < 1 || D > 512 || words < 1 || block_size < 1 || max_blocks < 1) return -2;
+  if (T < 0 || B < 0 || n_kv < 1 || n_q < 1 || n_q % n_kv || D < 1 || D > 512 || words < 1 || block_size < 1 || max_blocks < 0) return -2;
   if (T == 0) return 0;
   int served = 0;
-  if (workspace_bytes < xl_attention_tree_workspace(T, B, block_size, n_q, n_kv, D, f32 || !tc, max_q, max_kv, &served)) return -2;
+  if (workspace_bytes < xl_attention_tree_workspace(T, B, max_blocks, block_size, num_blocks, n_q, n_kv, D, f32 || !tc, max_q, max_kv, &served)) return -2;
   const int sms = xl_host::sm_count();
   Params p{};
   p.q = q; p.k_cache = k_cache; p.v_cache = v_cache; p.out = out;
@@ -1209,12 +1219,9 @@ XL_API int xl_attention_tree(const void* q, const void* k_cache, const void* v_c
   p.scale = scale; p.window = window;
   auto s = static_cast<cudaStream_t>(stream);
   if (tc) {
-    if (B < 1 || !workspace || !tc_serves(q, k_cache, v_cache, block_size, n_q, n_kv, D, q_row, q_head, scale, f32)) return -2;
+    if (!workspace || !tc_counts(T, B, max_blocks, block_size, num_blocks, n_q, n_kv) || !tc_serves(q, k_cache, v_cache, block_size, n_q, n_kv, D, q_row, q_head, scale, f32)) return -2;
     const bool pair = long(max_q) * (n_q / n_kv) > BQ;
     const int ctas = tc_ctas(T, B, n_q, n_kv, max_kv, sms);
-    if (p.num_slots > 0x7fffffffl) return -2;
-    // the kernel counts its work in 32 bits
-    if ((long(B) + long(T) * (n_q / n_kv) / BQ) * n_kv * (long(max_blocks) * block_size / BKV + 2 + kItemCost) > 0x7fffffffl) return -2;
     TcParams t{};
     t.a = p;
     t.group = n_q / n_kv;

@@ -26,7 +26,7 @@ using StepRowsFn = int (*)(const void*, const void*, const void*, const void*, c
                            int, long, int, int, int, int, int, int, void*);
 using AcceptFn = int (*)(const void*, const void*, const void*, const void*, const void*, const void*, void*, void*, void*, int, int, int, int, int,
                          void**, const int*, const int*, int, int, void*);
-using WorkspaceFn = long (*)(int, int, int, int, int, int, int, int, int, int*);
+using WorkspaceFn = long (*)(int, int, int, int, int, int, int, int, int, int, int, int*);
 using AttentionFn = int (*)(const void*, const void*, const void*, void*, const void*, const void*, const void*, const void*, const void*, const void*,
                             int, int, int, int, int, int, int, int, int, long, long, float, int, int, int, int, int, void*, long, void*);
 using LogitsFn = int (*)(void*, int, int, int, long, const void*, const void*, int, int, int, const void*, long, int, const void*, const void*,
@@ -98,19 +98,18 @@ py::object tree_attention(Tensor q, const Tensor& k, const Tensor& v, const Tens
   const auto i32 = at::kInt, type = q.scalar_type();
   if (q.dim() != 3 || (type != at::kFloat && type != at::kBFloat16) || k.dim() != 4 || tree.dim() != 2 || tables.dim() != 2 || B < 0) return py::none();
   const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2), blocks = k.size(0), block = k.size(1), Hkv = k.size(2), W = tree.size(1);
-  if (!like(k, type, {blocks, block, Hkv, D}) || !like(v, type, {blocks, block, Hkv, D}) || D < 1 || D > 512 || Hkv < 1 || Hq % Hkv != 0 || W < 1 ||
+  if (!like(k, type, {blocks, block, Hkv, D}) || !like(v, type, {blocks, block, Hkv, D}) || D < 1 || D > 512 || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || block < 1 || block > INT32_MAX || W < 1 ||
       W > kTreeRows / 64 || max_q > kTreeRows || !like(tree, at::kLong, {T, W}) || !like(q_cu, i32, {B + 1}) || !like(kv_lens, i32, {B}) ||
       !like(tables, i32, {B, tables.size(1)}) || !like(token_seq, i32, {T}) || !like(positions, i32, {T}) || T * Hq > INT32_MAX || blocks > INT32_MAX ||
       max_kv > INT32_MAX || window > INT32_MAX || window < INT32_MIN)
     return py::none();
   const c10::cuda::CUDAGuard guard(q.device());
   const Tensor out = at::empty({T, Hq * D}, q.options());
-  // no tensor-core kernel: for scores that do not grow with the product, nor where the caches lie off 16-byte boundaries or have more
-  // places than a copy's coordinate counts
+  // no tensor-core kernel: for scores that do not grow with the product, nor where the caches lie off 16-byte boundaries
   const auto address = [](const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()); };
-  const bool f32 = type == at::kFloat, plain = f32 || !(scale > 0) || B == 0 || (address(k) | address(v)) % 16 != 0 || blocks * block > INT32_MAX;
+  const bool f32 = type == at::kFloat, plain = f32 || !(scale > 0) || (address(k) | address(v)) % 16 != 0;
   int tc = 0;
-  const long size = f_workspace(int(T), int(B), int(block), int(Hq), int(Hkv), int(D), plain, int(max_q), int(max_kv), &tc);
+  const long size = f_workspace(int(T), int(B), int(tables.size(1)), int(block), int(blocks), int(Hq), int(Hkv), int(D), plain, int(max_q), int(max_kv), &tc);
   if (q.stride(2) != 1 || (tc && (q.stride(1) < 1 || q.stride(0) < 1 || q.stride(1) % 8 || q.stride(0) % std::max<int64_t>(8, q.stride(1)) ||
                                   address(q) % 16)))
     q = q.clone(at::MemoryFormat::Contiguous);

@@ -400,8 +400,9 @@ def tree_attention(q, k_cache, v_cache, inp, tree, scale, sliding_window=-1):
     T, Hq, D = q.shape
     dev, i32, B = q.get_device(), torch.int32, inp.n_seqs
     assert q.dtype is k_cache.dtype is v_cache.dtype and q.dtype in (torch.bfloat16, torch.float32), "q and caches: one type, bf16 or fp32"
-    assert k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.shape[3] == D and D <= 512, "caches: [blocks, block, Hkv, D]"
-    assert Hq % k_cache.shape[2] == 0 and k_cache.is_contiguous() and v_cache.is_contiguous(), "caches: contiguous, key heads that divide q's"
+    assert k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.shape[3] == D and 1 <= D <= 512, "caches: [blocks, block, Hkv, D]"
+    assert k_cache.shape[1] >= 1 and Hq >= 1 and k_cache.shape[2] >= 1 and Hq % k_cache.shape[2] == 0, "caches: key heads that divide q's"
+    assert k_cache.is_contiguous() and v_cache.is_contiguous(), "caches: contiguous"
     assert k_cache.get_device() == v_cache.get_device() == dev, "caches: on q's device"
     assert inp.max_q <= TREE_MAX_ROWS, f"trees have at most {TREE_MAX_ROWS} rows a sequence"
     tables = inp.block_tables
@@ -499,7 +500,7 @@ def accept_tree(target, inp, parents, caches=(), max_depth=None):
     assert tables.dim() == 2, "block_tables: [B, blocks]"
     _like(tables, i32, (B, tables.shape[1]), dev, "block_tables")
     assert inp.max_q <= TREE_MAX_ROWS, f"trees have at most {TREE_MAX_ROWS} rows a sequence"
-    assert 0 <= depth < TREE_MAX_ROWS and B < 65536
+    assert 0 <= depth < TREE_MAX_ROWS and B < 65536 and block >= 1
     for c in caches:
         assert c.is_contiguous() and c.dim() >= 2 and c.shape[1] == block and c.get_device() == dev, "caches: [blocks, block, ...], contiguous"
     held = sorted((c.data_ptr(), c.data_ptr() + c.nbytes) for c in caches if c.numel())
