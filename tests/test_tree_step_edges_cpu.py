@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import oracle_tree as oracle
-from test_tree_step_cpu import attention_inputs, rules
+from test_tree_step_cpu import acceptance, attention_inputs, rules
 from xllm_wxh_b200 import ops
 
 
@@ -51,3 +51,33 @@ def test_tree_attention_refuses_heads_and_blocks_of_nothing():
         a = {**dict(q=q, k=k, v=v), **bad}
         with pytest.raises(AssertionError):
             ops.tree_attention(a["q"], a["k"], a["v"], step.inp, step.tree, 1.0)
+
+
+def test_accept_tree_places_outside_tables_and_caches():
+    """Tables too short for the path, entries that name no block, fewer keys than rows, caches of different lengths: those rows stay."""
+    step = oracle.Step([6, 9, 0], [20, 12, 9], 4, seed=6, deep=True, junk_tables=False)
+    target = acceptance(step, 7, 1)
+    for a, n in zip(step.cu.tolist(), step.counts):              # two rows follow every second one, and the second of them is agreed with
+        step.inp.tokens[a + 1:a + n:2] = 1
+        step.parents[a + 1:a + n] = torch.arange(n - 1) // 2 * 2
+    step.parents_of = [step.parents[a:a + n].tolist() for a, n in zip(step.cu.tolist(), step.counts)]
+    step.inp.kv_lens[2] = 5
+    step.inp.block_tables[1, 4] = -3
+    step.inp.block_tables[0, 3] = 10 ** 6
+    step.inp.block_tables = step.inp.block_tables[:, :5].contiguous()
+    caches = [torch.randn(step.blocks, 4, 3), torch.randn(step.blocks - 3, 4, 8)]
+    want, moved = [c.clone() for c in caches], 0
+    for i, n in enumerate(step.counts):
+        a, base = int(step.cu[i]), int(step.inp.kv_lens[i]) - n
+        rows = oracle.accepted_path(step.inp.tokens[a:a + n].tolist(), step.parents_of[i], target[a:a + n].tolist(), 19)
+        for j, r in enumerate(rows):
+            s, d = base + r, base + j
+            if min(s, d) >= 0 and max(s, d) < 20:
+                (b0, o0), (b1, o1) = step.place(i, s), step.place(i, d)
+                for c, w in zip(caches, want):
+                    if 0 <= b0 < len(c) and 0 <= b1 < len(c):
+                        moved += s != d
+                        w[b1, o1] = c[b0, o0]
+    assert moved > 5 and step.inp.block_tables.shape[1] == 5
+    ops.accept_tree(target, step.inp, step.parents, caches)
+    assert all(torch.equal(c, w) for c, w in zip(caches, want))

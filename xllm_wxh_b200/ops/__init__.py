@@ -484,7 +484,8 @@ def accept_tree(target, inp, parents, caches=(), max_depth=None):
     first row that follows with the target's token, up to max_depth rows (default: inp.max_q - 1).  Returns (out [B, max_depth + 1]: the
     target's tokens along the path, then -1; accepted [B]: drafted rows on the path; path [B, max_depth + 1]: their numbers, then -1).
     In every tensor of `caches` ([blocks, block, ...], contiguous, no memory twice) the path's rows move to the positions behind the
-    sequence's earlier tokens, which then has 1 + accepted more; the other drafted rows' places hold what they held."""
+    sequence's earlier tokens, which then has 1 + accepted more; the other drafted rows' places hold what they held.  Rows move only
+    between places that lie in the table and in the cache."""
     depth = max(0, inp.max_q - 1) if max_depth is None else max_depth
     if target.is_cuda:
         out = _tree().accept_tree(target, inp, parents, caches, depth)

@@ -931,9 +931,11 @@ def accept_tree(target, inp, parents, caches, depth: int):
             out[b, i], path[b, i] = want[a + j], j
         accepted[b] = max(len(rows) - 1, 0)
         base = int(inp.kv_lens[b]) - n
-        place = lambda p: (int(inp.block_tables[b, p // block]), p % block)
+        held = inp.block_tables[b].tolist()
+        place = lambda p: (held[p // block] if 0 <= p < len(held) * block else -1, p % block)
         for i, j in enumerate(rows):
             (b1, o1), (b0, o0) = place(base + i), place(base + j)
             for c in caches:
-                c[b1, o1] = c[b0, o0]
+                if 0 <= b0 < c.shape[0] and 0 <= b1 < c.shape[0]:
+                    c[b1, o1] = c[b0, o0]
     return out, accepted, path
