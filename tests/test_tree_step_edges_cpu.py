@@ -1,4 +1,6 @@
 """Operators of a step with trees of drafted tokens on the CPU at the edges of what their documentation allows."""
+import types
+
 import pytest
 import torch
 
@@ -81,3 +83,23 @@ def test_accept_tree_places_outside_tables_and_caches():
     assert moved > 5 and step.inp.block_tables.shape[1] == 5
     ops.accept_tree(target, step.inp, step.parents, caches)
     assert all(torch.equal(c, w) for c, w in zip(caches, want))
+
+
+def test_chained_drafts_share_one_block_table():
+    """Drafts 2 to k of a chain run on the same tables; positions, places and lengths grow by one a draft."""
+    from xllm_wxh_b200.runtime.speculative import SpeculativeEngine
+    k, bs, ints = 4, 4, lambda *v: torch.tensor(v, dtype=torch.int32)
+    tables = torch.arange(1, 3 * 8 + 1, dtype=torch.int32).view(3, 8)
+    inp = types.SimpleNamespace(token_seq=ints(1, 1, 0, 2), block_tables=tables, block_size=bs, max_kv=20, layout=types.SimpleNamespace(MB_cap=8))
+    seen = []
+    draft = types.SimpleNamespace(forward_mtp=lambda mini, kv, h: seen.append(mini) or h + 1)
+    engine = types.SimpleNamespace(k=k, draft=draft, draft_kv=None, _propose=lambda h, rows: h[:, 0].int() * 10)
+    pos = ints(7, 0, 18)
+    out = SpeculativeEngine._chain_drafts(engine, inp, torch.tensor([0, 2, 3]), ints(5, 6, 7), torch.zeros(3, 2), pos)
+    assert out.view(3, k).tolist() == [[f, 10, 20, 30] for f in (5, 6, 7)] and pos.tolist() == [7, 0, 18]
+    assert len(seen) == k - 1 and len({m.block_tables.data_ptr() for m in seen}) == 1
+    for j, m in enumerate(seen):
+        at = [p + j for p in (7, 0, 18)]
+        assert m.positions.tolist() == at and m.kv_lens.tolist() == [p + 1 for p in at] and m.q_cu.tolist() == [0, 1, 2, 3]
+        assert m.slots.tolist() == [int(tables[s, p // bs]) * bs + p % bs for s, p in zip((1, 0, 2), at)]
+        assert torch.equal(m.block_tables, tables[[1, 0, 2]]) and m.max_kv == 21 + j

@@ -279,20 +279,21 @@ class SpeculativeEngine(LLMEngine):
         if k == 1:
             return first
         B = first.shape[0]
-        seq = inp.token_seq.index_select(0, seq_rows)                        # index of each sequence in the step's tables
+        seq = inp.token_seq.index_select(0, seq_rows).long()                 # index of each sequence in the step's tables
+        bt = inp.block_tables.index_select(0, seq)                           # the same for all drafts: every block is there already
         bs = inp.block_size
-        lens = torch.zeros(inp.block_tables.shape[0], dtype=torch.int32, device=first.device)
-        lens.index_copy_(0, seq.long(), pos.int())
-        one = torch.ones_like(seq)
+        lens = pos.int()
+        seqs = torch.arange(B, dtype=torch.int32, device=first.device)
+        one = torch.ones_like(seqs)
         out = [first]
         tok, h = first, hidden
         for j in range(1, k):
-            r = ops.step_rows(inp.block_tables, lens, seq, one, B, bs, max_q=1)
-            mini = _DraftRows(tok, r.positions, r.slots, r.q_cu, r.kv_lens, r.block_tables, bs, inp.layout.MB_cap, max_kv=inp.max_kv + j)
+            r = ops.step_rows(bt, lens, seqs, one, B, bs, max_q=1, max_blocks=0)
+            mini = _DraftRows(tok, r.positions, r.slots, r.q_cu, r.kv_lens, bt, bs, inp.layout.MB_cap, max_kv=inp.max_kv + j)
             h = self.draft.forward_mtp(mini, self.draft_kv, h)
             tok = self._propose(h, None)
             out.append(tok)
-            lens += 1
+            lens = r.kv_lens                                                 # (with the row of this draft)
         return torch.stack(out, 1).reshape(-1)
 
     # ------------------------------------------------------------------ rank 0
