@@ -7,7 +7,7 @@ import torch
 
 import oracle_tree as oracle
 from test_tree_step_cpu import acceptance, attention_inputs, check_rules, rules
-from test_tree_step_gpu import cuda, status      # noqa: F401 (every test reads the status word)
+from test_tree_step_gpu import check_attention, cuda, status      # noqa: F401 (every test reads the status word)
 from xllm_wxh_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -154,3 +154,11 @@ def test_accept_tree_places_outside_tables_and_caches():
     dev = [c.cuda() for c in caches]
     ops.accept_tree(target.cuda(), step.to("cuda"), step.parents.cuda(), dev)
     assert all(torch.equal(c.cpu(), w) for c, w in zip(dev, want))
+
+@pytest.mark.parametrize("Hq,D", [(16, 64), (12, 128)])
+def test_tree_attention_many_pieces_of_one_and_two_row_tiles(Hq, D):
+    """A stretch of many short items, with one and with two row tiles in any order, and items of more row tiles than two."""
+    counts = [(i * 7) % 23 if i % 29 else 40 for i in range(300)]
+    step = oracle.Step([(i * 13) % 150 for i in range(300)], counts, 16, seed=10)
+    check_attention(step, Hq, 1, D, torch.bfloat16)
+    check_attention(step, Hq, 1, D, torch.bfloat16, window=33)

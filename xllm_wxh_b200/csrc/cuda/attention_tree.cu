@@ -451,7 +451,8 @@ int launch_simt(const Params& p, int row_tiles, int splits, int part_keys, float
 // Masks: keys ahead of the tree are seen by all rows (within the window), the tree's by the row's words; only tiles that hold either
 // border look at them.  There, values behind the last row are cleared, and values that are not finite are taken out of the tile and
 // added to the rows that do see them, so that whatever stands in a masked place reaches no other row.
-// Every wait is bounded; on expiry the kernel records a status code and leaves.
+// Every wait on an mbarrier is bounded; on expiry the kernel records a status code and leaves once its copies and products in flight have ended.
+// The softmax warps meet at named barriers, which know no bound: they decide together whether to leave, and go on without waiting until then.
 constexpr int BQ = 128;
 constexpr int kTcThreads = 352;
 constexpr int Q_SLAB = BQ * 128, KV_SLAB = BKV * 128;
@@ -472,7 +473,7 @@ struct Piece {
 };
 struct TcBarriers {
   uint64_t full[kMaxUnits], empty[kMaxUnits];
-  uint64_t q_full, q_empty, info[kPieces];
+  uint64_t q_full, q_empty, info[kPieces], drained[2];
   // [group][buffer]: softmax may be two tiles ahead of the products and need not look at each one's end, so that a barrier a group
   // would be a phase off
   uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];
@@ -577,6 +578,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
     mbar_init(&bars->q_empty, 2);
     for (int i = 0; i < kPieces; ++i) mbar_init(&bars->info[i], 1);
     for (int g = 0; g < 2; ++g) {
+      mbar_init(&bars->drained[g], 1);
       for (int b = 0; b < 2; ++b) {
         mbar_init(&bars->s_full[g][b], 1);
         mbar_init(&bars->p_full[g][b], 4);
@@ -661,7 +663,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
       w += at;
     }
     bool ok = true;
-    int st = 0, phase = 0, count = 0;
+    int st = 0, phase = 0, count = 0, units = 0, q_sent = 0;           // (q_sent: of lane 0)
     while (ok && busy && w < w1) {
       // the part of the item that lies in the stretch
       x.j0 = max(w0 - w - kItemCost, 0);
@@ -690,6 +692,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
             bars->piece[info] = x;
             mbar_arrive(&bars->info[info]);
             const int tiles = x.pair ? 2 : 1;
+            ++q_sent;
             mbar_arrive_expect_tx(&bars->q_full, uint32_t(tiles * QS * 128 * p.group * p.nodes));
             for (int h = 0; h < tiles; ++h)
 #pragma unroll
@@ -704,6 +707,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
             if (ok) mbar_arrive_expect_tx(&bars->full[st], UNIT);
           }
           ok = __shfl_sync(0xffffffffu, ok, 0);
+          units += ok;
           if (ok && lane < per_unit)
             tma_load_3d(ring + st * UNIT + slab * KV_SLAB + bx * p.box_tokens * 128, map, &bars->full[st], slab * 64, x.head, slot);
           if (++st == U) {
@@ -757,6 +761,9 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
       mbar_arrive(&bars->info[count % kPieces]);
       if (count == 0) p.ws_desc[blockIdx.x * 8 + DESC_MERGE] = 0;
       if (!ok) atomicExch(p.status, XL_ERR_WAIT_EMPTY);
+      // no copy may land behind the CTA's end (all have, unless a wait ran out)
+      ok = q_sent == 0 || mbar_wait(&bars->q_full, (q_sent - 1) & 1);
+      for (int u = max(units - U, 0); ok && u < units; ++u) ok = mbar_wait(&bars->full[u % U], (u / U) & 1);
     }
   } else if (warp <= 2) {
     // ---------------------------------------------------------- MMA issuer of group g
@@ -825,6 +832,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
         }
       }
       if (!ok) atomicExch(p.status, XL_ERR_WAIT_FULL);
+      tc_commit(&bars->drained[g]);                                    // nor a product run on memory that has been given back
+      mbar_wait(&bars->drained[g], 0);
     }
   } else {
     // ---------------------------------------------------------- softmax, one row per thread
@@ -835,6 +844,18 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
     const float sc = p.scale_log2;
     auto group_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory"); };
     auto both_sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+    auto both_agree = [](bool mine) {                                  // whether it is true of all threads of the two groups
+      uint32_t all;
+      asm volatile(
+          "{\n\t.reg .pred P, Q;\n\t"
+          "setp.ne.u32 P, %1, 0;\n\t"
+          "barrier.cta.red.and.pred Q, 1, 256, P;\n\t"
+          "selp.u32 %0, 1, 0, Q;\n\t}"
+          : "=r"(all)
+          : "r"(uint32_t(mine))
+          : "memory");
+      return all != 0;
+    };
     // idle rows: every thread looks at one of this CTA's share, a warp clears what its lanes found
     for (long t0 = blockIdx.x; t0 < a.T; t0 += 256l * gridDim.x) {
       const long t = t0 + (tid - 96l) * gridDim.x;
@@ -847,7 +868,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
     bool ok = true;
     int u0 = 0, count = 0;                                             // units ahead of the piece; tiles of this group so far
     for (int piece = 0;; ++piece) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&bars->info[piece % kPieces], (piece / kPieces) & 1))) {
+      // (a warp that left alone would be missed at the barriers by those that saw the piece)
+      if (!both_agree(mbar_wait(&bars->info[piece % kPieces], (piece / kPieces) & 1))) {
         ok = false;
         break;
       }
