@@ -868,11 +868,13 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
     bool ok = true;
     int u0 = 0, count = 0;                                             // units ahead of the piece; tiles of this group so far
     for (int piece = 0;; ++piece) {
-      // (a warp that left alone would be missed at the barriers by those that saw the piece)
+      // Both groups have read the last piece's O and maxima.  (And a warp that left alone would be missed at the barriers by those that saw
+      // the piece.)
       if (!both_agree(mbar_wait(&bars->info[piece % kPieces], (piece / kPieces) & 1))) {
         ok = false;
         break;
       }
+      tc_fence_after();
       const Piece& x = bars->piece[piece % kPieces];
       const int nt = x.nt;
       if (nt == 0) break;
@@ -1079,7 +1081,6 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_c
         group_sync();
       }
       tc_fence_before();
-      if (!pair) both_sync();                                          // both groups have read O and the maxima
     }
     if (!ok && lane == 0) atomicExch(p.status, XL_ERR_WAIT_TMEM_FULL);
   }
