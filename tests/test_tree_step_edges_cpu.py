@@ -1,4 +1,5 @@
 """Operators of a step with trees of drafted tokens on the CPU at the edges of what their documentation allows."""
+import os
 import types
 
 import pytest
@@ -103,3 +104,15 @@ def test_chained_drafts_share_one_block_table():
         assert m.positions.tolist() == at and m.kv_lens.tolist() == [p + 1 for p in at] and m.q_cu.tolist() == [0, 1, 2, 3]
         assert m.slots.tolist() == [int(tables[s, p // bs]) * bs + p % bs for s, p in zip((1, 0, 2), at)]
         assert torch.equal(m.block_tables, tables[[1, 0, 2]]) and m.max_kv == 21 + j
+
+
+def test_entry_points_have_one_signature():
+    """The host side takes the kernels' argument lists from the header that their definitions include, not from a copy."""
+    from xllm_wxh_b200 import build_ext
+    from xllm_wxh_b200.ops import tree_cuda
+    read = lambda *p: open(os.path.join(*p)).read()
+    api = read(build_ext.CUDA_DIR, "tree_api.h")
+    for name in tree_cuda._ENTRIES:
+        assert f" {name}(" in api and f"decltype(&{name})" in read(build_ext.TREE_HOST_SRC)
+    for f in ("tree_step.cu", "attention_tree.cu", "logit_rules.cu"):
+        assert '#include "tree_api.h"' in read(build_ext.CUDA_DIR, f)

@@ -92,14 +92,15 @@ TREE_HOST_SO = os.path.join(HERE, "_tree_host" + sysconfig.get_config_var("EXT_S
 
 def build_tree_host(force=False):
     """`_tree_host`: argument checks, allocation and launches of the tree operators in C++ over torch's tensors."""
-    if not force and not _newer([TREE_HOST_SRC], TREE_HOST_SO):
+    srcs = [TREE_HOST_SRC, os.path.join(CUDA_DIR, "tree_api.h")]
+    if not force and not _newer(srcs, TREE_HOST_SO):
         return TREE_HOST_SO
     from torch.utils import cpp_extension
     libs = cpp_extension.library_paths()
     cuda = os.path.dirname(os.path.dirname(NVCC))
     _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-Wall", "-Wno-unknown-pragmas",
           *[f"-I{p}" for p in cpp_extension.include_paths()], "-I", os.path.join(cuda, "include"), "-I", sysconfig.get_paths()["include"],
-          TREE_HOST_SRC, "-o", TREE_HOST_SO, *[f"-L{p}" for p in libs], "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
+          "-I", CUDA_DIR, TREE_HOST_SRC, "-o", TREE_HOST_SO, *[f"-L{p}" for p in libs], "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
           *[f"-Wl,-rpath,{p}" for p in libs]])
     return TREE_HOST_SO
 

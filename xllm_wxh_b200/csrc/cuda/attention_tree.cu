@@ -6,6 +6,7 @@
 #include <type_traits>
 
 #include "attention_tc.cuh"
+#include "tree_api.h"
 #include "vec8.cuh"
 
 namespace xl_at {
@@ -1203,8 +1204,6 @@ static int tc_ctas(int T, int B, int n_q, int n_kv, int max_kv, int sms) {
   return int(max(1l, min(long(sms), (long(max_kv) / 64 + 1) * n_kv * (B + long(T) * (n_q / n_kv) / xl_at::BQ))));
 }
 
-// Bytes of the workspace.  max_q, max_kv: bounds of a sequence's rows and keys; plain: fp32, or scores or caches that the tensor-core kernel does not
-// take.  *tc: whether that kernel serves these sizes (for query rows on 16-byte boundaries).
 XL_API long xl_attention_tree_workspace(int T, int B, int max_blocks, int block_size, int num_blocks, int n_q, int n_kv, int D, int plain, int max_q,
                                         int max_kv, int* tc) {
   *tc = tc_serves(nullptr, nullptr, nullptr, block_size, n_q, n_kv, D, 8, 8, 1.f, plain) &&

@@ -20,6 +20,7 @@
 // are whole numbers and the last bias of an id wins by its index: the order in which threads arrive changes nothing.
 #include <atomic>
 
+#include "tree_api.h"
 #include "vec8.cuh"
 
 namespace xl_lr {

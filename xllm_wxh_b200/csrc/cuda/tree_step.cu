@@ -4,6 +4,7 @@
 // Both are bound by latency for small steps and by copying for large ones (block tables; kept cache rows), so each is one launch:
 // every CTA finds the little it needs of the other sequences by itself instead of waiting for a kernel that prepares it.
 #include "common.cuh"
+#include "tree_api.h"
 
 namespace xl_ts {
 using namespace xl;
@@ -274,7 +275,6 @@ XL_API int xl_step_rows(const void* tables, const void* lens, const void* seqs, 
   return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }
 
-// `caches`, `units`, `blocks`: host arrays of n entries.  unit: bytes that move at once (16, 4, 2 or 1).
 XL_API int xl_accept_tree(const void* target, const void* tokens, const void* parents, const void* q_cu, const void* kv_lens,
                           const void* block_tables, void* out, void* accepted, void* path, int T, int B, int max_blocks, int block_size, int depth,
                           void** caches, const int* units, const int* blocks, int n, int unit, void* stream) {

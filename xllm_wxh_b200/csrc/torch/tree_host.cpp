@@ -15,6 +15,8 @@
 #include <utility>
 #include <vector>
 
+#include "tree_api.h"
+
 namespace py = pybind11;
 using at::Tensor;
 
@@ -22,29 +24,18 @@ namespace {
 
 constexpr int64_t kTreeRows = 256;
 
-using StepRowsFn = int (*)(const void*, const void*, const void*, const void*, const void*, void*, void*, void*, void*, void*, void*, void*, int,
-                           int, long, int, int, int, int, int, int, void*);
-using AcceptFn = int (*)(const void*, const void*, const void*, const void*, const void*, const void*, void*, void*, void*, int, int, int, int, int,
-                         void**, const int*, const int*, int, int, void*);
-using WorkspaceFn = long (*)(int, int, int, int, int, int, int, int, int, int, int, int*);
-using AttentionFn = int (*)(const void*, const void*, const void*, void*, const void*, const void*, const void*, const void*, const void*, const void*,
-                            int, int, int, int, int, int, int, int, int, long, long, float, int, int, int, int, int, void*, long, void*);
-using LogitsFn = int (*)(void*, int, int, int, long, const void*, const void*, int, int, int, const void*, long, int, const void*, const void*,
-                         const void*, const void*, const void*, const void*, const void*, const void*, const void*, const void*, int, const void*, int,
-                         int, const void*, void*);
-
-StepRowsFn f_step_rows;
-AcceptFn f_accept;
-WorkspaceFn f_workspace;
-AttentionFn f_attention;
-LogitsFn f_logits;
+decltype(&xl_step_rows) f_step_rows;
+decltype(&xl_accept_tree) f_accept;
+decltype(&xl_attention_tree_workspace) f_workspace;
+decltype(&xl_attention_tree) f_attention;
+decltype(&xl_adjust_logits) f_logits;
 
 void bind(const std::unordered_map<std::string, uint64_t>& at) {
-  f_step_rows = reinterpret_cast<StepRowsFn>(at.at("xl_step_rows"));
-  f_accept = reinterpret_cast<AcceptFn>(at.at("xl_accept_tree"));
-  f_workspace = reinterpret_cast<WorkspaceFn>(at.at("xl_attention_tree_workspace"));
-  f_attention = reinterpret_cast<AttentionFn>(at.at("xl_attention_tree"));
-  f_logits = reinterpret_cast<LogitsFn>(at.at("xl_adjust_logits"));
+  f_step_rows = reinterpret_cast<decltype(f_step_rows)>(at.at("xl_step_rows"));
+  f_accept = reinterpret_cast<decltype(f_accept)>(at.at("xl_accept_tree"));
+  f_workspace = reinterpret_cast<decltype(f_workspace)>(at.at("xl_attention_tree_workspace"));
+  f_attention = reinterpret_cast<decltype(f_attention)>(at.at("xl_attention_tree"));
+  f_logits = reinterpret_cast<decltype(f_logits)>(at.at("xl_adjust_logits"));
 }
 
 using Opt = std::optional<Tensor>;
