@@ -1,5 +1,6 @@
 """Operators of a step with trees of drafted tokens on the CPU at the edges of what their documentation allows."""
 import os
+import sys
 import types
 
 import pytest
@@ -104,6 +105,36 @@ def test_chained_drafts_share_one_block_table():
         assert m.positions.tolist() == at and m.kv_lens.tolist() == [p + 1 for p in at] and m.q_cu.tolist() == [0, 1, 2, 3]
         assert m.slots.tolist() == [int(tables[s, p // bs]) * bs + p % bs for s, p in zip((1, 0, 2), at)]
         assert torch.equal(m.block_tables, tables[[1, 0, 2]]) and m.max_kv == 21 + j
+
+
+def test_host_extension_is_built_again_for_another_torch_and_other_entry_points(tmp_path, monkeypatch):
+    from xllm_wxh_b200 import build_ext
+    so, built = tmp_path / "_tree_host.so", []
+    monkeypatch.setattr(build_ext, "TREE_HOST_SO", str(so))
+    monkeypatch.setattr(build_ext, "_run", lambda cmd, log=None: built.append(cmd))
+    build_ext.build_tree_host()
+    assert len(built) == 1 and any(torch.__version__ in a for a in built[0])                # missing
+    so.write_bytes(b"\0built for torch " + torch.__version__.encode() + b";\0")
+    build_ext.build_tree_host()
+    assert len(built) == 1                                                                  # as it should be
+    api = os.path.join(build_ext.CUDA_DIR, "tree_api.h")
+    os.utime(so, (0, os.path.getmtime(api) - 1))
+    build_ext.build_tree_host()
+    assert len(built) == 2                                                                  # older than the entry points' signatures
+    so.write_bytes(b"\0built for torch 1.0;\0")
+    build_ext.build_tree_host()
+    assert len(built) == 3
+
+
+def test_host_extension_that_does_not_load_says_why(monkeypatch):
+    import xllm_wxh_b200
+    from xllm_wxh_b200.ops import cuda_ops, tree_cuda
+    monkeypatch.setattr(tree_cuda, "_host", None)
+    monkeypatch.setattr(cuda_ops, "lib", lambda: None)
+    monkeypatch.delattr(xllm_wxh_b200, "_tree_host", raising=False)
+    monkeypatch.setitem(sys.modules, "xllm_wxh_b200._tree_host", None)
+    with pytest.raises(RuntimeError, match="does not load .*None in sys.modules.*build_ext"):
+        tree_cuda.host()
 
 
 def test_entry_points_have_one_signature():

@@ -90,17 +90,25 @@ TREE_HOST_SRC = os.path.join(HERE, "csrc", "torch", "tree_host.cpp")
 TREE_HOST_SO = os.path.join(HERE, "_tree_host" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
+def _built_for(so, torch_version):
+    """Whether an extension over torch's C++ interface was built against that version of torch (it says so in its data)."""
+    with open(so, "rb") as f:
+        return f"built for torch {torch_version};".encode() in f.read()
+
+
 def build_tree_host(force=False):
-    """`_tree_host`: argument checks, allocation and launches of the tree operators in C++ over torch's tensors."""
+    """`_tree_host`: argument checks, allocation and launches of the tree operators in C++ over torch's tensors.  Built again for
+    another torch or other entry points of the kernel library (`tree_api.h`)."""
+    import torch
     srcs = [TREE_HOST_SRC, os.path.join(CUDA_DIR, "tree_api.h")]
-    if not force and not _newer(srcs, TREE_HOST_SO):
+    if not force and not _newer(srcs, TREE_HOST_SO) and _built_for(TREE_HOST_SO, torch.__version__):
         return TREE_HOST_SO
     from torch.utils import cpp_extension
     libs = cpp_extension.library_paths()
     cuda = os.path.dirname(os.path.dirname(NVCC))
     _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-Wall", "-Wno-unknown-pragmas",
           *[f"-I{p}" for p in cpp_extension.include_paths()], "-I", os.path.join(cuda, "include"), "-I", sysconfig.get_paths()["include"],
-          "-I", CUDA_DIR, TREE_HOST_SRC, "-o", TREE_HOST_SO, *[f"-L{p}" for p in libs], "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
+          "-I", CUDA_DIR, f'-DXL_TORCH_VERSION="{torch.__version__}"', TREE_HOST_SRC, "-o", TREE_HOST_SO, *[f"-L{p}" for p in libs], "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
           *[f"-Wl,-rpath,{p}" for p in libs]])
     return TREE_HOST_SO
 

@@ -209,6 +209,9 @@ py::object accept_tree(const Tensor& target, const Tensor& tokens, const Tensor&
 
 }  // namespace
 
+// what build_ext finds in the file when it decides whether to build again
+__attribute__((used)) const char kBuiltFor[] = "built for torch " XL_TORCH_VERSION ";";
+
 PYBIND11_MODULE(_tree_host, m) {
   m.def("bind", &bind);
   m.def("step_rows", &step_rows);

@@ -22,7 +22,7 @@ def host():
         try:
             from .. import _tree_host as h
         except ImportError as e:
-            raise RuntimeError("_tree_host is missing: run `python -m xllm_wxh_b200.build_ext` (needs g++)") from e
+            raise RuntimeError(f"_tree_host does not load ({e}): run `python -m xllm_wxh_b200.build_ext` (needs g++)") from e
         h.bind({name: ctypes.cast(getattr(real, name), ctypes.c_void_p).value for name in _ENTRIES})
         _host, _timed = h, cuda_ops.kernel_timing()
     return _host
