@@ -113,6 +113,88 @@ def test_tree_attention_visible_values_and_scores_that_are_not_finite(before, at
     k[step.place(0, at)][..., 4] = float("nan")
     assert not check_not_finite(step, q, k, v, dtype).any()
 
+def seen_bound(step, q, k, want, size, scale, longest, dtype, hidden):
+    """The bound of roundings from the keys that some row sees."""
+    k = k.clone()
+    k[hidden] = 0
+    return oracle.attention_bound(q, k, want, size, scale, longest, dtype)
+
+
+@pytest.mark.parametrize("D,dtype", [(128, torch.bfloat16), (64, torch.float32), (192, torch.bfloat16)])
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("before,n,window", [(70, 10, -1), (3, 70, -1), (300, 12, 50), (128, 4, -1), (60, 3, -1), (900, 20, 100)])
+def test_tree_attention_largest_numbers_behind_masks(before, n, window, sign, D, dtype):
+    """The largest finite numbers in places that no row sees, and in branches that others see: bounds by what a row sees."""
+    step = oracle.Step([before, 9], [n, 2], 16, seed=7, words=2)
+    q, k, v = attention_inputs(step, 8, 2, D, dtype)
+    hidden = torch.ones(step.blocks, step.block, dtype=torch.bool)
+    for i, (b, m) in enumerate(zip(step.before, step.counts)):
+        for p in range(max(0, b - window) if window > 0 else 0, b + m):
+            hidden[step.place(i, p)] = False
+    k[hidden], v[hidden] = sign * torch.finfo(dtype).max, sign * torch.finfo(dtype).max
+    scale = D ** -0.5
+    got = ops.tree_attention(q.cuda(), k.cuda(), v.cuda(), step.to("cuda"), step.tree.cuda(), scale, window).view(step.T, 8, D).cpu().double()
+    want, size = oracle.attention(q, k, v, step, step.tree, scale, window)
+    bound = seen_bound(step, q, k, want, size, scale, before + n, dtype, hidden)
+    # a weight's and the result's roundings, 2^-8 each, of values below 8: far below the values themselves
+    assert bound.max() < 0.07 and want.abs().max() > 1
+    assert ((got - want).abs() <= bound).all()
+    # the last row, which no other sees, holds the largest numbers as values and keys: the other rows are as before
+    last = int(step.cu[1]) - 1
+    k[step.place(0, before + n - 1)], v[step.place(0, before + n - 1)] = -sign * torch.finfo(dtype).max, sign * torch.finfo(dtype).max
+    rest = torch.arange(step.T) != last
+    got = ops.tree_attention(q.cuda(), k.cuda(), v.cuda(), step.to("cuda"), step.tree.cuda(), scale, window).view(step.T, 8, D).cpu().double()
+    assert ((got - want).abs() <= bound)[rest].all()
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,length", [(262149, 40), (262213, 20000), (600000, 300)])
+def test_adjust_logits_vocabulary_of_several_slices(V, length, dtype):
+    """More ids than a bitmap holds: histories, paths, biases and masks on either side of the border between slices."""
+    g = torch.Generator().manual_seed(length)
+    edge = torch.tensor([0, 31, 262142, 262143, 262144, 262145, V - 1], dtype=I32)
+    ids = torch.randint(0, V, (3, length), generator=g, dtype=I32)
+    ids[:, :14] = edge.repeat(2)
+    ids[1] = ids[1, :14].repeat(length // 14 + 1)[:length]
+    lens, prompts = torch.tensor([length, length - 1, 3], dtype=I32), torch.tensor([length // 2, 0, 9], dtype=I32)
+    pen = (torch.tensor([1.3, 0.7, 1.5]), torch.tensor([0.1, -0.02, 0.3]), torch.tensor([0.5, 0.1, 0.0]))
+    cu, seqs = torch.tensor([0, 3, 4, 6], dtype=I32), torch.tensor([2, 0, 1], dtype=I32)
+    tokens = torch.tensor([262143, 262144, V - 1, 262144, 5, 262143], dtype=I32)
+    parents = torch.tensor([-1, 0, 1, -1, -1, 0], dtype=I32)
+    n = 50
+    bias = (torch.tensor([0, n, 2 * n, 3 * n], dtype=I32), torch.randint(0, V, (3 * n,), generator=g, dtype=I32), torch.randn(3 * n, generator=g))
+    bias[1][:7], bias[1][n:n + 7] = edge, edge.flip(0)
+    bias[1][7] = 262144                                           # twice: the last one holds
+    words = torch.randint(-2 ** 31, 2 ** 31, (2, -(-V // 32)), generator=g, dtype=torch.int64).int()
+    words[0, 262112 // 32:262176 // 32] = -1
+    of = torch.tensor([0, 1, -1, 0, 0, -1], dtype=I32)
+    x = (torch.randn(6, V, generator=g) * 3).to(dtype)
+    got = x.cuda()
+    ops.adjust_logits(got, *cuda((cu, seqs, (ids, lens, prompts), pen, tokens, parents, bias, (words, of))), max_q=3)
+    got = got.cpu().double()
+    allowed = ((words[..., None] >> torch.arange(32).int()) & 1).flatten(1)[:, :V].bool()
+    for b, p in enumerate(seqs.tolist()):
+        text = ids[p, :int(lens[p])].long()
+        seen, made = torch.bincount(text, minlength=V), torch.bincount(text[int(prompts[p]):], minlength=V)
+        add = torch.zeros(V, dtype=torch.float64)
+        for i, v in zip(bias[1][p * n:(p + 1) * n].tolist(), bias[2][p * n:(p + 1) * n].tolist()):
+            add[i] = v
+        rep, freq, pres = (float(t[p].double()) for t in pen)
+        for r in range(int(cu[b]), int(cu[b + 1])):
+            a = int(cu[b])
+            mine = [int(tokens[a + j]) for j in reversed(oracle.line(parents[a:int(cu[b + 1])].tolist(), r - a))]
+            behind = [t for j, t in enumerate(mine) if int(lens[p]) + j >= int(prompts[p])]
+            count = lambda t: torch.bincount(torch.tensor(t, dtype=torch.int64), minlength=V)
+            c = (made + count(behind)).double()
+            y = x[r].double()
+            z = y - c * freq - (c > 0) * pres
+            z = torch.where(seen + count(mine) > 0, torch.where(z < 0, z * rep, z / rep), y) + add
+            # six roundings of fp32 to values of at most this size
+            big = (y.abs() + c * abs(freq) + abs(pres)) * max(rep, 1 / rep) + add.abs()
+            bound = 2.0 ** -24 * 6 * big + (z.abs() * 2.0 ** -8 * 1.01 if dtype == torch.bfloat16 else 0)
+            open_ = allowed[of[r]] if of[r] >= 0 else torch.ones(V, dtype=torch.bool)
+            assert (got[r][~open_] == -float("inf")).all()
+            assert ((got[r] - z).abs() <= bound)[open_].all()
+
 def test_adjust_logits_refuses_parts_that_are_missing():
     f, i = torch.ones(1, device="cuda"), lambda *v: torch.tensor(v, dtype=I32).cuda()
     x, words = torch.zeros(3, 40, device="cuda"), torch.zeros(1, 2, dtype=I32, device="cuda")
