@@ -76,7 +76,8 @@ __device__ __forceinline__ uint64_t seen_keys(const Params& p, const Seq& q, int
     if (p.window > 0 && pos - p.window >= q.base)
       for (uint64_t todo = bits; todo; todo &= todo - 1) {
         const int k = __ffsll(todo) - 1;
-        if (row_position(p, q, q.q_start + kv0 + k - q.base) <= pos - p.window) bits &= ~(1ull << k);
+        // (as `row_position` would say: the border lies between the first and the last row's)
+        if (p.positions[q.q_start + kv0 + k - q.base] <= pos - p.window) bits &= ~(1ull << k);
       }
     see |= bits;
   }
