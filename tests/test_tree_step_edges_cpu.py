@@ -9,6 +9,7 @@ import torch
 import oracle_tree as oracle
 from test_tree_step_cpu import acceptance, attention_inputs, rules
 from xllm_wxh_b200 import ops
+from xllm_wxh_b200.framework.step_input import TreeStep
 
 
 def test_adjust_logits_refuses_parts_that_are_missing():
@@ -147,3 +148,12 @@ def test_entry_points_have_one_signature():
         assert f" {name}(" in api and f"decltype(&{name})" in read(build_ext.TREE_HOST_SRC)
     for f in ("tree_step.cu", "attention_tree.cu", "logit_rules.cu"):
         assert '#include "tree_api.h"' in read(build_ext.CUDA_DIR, f)
+
+
+@pytest.mark.parametrize("shape", [(5,), (7,), (0,), (6, 1)])
+def test_tree_step_needs_a_token_for_every_row(shape):
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32)
+    rows = ops.step_rows(torch.ones(1, 4, dtype=torch.int32), ints(3), ints(0), ints(4), 6, 4, ints(-1, 0, 0, 1, 0, 0), max_q=4)
+    with pytest.raises(ValueError):
+        TreeStep(torch.zeros(shape, dtype=torch.int32), rows, 4, 4, 7)
+    assert TreeStep(torch.zeros(6, dtype=torch.int32), rows, 4, 4, 7).n_tokens == 6

@@ -87,6 +87,8 @@ class TreeStep:
         self.positions, self.slots, self.token_seq, self.q_cu, self.kv_lens, self.block_tables, self.tree = rows
         if self.tree is None:
             raise ValueError("rows of a tree step come from step_rows with parents")
+        if tokens.dim() != 1 or tokens.shape != self.positions.shape:          # the layers' kernels go by the tokens' number
+            raise ValueError(f"tokens of a tree step: one for each of its {self.positions.shape[0]} rows, not {tuple(tokens.shape)}")
         self.n_tokens = self.T = tokens.shape[0]
         self.n_seqs = self.B = self.kv_lens.shape[0]
         self.block_size, self.max_q, self.max_kv = block_size, max_q, max_kv
