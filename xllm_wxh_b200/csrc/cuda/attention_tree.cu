@@ -90,7 +90,8 @@ __device__ __forceinline__ uint64_t seen_keys(const Params& p, const Seq& q, int
 // scores and 4 rows x 4 NC columns of the sums, so that the multiply-adds bound it rather than shared memory; parts of the keys
 // keep the SMs busy when there are few rows, and are joined by a second kernel.  Scores, weights and sums stay fp32; only the result is
 // rounded.  8 trees of 3 to 12 rows, 14 query heads for 2 key heads of 64 columns, up to 2000 keys in fp32: 28 us (floor of the bytes 1.4),
-// two tiles of keys a CTA, of which loads through the table, latency of 4 x 2 products and the join (4 us) are all of it.
+// four tiles of keys a CTA (parts of 128 keys), of which loads through the table, latency of 4 x 2 products and the join (4 us) are all of it;
+// of the 768 CTAs that the bounds ask for, about 270 have rows and keys.
 constexpr int SR = 32, SK = 32, kSimtThreads = 128, kMaxParts = 64;
 template <int NC> struct SimtSmem {
   static constexpr int DP = 64 * NC, PITCH = DP + 4;         // 16 rows apart lie in 16 banks
@@ -1191,7 +1192,8 @@ static SimtPlan simt_plan(int B, int n_q, int n_kv, int max_q, int max_kv, int s
   SimtPlan s{};
   s.row_tiles = max(1, int((long(max_q) * (n_q / n_kv) + xl_at::SR - 1) / xl_at::SR));
   const long units = long(s.row_tiles) * n_kv * max(B, 1);
-  // parts of 64 keys at least, as many as give an SM eight CTAs if all sequences were as long as the longest
+  // parts of a multiple of 64 keys, up to eight CTAs an SM (its registers hold two or three at a time) by the bounds, as if every
+  // sequence had max_q rows and max_kv keys
   s.splits = int(max(1l, min(min(long(max_kv + 63) / 64, long(xl_at::kMaxParts)), 8l * sms / units)));
   max_kv = min(max(max_kv, 1), 0x7fffffff - 4096);
   s.part_keys = (max_kv + s.splits - 1) / s.splits;

@@ -7,7 +7,8 @@
 // Two kernels that never write the same logit, so that they may run side by side:
 //   masks    : (row, columns) - writes -inf where the mask forbids and reads no logit; bound by the bytes written.  1024 rows of 152064 fp32
 //              logits, seven of ten forbidden: 100 us alone, about 440 MB (67 us at a copy's rate).  Single open ids among forbidden
-//              ones leave sectors that are written in part, and these keep it from that rate;
+//              ones leave sectors that are written in part, which the 43 MB that it reads come from; that does not account for
+//              all of the distance;
 //   penalties: (sequence, part, rows) - counts the history's ids in a table in shared memory, so that nothing of the history has to be
 //              counted and sent by the host, and touches only the logits whose ids are in it (one sector each); forbidden ids are left
 //              to the other kernel.  Bound by the latency of a few dependent loads and of the shared-memory counts when there are few rows:

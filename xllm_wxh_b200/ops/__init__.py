@@ -426,7 +426,7 @@ def adjust_logits(logits, q_cu, seqs=None, history=None, penalties=None, tokens=
     for every id among the lens[p] first ones, made of them behind the prompt: x -= made * frequency + (made > 0) * presence, then
     x * repetition below 0, else x / repetition.  With `tokens` (int32 [S]) a row's own token and those of the rows ahead of it follow the
     lens[p] first ones: with `parents` (as in `step_rows`) its ancestors', without all earlier rows' of the sequence.  At most 256 rows a
-    sequence then; rows past max_q of a sequence are left as they are.
+    sequence then; rows past max_q of a sequence are changed by masks only.
     bias = (cu int32 [pool + 1], ids int32, values fp32): added; the last entry of an id holds.
     mask = (words int32 [masks, >= V / 32], rows int32 [S]): ids whose bit is 0 in the row's mask become -inf (rows: -1 for none).
     Ids outside the vocabulary are passed over.  Returns logits."""
